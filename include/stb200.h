@@ -40,7 +40,12 @@ enum stb_status {
 };
 
 /* Element types of weight payloads, as SafeTensors' SafeDType (io/.../SafeTensors.scala:9-16). */
-enum stb_dtype { STB_F32 = 0, STB_BF16 = 1, STB_F16 = 2 };
+enum stb_dtype {
+  STB_F32 = 0,
+  STB_BF16 = 1,
+  STB_F16 = 2,
+  STB_E4M3 = 3, /* paged caches only: 8-bit floats with a power-of-two scale per token and head */
+};
 
 /* ---------------------------------------------------------------- library / session */
 
@@ -137,6 +142,28 @@ typedef struct stb_adapter {
  * first. */
 int stb_linear_adapted(stb_session *s, uint64_t x, uint64_t w, int w_dtype, uint64_t bias,
                        const stb_adapter *adapters, int count, uint64_t y, int M, int N, int K);
+/* Adapters of many requests beside one shared projection: a pool of `slots` resident factor pairs and an
+ * adapter per row.  a: [slots][max_rank][K], b: [slots][N][max_rank], both of `dtype` (F32, BF16, F16);
+ * ranks: int32 [slots] on the device, the rank of each slot (clamped to 0 .. max_rank; the factors behind it
+ * are not read into the result); scales: Float32 [slots] on the device, LowRankAdapter.scale of each slot.
+ * The caller loads and unloads slots between calls. */
+typedef struct stb_adapter_pool {
+  uint64_t a;
+  uint64_t b;
+  uint64_t ranks;
+  uint64_t scales;
+  int dtype;
+  int slots;
+  int max_rank; /* 1 .. 256 */
+} stb_adapter_pool;
+
+/* y[m] = x[m].W^T + scales[t] * (x[m].A_t^T).B_t^T + bias with t = rows[m], int32 [M] on the device: the slot
+ * of row m, negative for a row without an adapter.  Rows may name slots in any order and repeat them; every
+ * slot's factors are read once per call for all its rows (16 rows at a time).  The shared product is stb_linear's; the thin
+ * products accumulate in Float32.  A slot >= pool->slots leaves its row without an adapter and fails the next
+ * stb_sync / stb_download.  y may not overlap an input. */
+int stb_linear_pool(stb_session *s, uint64_t x, uint64_t w, int w_dtype, uint64_t bias,
+                    const stb_adapter_pool *pool, uint64_t rows, uint64_t y, int M, int N, int K);
 /* Host-buffer form used for end-to-end measurement: copies x from host, runs stb_linear against
  * the resident weight, copies y back.  Synchronous.  Requests of up to 64 MiB of x and y keep one
  * grow-only device buffer in the session between calls (charged to its budget). */
@@ -195,6 +222,65 @@ int stb_op_cache_append(stb_session *s, uint64_t src, uint64_t cache, int batch,
 int stb_op_causal_attention(stb_session *s, uint64_t q, uint64_t k, uint64_t v, uint64_t y, int batch, int heads,
                             int tokens, int width, int kv_heads, int keys, int key_stride, int value_width,
                             int start);
+
+/* ---------------------------------------------------------------- serving several requests
+ *
+ * Operators of a batch whose rows belong to different requests, each at its own position.  No counterpart in
+ * the reference, whose caches hold one position for the whole batch.  Row indices, positions, lengths and page
+ * tables are int32 device buffers, so a captured step is replayed with new ones; the calls allocate nothing
+ * after the first of a session (which a capture must not be).  An index that names nothing (a page outside the
+ * cache, a position behind the table) is skipped, and the next stb_sync / stb_download fails with STB_ERR_CUDA.
+ * All buffers are Float32 unless stated; strides are in elements. */
+
+/* Norm and rotation of the query and key heads in one pass, for rows at positions of their own: each head h
+ * of row r becomes R(p) (h / sqrt(mean(h^2) + eps) * weight), with R the rotation of stb_op_rope at position
+ * p = positions[r].  q: heads * width values per row, rows q_row apart; k the same with kv_heads.  q_weight /
+ * k_weight: [width], or 0 to rotate without a norm.  Sums, norm, angle and rotation in double, one rounding.
+ * Rows with a negative position are padding: their outputs stay as they were.  In place (q_out == q with the
+ * same row stride, likewise k) is allowed; any other overlap is not.  width is even, at most 512. */
+int stb_op_qk_norm_rope(stb_session *s, uint64_t q, int64_t q_row, int heads, uint64_t k, int64_t k_row, int kv_heads,
+                        int width, int rows, uint64_t q_weight, uint64_t k_weight, uint64_t positions, double eps,
+                        double theta, uint64_t q_out, int64_t q_out_row, uint64_t k_out, int64_t k_out_row);
+
+/* A key/value cache handed out by pages, in buffers of the caller: keys and values (pages, kv_heads,
+ * page_size, width) of `dtype` (F32, BF16, F16 or E4M3).  E4M3 rows carry a power-of-two scale each:
+ * key_scales / value_scales (pages, kv_heads, page_size) bytes, the exponent plus 127 (0 for other types).
+ * A request's token at position p lies in slot p % page_size of page tables[sequence][p / page_size]. */
+typedef struct stb_paged_cache {
+  uint64_t keys;
+  uint64_t values;
+  uint64_t key_scales;
+  uint64_t value_scales;
+  int dtype;
+  int pages;
+  int page_size;
+  int kv_heads;
+  int width; /* 1 .. 512 */
+} stb_paged_cache;
+
+/* Writes rows of keys and values into the cache: element d of head h of row r is k[r * k_row + h * k_head + d],
+ * stored at token positions[r] of request sequences[r] (both int32 [rows]; tables int32 [batch][blocks]).
+ * F32 is copied, BF16 and F16 round to nearest even.  E4M3 takes the smallest power-of-two scale 2^e, e >= -126,
+ * that brings the row's largest finite magnitude to 448 or below (2^0 for a row of zeros) and rounds x / 2^e to
+ * nearest even; infinities and NaNs become NaN.  Rows with a negative sequence or position are padding and are
+ * skipped.  Two rows of one call may not name the same token: which of them is kept is not defined. */
+int stb_op_paged_append(stb_session *s, const stb_paged_cache *cache, uint64_t k, int64_t k_row, int64_t k_head,
+                        uint64_t v, int64_t v_row, int64_t v_head, uint64_t tables, int batch, int blocks,
+                        uint64_t sequences, uint64_t positions, int rows);
+/* The reverse: the named tokens' keys and values widened to Float32 (exact for every type), padding rows left
+ * as they were.  k_row = width with k_head = rows * width gives stb_op_causal_attention's head-major layout. */
+int stb_op_paged_read(stb_session *s, const stb_paged_cache *cache, uint64_t tables, int batch, int blocks,
+                      uint64_t sequences, uint64_t positions, int rows, uint64_t k, int64_t k_row, int64_t k_head,
+                      uint64_t v, int64_t v_row, int64_t v_head);
+/* Attention of one new token per request over its cached tokens: row b's query heads (heads * width values,
+ * rows q_row apart; head h reads key/value head h / (heads / kv_heads)) against the first lengths[b] tokens of
+ * tables[b], scores scaled by 1 / sqrt(width), softmax in Float32 with the running maximum.  lengths: int32
+ * [batch] on the device, the new token's own key included (append first).  A length of zero or below gives a
+ * row of zeros; one behind the table is cut to it.  The cache is split over its length among all SMs and the
+ * parts joined in a fixed order: the same call gives the same bits.  The session's one workspace serves all
+ * calls, in stream order: replay graphs that captured this call on one stream at a time. */
+int stb_op_paged_attention(stb_session *s, const stb_paged_cache *cache, uint64_t q, int64_t q_row, int heads,
+                           uint64_t tables, int batch, int blocks, uint64_t lengths, uint64_t y, int64_t y_row);
 
 /* ---------------------------------------------------------------- synthetic weights */
 

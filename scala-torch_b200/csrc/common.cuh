@@ -79,7 +79,9 @@ struct stb_session {
   int tp_rank = 0, tp_size = 1;
   std::atomic<uint64_t> launches{0};
   uint64_t scratch = 0, scratch_bytes = 0;  // grow-only device scratch (charged to the budget)
+  bool scratch_captured = false;            // a graph holds the scratch's address: keep it when it grows
   uint64_t err_word = 0;                    // device int: nonzero when a bounded device wait expired
+  uint64_t paged_ws = 0;                    // workspace of the paged attention (one size for all calls)
   bool closed = false;
 };
 
@@ -106,6 +108,10 @@ void fill_value(stb_session *s, uint64_t dst, int dtype, uint64_t count, float v
 uint64_t session_scratch(stb_session *s, uint64_t bytes);
 // Device error word kernels write when a bounded wait expires (allocated and zeroed on first use).
 int *session_error_word(stb_session *s);
+// Codes of the error word from here on name an index outside its table (smaller ones an expired wait).
+constexpr int DEV_BAD_INDEX = 200;
+// True while the session stream is being captured into a graph: nothing may be allocated then.
+bool capturing(stb_session *s);
 // After a stream synchronisation: throws (and clears the word) if a kernel recorded an error.
 // Completes the session stream and reports an expired device wait, reading the error word with
 // the same synchronisation.

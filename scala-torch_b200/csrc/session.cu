@@ -49,10 +49,23 @@ void session_free(stb_session *s, uint64_t ptr) {
   s->allocations.erase(it);
 }
 
+bool capturing(stb_session *s) {
+  cudaStreamCaptureStatus status;
+  STB_CUDA(cudaStreamIsCapturing(s->stream, &status));
+  return status != cudaStreamCaptureStatusNone;
+}
+
 uint64_t session_scratch(stb_session *s, uint64_t bytes) {
-  if (bytes <= s->scratch_bytes && s->scratch) return s->scratch;
+  const bool captured = capturing(s);
+  if (bytes <= s->scratch_bytes && s->scratch) {
+    s->scratch_captured |= captured;
+    return s->scratch;
+  }
+  if (captured) throw Error(STB_ERR_STATE, "the scratch cannot grow inside a capture: make a call of this size before it");
   if (s->scratch) {
-    session_free(s, s->scratch);
+    // a captured graph that replays on the old buffer keeps it (freed with the session)
+    if (!s->scratch_captured) session_free(s, s->scratch);
+    s->scratch_captured = false;
     s->scratch = 0;
     s->scratch_bytes = 0;
   }
@@ -64,6 +77,7 @@ uint64_t session_scratch(stb_session *s, uint64_t bytes) {
 
 int *session_error_word(stb_session *s) {
   if (!s->err_word) {
+    if (capturing(s)) throw Error(STB_ERR_STATE, "a session's first call of this kind cannot be captured: make one before");
     s->err_word = session_alloc(s, 256);
     STB_CUDA(cudaMemsetAsync((void *)s->err_word, 0, 256, s->stream));
   }
@@ -85,6 +99,12 @@ static void finish_error_read(stb_session *s) {
   const int code = *s->err_host;
   *s->err_host = 0;
   STB_CUDA(cudaMemset((void *)s->err_word, 0, 4));
+  if (code >= DEV_BAD_INDEX)
+    throw Error(STB_ERR_CUDA, "an index on the device is out of range (code " + std::to_string(code) + "): " +
+                                  (code == DEV_BAD_INDEX       ? "a page, sequence or position of a paged cache"
+                                   : code == DEV_BAD_INDEX + 1 ? "a cache length behind its page table"
+                                                               : "an adapter behind its pool") +
+                                  "; what it named was skipped");
   throw Error(STB_ERR_CUDA, "a device-side wait expired (code " + std::to_string(code) + "); results are invalid");
 }
 

@@ -26,7 +26,9 @@ import numpy as np
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(HERE), "libstb200.so")
 
-STB_F32, STB_BF16, STB_F16 = 0, 1, 2
+STB_F32, STB_BF16, STB_F16, STB_E4M3 = 0, 1, 2, 3
+STB_U8, STB_I32 = 4, 5  # element types of this binding's buffers alone: scale bytes and row indices
+ELEMENT_BYTES = {STB_F32: 4, STB_BF16: 2, STB_F16: 2, STB_E4M3: 1, STB_U8: 1, STB_I32: 4}
 DTYPE_NAMES = {"F32": STB_F32, "BF16": STB_BF16, "F16": STB_F16}
 STATUS = {0: "OK", 1: "INVALID", 2: "BUDGET", 3: "CUDA", 4: "NCCL", 5: "THREAD", 6: "STATE", 7: "UNSUPPORTED"}
 
@@ -47,6 +49,7 @@ _lib = None
 _p = ctypes.c_void_p
 _u64 = ctypes.c_uint64
 _i = ctypes.c_int
+_i64 = ctypes.c_int64
 _pp = ctypes.POINTER(ctypes.c_void_p)
 
 
@@ -99,6 +102,12 @@ def _declare(L):
         "stb_op_embedding": (_i, [_p, _u64, _i, ctypes.c_int64, _i, _p, _u64, _u64]),
         "stb_op_cache_append": (_i, [_p, _u64, _u64, _i, _i, _i, _i, _i, _i]),
         "stb_op_causal_attention": (_i, [_p, _u64, _u64, _u64, _u64] + [_i] * 9),
+        "stb_linear_pool": (_i, [_p, _u64, _u64, _i, _u64, _p, _u64, _u64, _i, _i, _i]),
+        "stb_op_qk_norm_rope": (_i, [_p, _u64, _i64, _i, _u64, _i64, _i, _i, _i, _u64, _u64, _u64, ctypes.c_double,
+                                     ctypes.c_double, _u64, _i64, _u64, _i64]),
+        "stb_op_paged_append": (_i, [_p, _p, _u64, _i64, _i64, _u64, _i64, _i64, _u64, _i, _i, _u64, _u64, _i]),
+        "stb_op_paged_read": (_i, [_p, _p, _u64, _i, _i, _u64, _u64, _i, _u64, _i64, _i64, _u64, _i64, _i64]),
+        "stb_op_paged_attention": (_i, [_p, _p, _u64, _i64, _i, _u64, _i, _i, _u64, _u64, _i64]),
         "stb_nccl_unique_id": (_i, [_p]),
         "stb_session_init_tp": (_i, [_p, _i, _i, _p]),
         "stb_allreduce_sum_f32": (_i, [_p, _u64, _u64]),
@@ -144,6 +153,8 @@ class DeviceTensor:
     _alive: list = field(default_factory=lambda: [True])
     # handles on one allocation (reshape views share it, CudaSession.scala:95-101); freed at zero
     _refs: list = field(default_factory=lambda: [1])
+    # elements between entries of axis 0 in a view of some columns (B200Session.columns); 0: packed
+    row_stride: int = 0
 
     @property
     def numel(self) -> int:
@@ -160,6 +171,19 @@ class StbAdapter(ctypes.Structure):
     """stb_adapter (include/stb200.h)."""
     _fields_ = [("a", ctypes.c_uint64), ("b", ctypes.c_uint64), ("rank", ctypes.c_int), ("scale", ctypes.c_float),
                 ("scoped", ctypes.c_int), ("multiplier", ctypes.c_float)]
+
+
+class StbAdapterPool(ctypes.Structure):
+    """stb_adapter_pool (include/stb200.h)."""
+    _fields_ = [("a", ctypes.c_uint64), ("b", ctypes.c_uint64), ("ranks", ctypes.c_uint64), ("scales", ctypes.c_uint64),
+                ("dtype", ctypes.c_int), ("slots", ctypes.c_int), ("max_rank", ctypes.c_int)]
+
+
+class StbPagedCache(ctypes.Structure):
+    """stb_paged_cache (include/stb200.h)."""
+    _fields_ = [("keys", ctypes.c_uint64), ("values", ctypes.c_uint64), ("key_scales", ctypes.c_uint64),
+                ("value_scales", ctypes.c_uint64), ("dtype", ctypes.c_int), ("pages", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("kv_heads", ctypes.c_int), ("width", ctypes.c_int)]
 
 
 class LowRankAdapter:
@@ -235,7 +259,8 @@ class B200Session:
         self._check()
         shape = tuple(int(d) for d in shape)
         require(all(d >= 0 for d in shape), "negative dimension")
-        esz = 4 if dtype == STB_F32 else 2
+        require(dtype in ELEMENT_BYTES, "unknown element type")
+        esz = ELEMENT_BYTES[dtype]
         n = 1
         for d in shape:
             n *= d
@@ -258,12 +283,60 @@ class B200Session:
         require(isinstance(t, DeviceTensor) and t.session is self, "tensor belongs to another session")
         if not t._alive[0]:
             raise IllegalStateException("validate", 6, "tensor was released")
+        require(t.row_stride == 0, "operation takes packed tensors, not a view of columns")
 
     def shape(self, t: DeviceTensor) -> tuple:
         self._validate(t)
         return t.shape
 
+    def wrap(self, address: int, shape, dtype: int = STB_F32) -> DeviceTensor:
+        """A tensor over device memory that the caller owns (another library's buffer, a slice of an arena): never
+        freed here and not charged to the budget.  The caller orders its own work on that memory with the
+        session's stream and keeps it alive."""
+        self._check()
+        shape = tuple(int(d) for d in shape)
+        require(dtype in ELEMENT_BYTES, "unknown element type")
+        require(all(d >= 0 for d in shape), "negative dimension")
+        nbytes = math.prod(shape) * ELEMENT_BYTES[dtype]
+        require(address % ELEMENT_BYTES[dtype] == 0 and (address != 0 or nbytes == 0), "null or misaligned memory")
+        return DeviceTensor(self, address, shape, dtype, nbytes, owner=False)
+
+    def columns(self, t: DeviceTensor, begin: int, shape) -> DeviceTensor:
+        """A view of some columns of a matrix: entry r of axis 0 is t[r, begin : begin + prod(shape)] in `shape` --
+        the query, key or value heads inside the rows of a fused projection.  Released like a reshape view; taken
+        by the operators whose rows may lie apart (qk_norm_rope, a paged cache's append, read and attend)."""
+        self._validate(t)
+        shape = tuple(int(d) for d in shape)
+        require(len(t.shape) == 2 and not t.transposed_weight and all(d > 0 for d in shape), "columns of a matrix")
+        require(0 <= begin and begin + math.prod(shape) <= t.shape[1], "columns outside the matrix")
+        t._refs[0] += 1
+        return DeviceTensor(self, t.address + begin * ELEMENT_BYTES[t.dtype], (t.shape[0],) + shape, t.dtype, 0,
+                            owner=t.owner, _refs=t._refs, row_stride=t.shape[1])
+
+    def as_weight(self, t: DeviceTensor) -> DeviceTensor:
+        """A view of a resident (out,in) matrix as the weight that matmul and the Linear forms take."""
+        require(len(t.shape) == 2 and t.dtype in (STB_F32, STB_BF16, STB_F16) and not t.transposed_weight,
+                "Linear weight must have shape (out, in)")
+        w = self.reshape(t, t.shape)
+        w.shape, w.transposed_weight = (t.shape[1], t.shape[0]), True
+        return w
+
     # -- transfers
+    def upload_ints(self, source) -> DeviceTensor:
+        """Row indices, positions, lengths or page tables: int32 on the device.  Values outside Int are rejected."""
+        a = np.asarray(source)
+        require(a.dtype.kind in "iu" or a.size == 0, "indices must be whole numbers")
+        require(a.size == 0 or (int(a.min()) >= -(1 << 31) and int(a.max()) < 1 << 31), "index exceeds Int")
+        a = np.ascontiguousarray(a, np.int32)
+        t = self.allocate(a.shape, STB_I32)
+        try:
+            if a.size:
+                call("stb_upload", self.handle, a.ctypes.data, a.nbytes, t.address)
+        except Exception:
+            self.release(t)
+            raise
+        return t
+
     def upload(self, source: np.ndarray) -> DeviceTensor:
         """FloatBackend.upload of a Float32 tensor (packed row-major)."""
         a = np.ascontiguousarray(source, dtype=np.float32)
@@ -539,6 +612,118 @@ class B200Session:
         self._check()
         return B200AttentionCache(self, batch_size, heads, capacity, key_width, value_width, max_bytes)
 
+    # -- several requests in one batch
+    def _rows_of(self, t: DeviceTensor, dtype: int = STB_F32) -> int:
+        """Checks a tensor whose rows may lie apart; elements between its rows."""
+        if t.__class__ is not DeviceTensor or t.session is not self:
+            raise IllegalArgumentException("tensor belongs to another session")
+        if not t._alive[0]:
+            raise IllegalStateException("validate", 6, "tensor was released")
+        if t.dtype != dtype or t.transposed_weight:
+            raise IllegalArgumentException("operation takes Float32 rows and int32 indices")
+        if t.row_stride:
+            return t.row_stride
+        n = 1
+        for d in t.shape[1:]:
+            n *= d
+        return n
+
+    def _outs(self, *shapes):
+        """Float32 outputs of an operator that has several; none is left behind where one does not fit."""
+        made = []
+        try:
+            for shape in shapes:
+                made.append(self._out(shape))
+        except Exception:
+            for t in made:
+                self.release(t)
+            raise
+        return tuple(made)
+
+    def _indices(self, t: DeviceTensor, shape) -> int:
+        """Checks a packed int32 index tensor; its address."""
+        self._rows_of(t, STB_I32)
+        if t.shape != shape or t.row_stride:
+            raise IllegalArgumentException("index shape mismatch")
+        return t.address
+
+    def qk_norm_rope(self, query: DeviceTensor, key: DeviceTensor, query_weight: DeviceTensor | None,
+                     key_weight: DeviceTensor | None, positions: DeviceTensor, epsilon: float = 1e-6,
+                     theta: float = 10000.0, out=None):
+        """RMSNorm of each query and key head (no norm where the weight is None) and rotary embedding of its row's
+        own position, in one pass: query (rows, heads, width), key (rows, kv_heads, width), positions int32 (rows,).
+        query and key may be columns of a fused projection.  Returns (query, key); out = (query, key) tensors to
+        write, which may be the inputs themselves.  A row with a negative position is padding and left as it is."""
+        self._check()
+        q_row, k_row = self._rows_of(query), self._rows_of(key)
+        if len(query.shape) != 3 or len(key.shape) != 3 or query.shape[0] != key.shape[0] or query.shape[2] != key.shape[2]:
+            raise IllegalArgumentException("query and key heads must have shapes (rows, heads, width)")
+        rows, heads, width = query.shape
+        for w in (query_weight, key_weight):
+            if w is not None:
+                self._rows_of(w)
+                if w.shape != (width,):
+                    raise IllegalArgumentException("invalid RMSNorm shapes")
+        at = self._indices(positions, (rows,))
+        made = out is None
+        if made:
+            out = self._outs(query.shape, key.shape)
+        yq, yk = out
+        yq_row, yk_row = self._rows_of(yq), self._rows_of(yk)
+        if yq.shape != query.shape or yk.shape != key.shape:
+            raise IllegalArgumentException("output shape mismatch")
+        try:
+            call("stb_op_qk_norm_rope", self.handle, query.address, q_row, heads, key.address, k_row, key.shape[1], width,
+                 rows, query_weight.address if query_weight is not None else 0,
+                 key_weight.address if key_weight is not None else 0, at, epsilon, theta, yq.address, yq_row, yk.address,
+                 yk_row)
+        except Exception:
+            if made:
+                self.release(yq)
+                self.release(yk)
+            raise
+        return out
+
+    def paged_cache(self, keys: DeviceTensor, values: DeviceTensor, key_scales: DeviceTensor | None = None,
+                    value_scales: DeviceTensor | None = None) -> "B200PagedCache":
+        """A paged cache over buffers of the caller: keys and values (pages, kv_heads, page_size, width) in Float32,
+        BF16, F16 or E4M3, the last with a scale byte per (page, head, slot)."""
+        return B200PagedCache(self, keys, values, key_scales, value_scales)
+
+    def adapter_pool(self, a: DeviceTensor, b: DeviceTensor, ranks: DeviceTensor, scales: DeviceTensor) -> "AdapterPool":
+        """Low-rank adapters that the rows of one call choose from (linear_adapted): a (slots, max_rank, in),
+        b (slots, out, max_rank), ranks int32 (slots,), scales Float32 (slots,)."""
+        return AdapterPool(self, a, b, ranks, scales)
+
+    def linear_adapted(self, x: DeviceTensor, weight: DeviceTensor, pool: "AdapterPool", rows: DeviceTensor,
+                       bias: DeviceTensor | None = None, out: DeviceTensor | None = None) -> DeviceTensor:
+        """x.W^T + scale (x.A^T).B^T + bias with row m's adapter rows[m] of the pool (int32; negative: none)."""
+        self._validate(x)
+        self._validate(weight)
+        require(weight.transposed_weight, "weight must be a resident (out,in) weight")
+        require(x.dtype == STB_F32 and not x.transposed_weight, "activations must be Float32")
+        require(len(x.shape) == 2 and weight.shape[0] == x.shape[1], "Linear shape mismatch")
+        M, K = x.shape
+        N = weight.shape[1]
+        require(pool.session is self and pool.inner == K and pool.out == N, "Linear adapter shape mismatch")
+        pool.check()
+        if bias is not None:
+            self._validate(bias)
+            require(bias.shape == (N,) and bias.dtype == STB_F32, "Linear bias shape mismatch")
+        at = self._indices(rows, (M,))
+        y = self._out((M, N)) if out is None else out
+        if out is not None:
+            self._validate(y)
+            require(y.shape == (M, N) and y.dtype == STB_F32 and not y.transposed_weight, "output shape mismatch")
+        try:
+            call("stb_linear_pool", self.handle, x.address, weight.address, weight.dtype,
+                 bias.address if bias is not None else 0, pool.ref, at, y.address, M, N, K)
+        except Exception:
+            if out is None:
+                self.release(y)
+            raise
+        return y
+
     # -- tensor parallel
     @staticmethod
     def nccl_unique_id() -> bytes:
@@ -623,3 +808,132 @@ class B200AttentionCache:
             self._closed = True
             self.session.release(self.keys)
             self.session.release(self.values)
+
+
+class AdapterPool:
+    """Resident factors of several low-rank adapters, one slot each (stb_adapter_pool).  Slots are loaded, replaced
+    and unloaded by writing the tensors between calls; a slot uses the first ranks[slot] rows of its factors."""
+
+    def __init__(self, session: B200Session, a: DeviceTensor, b: DeviceTensor, ranks: DeviceTensor, scales: DeviceTensor):
+        for t in (a, b, ranks, scales):
+            session._validate(t)
+        require(a.dtype in (STB_F32, STB_BF16, STB_F16) and a.dtype == b.dtype, "adapter factors must share one type")
+        require(len(a.shape) == 3 and len(b.shape) == 3 and min(a.shape + b.shape) > 0 and a.shape[0] == b.shape[0]
+                and a.shape[1] == b.shape[2] and a.shape[1] <= 256, "invalid adapter factor dimensions")
+        require(ranks.shape == (a.shape[0],) and ranks.dtype == STB_I32, "adapter ranks must be int32 (slots,)")
+        require(scales.shape == (a.shape[0],) and scales.dtype == STB_F32, "adapter scales must be Float32 (slots,)")
+        self.session, self.tensors = session, (a, b, ranks, scales)
+        self.slots, self.max_rank, self.inner = a.shape
+        self.out = b.shape[1]
+        self._struct = StbAdapterPool(a.address, b.address, ranks.address, scales.address, a.dtype, self.slots, self.max_rank)
+        self.ref = ctypes.byref(self._struct)
+
+    def check(self) -> None:
+        for t in self.tensors:
+            if not t._alive[0]:
+                raise IllegalStateException("adapter pool", 6, "tensor was released")
+
+
+class B200PagedCache:
+    """Keys and values of several requests in pages (stb_paged_cache), each request at its own position: the token at
+    position p of request r lies in page tables[r, p // page_size].  Beside B200AttentionCache, whose one written
+    prefix serves the whole batch in Float32.  The tensors are the caller's; tables (batch, blocks), sequences, positions
+    and lengths are int32 device tensors, so that a captured step can be replayed with new ones."""
+
+    def __init__(self, session: B200Session, keys: DeviceTensor, values: DeviceTensor, key_scales=None, value_scales=None):
+        scaled = [t for t in (key_scales, value_scales) if t is not None]
+        for t in (keys, values, *scaled):
+            session._validate(t)
+        require(keys.dtype in (STB_F32, STB_BF16, STB_F16, STB_E4M3) and keys.dtype == values.dtype, "paged cache type")
+        require(len(keys.shape) == 4 and min(keys.shape) > 0 and keys.shape == values.shape and keys.shape[3] <= 512,
+                "invalid paged cache dimensions")
+        require(len(scaled) == (2 if keys.dtype == STB_E4M3 else 0), "an E4M3 cache has scales, the other types have none")
+        require(all(t.shape == keys.shape[:3] and t.dtype == STB_U8 for t in scaled),
+                "paged cache scales must be bytes (pages, kv_heads, page_size)")
+        self.session, self.tensors = session, (keys, values, *scaled)
+        self.pages, self.kv_heads, self.page_size, self.width = keys.shape
+        self.dtype = keys.dtype
+        self._struct = StbPagedCache(keys.address, values.address, *([t.address for t in scaled] or [0, 0]), keys.dtype,
+                                     self.pages, self.page_size, self.kv_heads, self.width)
+        self.ref = ctypes.byref(self._struct)
+
+    def _tables(self, tables: DeviceTensor):
+        s = self.session
+        s._check()
+        for t in self.tensors:
+            if not t._alive[0]:
+                raise IllegalStateException("paged cache", 6, "tensor was released")
+        s._rows_of(tables, STB_I32)
+        if len(tables.shape) != 2 or tables.row_stride:
+            raise IllegalArgumentException("page tables must have shape (batch, blocks)")
+        return tables.shape
+
+    def _rows(self, t: DeviceTensor, rows: int, heads_first: bool = False):
+        """(row, head) strides of a (rows, kv_heads, width) or (kv_heads, rows, width) tensor."""
+        stride = self.session._rows_of(t)
+        if t.shape != ((self.kv_heads, rows, self.width) if heads_first else (rows, self.kv_heads, self.width)):
+            raise IllegalArgumentException("paged rows must have shape (rows, kv_heads, width)")
+        return (self.width, stride) if heads_first else (stride, self.width)
+
+    def append(self, key: DeviceTensor, value: DeviceTensor, tables: DeviceTensor, sequences: DeviceTensor,
+               positions: DeviceTensor) -> None:
+        """Writes key and value rows (rows, kv_heads, width) at positions[r] of request sequences[r], rounded or quantised
+        to the cache's type.  Rows with a negative sequence or position are padding; no two rows may name one token."""
+        batch, blocks = self._tables(tables)
+        s = self.session
+        rows = sequences.shape[0] if len(sequences.shape) == 1 else -1
+        seq, pos = s._indices(sequences, (rows,)), s._indices(positions, (rows,))
+        (kr, kh), (vr, vh) = self._rows(key, rows), self._rows(value, rows)
+        call("stb_op_paged_append", s.handle, self.ref, key.address, kr, kh, value.address, vr, vh, tables.address, batch,
+             blocks, seq, pos, rows)
+
+    def read(self, tables: DeviceTensor, sequences: DeviceTensor, positions: DeviceTensor, out=None,
+             heads_first: bool = False):
+        """(key, value) of the named tokens in Float32, (rows, kv_heads, width), or (kv_heads, rows, width) with
+        heads_first -- causal_attention's layout for one request.  With `out` the two tensors are written, padding
+        rows left as they are; without it padding rows come back as zeros."""
+        batch, blocks = self._tables(tables)
+        s = self.session
+        rows = sequences.shape[0] if len(sequences.shape) == 1 else -1
+        seq, pos = s._indices(sequences, (rows,)), s._indices(positions, (rows,))
+        made = out is None
+        if made:
+            shape = (self.kv_heads, rows, self.width) if heads_first else (rows, self.kv_heads, self.width)
+            out = s._outs(shape, shape)
+        try:
+            if made and out[0].numel:  # padding rows of a fresh output
+                for t in out:
+                    call("stb_fill_value", s.handle, t.address, STB_F32, t.numel, 0.0)
+            (kr, kh), (vr, vh) = (self._rows(t, rows, heads_first) for t in out)
+            call("stb_op_paged_read", s.handle, self.ref, tables.address, batch, blocks, seq, pos, rows, out[0].address, kr,
+                 kh, out[1].address, vr, vh)
+        except Exception:
+            if made:
+                s.release(out[0])
+                s.release(out[1])
+            raise
+        return out
+
+    def attend(self, query: DeviceTensor, tables: DeviceTensor, lengths: DeviceTensor,
+               out: DeviceTensor | None = None) -> DeviceTensor:
+        """Attention of one new token per request: query (batch, heads, width) against the first lengths[b] tokens of
+        tables[b] (the new token's own key among them: append first).  A length of zero gives a row of zeros."""
+        batch, blocks = self._tables(tables)
+        s = self.session
+        q_row = s._rows_of(query)
+        shape = query.shape
+        if len(shape) != 3 or shape[0] != batch or shape[2] != self.width or shape[1] % self.kv_heads or not shape[1]:
+            raise IllegalArgumentException("paged attention query must have shape (batch, heads, width)")
+        at = s._indices(lengths, (batch,))
+        y = s._out(shape) if out is None else out
+        y_row = s._rows_of(y)
+        if y.shape != shape:
+            raise IllegalArgumentException("output shape mismatch")
+        try:
+            call("stb_op_paged_attention", s.handle, self.ref, query.address, q_row, shape[1], tables.address, batch, blocks,
+                 at, y.address, y_row)
+        except Exception:
+            if out is None:
+                s.release(y)
+            raise
+        return y
