@@ -1,11 +1,35 @@
 // Attention of one new token per request over its paged cache (stb_op_paged_attention):
 //   y[b, h] = sum_j softmax_j(q[b, h] . k_j / sqrt(width)) v_j,   j < lengths[b],  h on kv head h / group,
-// zeros where lengths[b] <= 0.  Softmax with the running maximum and sum, everything in Float32.
+// zeros where lengths[b] <= 0.
+//
+// What bounds it: every cached byte is read once, 4 * group flops per element: HBM, as long as the arithmetic keeps
+// out of the way.  With 8 query heads on a kv head, Float32 FMAs would take 8 flops per BF16 byte (52 TFLOP/s at the
+// copy rate of 6.5 TB/s, near the SM's FP32 peak) and twice that for E4M3, so both products run on the tensor
+// cores (mma.sync: a 16-row operand is all there is to multiply, the 128-row tiles of tcgen05 would be padding), with
+// Float32 accuracy kept by splitting the Float32 side into terms that the products take exactly:
+//   * BF16 cache: q and p in three BF16 terms (24 bits);
+//   * F16 and E4M3 cache (E4M3 widens to F16 exactly): two F16 terms (22 bits), after a power of two that puts the
+//     largest q of a head at 2^12 and p at 2^7 .. 2^15, so that F16's range costs nothing;
+//   * F32 cache: both sides in two TF32 terms.
+// The tensor core truncates its sums, so chains are kept short (at most 8 products) and joined by Float32 additions.
+//
+// Work: items (request, kv head, chunk of 8 query heads) are cut into tiles of 16 keys, all tiles in one line; each
+// block takes an equal stretch of the line and each of its warps an equal stretch of that (lengths are known on
+// the device only: a captured step is replayed with new ones).  A warp runs alone over its stretch, across items,
+// with a ring of cp.async stages of its own: no block barrier until its end.  Row g of a 16-row operand is
+// query head g in its first term, row g + 8 the same head's second term, so a lane (g, t) of a product's result
+// holds head g at keys (dimensions) 2t, 2t + 1 and its lower terms: the running maximum needs two shuffles, and
+// weights become the next product's operand without moving.  Items that a block covers only in part are joined
+// first among its warps in shared memory, then by the last block to arrive, always in the order of the keys.
+#include <algorithm>
 #include <cmath>
+#include <mutex>
 
 #include "paged.cuh"
+#include "tc_common.cuh"
 
 namespace stb {
+
 namespace {
 
 struct AttendArgs {
@@ -13,22 +37,27 @@ struct AttendArgs {
   float *y;
   int64_t q_row, y_row;
   const int *lengths;
-  int heads, group;
-  float scale_log2;  // log2(e) / sqrt(width)
+  int heads, group, batch, first;  // requests first .. first + batch - 1 of the call
+  float scale_log2;                // log2(e) / sqrt(width)
+  float *pieces;                   // per block: two of its own, then one per warp
+  int *arrived;                    // per block, zero between calls
 };
 
 __device__ __forceinline__ int attend_length(const PagedView &c, const AttendArgs &a, int b) {
   const int n = a.lengths[b], most = c.blocks * c.page_size;
   if (n > most) *c.err = DEV_BAD_INDEX + 1;
-  return min(n, most);
+  return max(0, min(n, most));
 }
 
-// One block per (request, query head): its warps take keys in turn, a lane every 32nd dimension.
+// ------------------------------------------------------------------ any width, alignment and type
+
+// One block per (request, query head): its warps take keys in turn, a lane every 32nd dimension, Float32 FMAs.
+// For caches whose rows are no multiple of 16 bytes or wider than 256.
 template <int DTYPE>
-__global__ void __launch_bounds__(256) paged_attention_kernel(const PagedView c, const AttendArgs a) {
+__global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedView c, const AttendArgs a) {
   constexpr int W = 8, D = 16;  // warps; dimensions of a lane (width <= 512)
   __shared__ float s_max[W], s_sum[W], s_acc[W][512];
-  const int b = blockIdx.y, h = blockIdx.x, kvh = h / a.group;
+  const int b = a.first + blockIdx.y, h = blockIdx.x, kvh = h / a.group;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n = attend_length(c, a, b);
   float q[D], acc[D];
@@ -79,6 +108,648 @@ __global__ void __launch_bounds__(256) paged_attention_kernel(const PagedView c,
   }
 }
 
+// ------------------------------------------------------------------ rows of whole 16-byte chunks, width <= 256
+
+constexpr int TK = 16;             // keys of a tile
+constexpr int MAX_GRID = 160;
+constexpr int BLOCK_PIECES = 20800;  // floats of a block's pieces, at most: (2 + warps) of 8 heads x (width + 4)
+constexpr int MAX_BATCH = 1024;    // requests of one launch (their prefix sums lie in shared memory)
+constexpr float LAZY = 8.0f;       // a maximum moves only when a score passes it by 2^8
+constexpr float P_SHIFT = 128.0f;  // F16 weights times 2^7: at most 2^15, and 2^-32 apart at their lowest
+
+template <int DTYPE, int WP>
+struct Shape {
+  static constexpr int ESZ = DTYPE == STB_F32 ? 4 : (DTYPE == STB_E4M3 ? 1 : 2);
+  static constexpr int ROW = WP * ESZ;            // bytes of a key's row in shared memory
+  static constexpr int CHUNKS = ROW / 16;
+  static constexpr int TILE = 2 * TK * ROW;       // keys and values of a tile
+  // Warps and stages that fill about 192 KB: at least two stages in flight per warp, 128 KB per SM.
+  static constexpr int WARPS = TILE <= 2048 ? 16 : (TILE <= 8192 ? 8 : (TILE <= 16384 ? 4 : 2));
+  static constexpr int STAGES = 196608 / (WARPS * TILE) < 6 ? 196608 / (WARPS * TILE) : 6;
+  static constexpr int META = 64;                 // per stage: valid mask, scale bytes
+  static constexpr int THREADS = WARPS * 32;
+  static constexpr int RING = WARPS * STAGES * TILE;
+  static constexpr int PART = 8 * (WP + 4);       // floats of a partial result: per head max, weight max, sum, -, values
+  static constexpr int SMEM = RING + WARPS * STAGES * META + (MAX_BATCH + 1) * 8 + 1024;
+  static_assert(STAGES >= 3 && SMEM <= 232448, "shared memory per block");
+  static_assert(STAGES * TILE >= PART * 4, "a warp's last part reuses its ring");
+  static_assert((2 + WARPS) * PART <= BLOCK_PIECES, "workspace");
+};
+
+__device__ __forceinline__ uint32_t shared_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// 16 bytes of global memory to shared memory; `live` false writes zeros instead.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void load_matrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void load_matrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+// c += a . b, 16 x 8 results; a 16 x 16 (BF16, F16) or 16 x 8 (F32 taken as TF32).
+template <int DTYPE>
+__device__ __forceinline__ void product(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  if constexpr (DTYPE == STB_F32)
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else if constexpr (DTYPE == STB_BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// x = hi + lo in two TF32 values: hi rounded to 11 bits (half a step up, then cut), lo the exact rest, rounded likewise.
+__device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  lo = (__float_as_uint(x - __uint_as_float(hi)) + 0x1000u) & 0xffffe000u;
+}
+
+__device__ __forceinline__ uint32_t pack2(uint16_t lo, uint16_t hi) { return (uint32_t)lo | ((uint32_t)hi << 16); }
+
+// Three BF16 terms of two finite weights >= 0: rounded, rest rounded, rest rounded (rests are exact).
+__device__ __forceinline__ void split3_pair(float x, float y, uint32_t (&t)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; i++) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    t[i] = *reinterpret_cast<const uint32_t *>(&h);
+    x -= __uint_as_float(t[i] << 16);
+    y -= __uint_as_float(t[i] & 0xffff0000u);
+  }
+}
+// Two F16 terms.
+__device__ __forceinline__ void split2_pair(float x, float y, uint32_t (&t)[2]) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  t[0] = *reinterpret_cast<const uint32_t *>(&h);
+  t[1] = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+__device__ __forceinline__ uint32_t widen_pair(uint32_t two_bytes) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two_bytes, __NV_E4M3);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Shared-memory address of 16-byte chunk `chunk` of row `row`: 128-byte lines whose chunks are XORed with the line, so
+// that the same chunk of eight neighbouring rows lies in eight different places of a line (no bank conflict).
+template <int ROW>
+__device__ __forceinline__ uint32_t chunk_at(uint32_t base, int row, int chunk) {
+  if constexpr (ROW >= 128) return base + row * ROW + ((chunk ^ (row & 7)) << 4);
+  const int line = row * ROW / 128, at = (row * ROW % 128) / 16 + chunk;
+  return base + line * 128 + ((at ^ (line & 7)) << 4);
+}
+
+// A place on the line of tiles.
+struct Cursor {
+  int b, item, tile, tiles, n;  // request, its item (kv head * chunks + chunk), tile of the item, tiles and keys of the request
+};
+
+template <int DTYPE, int WP>
+__global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_kernel(const PagedView c, const AttendArgs a) {
+  using S = Shape<DTYPE, WP>;
+  constexpr int STEP = DTYPE == STB_F32 ? 8 : 16;   // dimensions of one product
+  constexpr int STEPS = WP / STEP, NT = WP / 8;
+  constexpr int QREGS = DTYPE == STB_BF16 ? 6 : 4;  // operand registers of q per step
+  constexpr bool HALF = DTYPE == STB_F16 || DTYPE == STB_E4M3, SCALED = DTYPE == STB_E4M3;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t *s_meta = smem + S::RING;
+  long long *s_start = (long long *)(s_meta + S::WARPS * S::STAGES * S::META);  // tiles before request b, per item of it
+  __shared__ long long s_scan[S::WARPS];
+  __shared__ float s_weight[MAX_GRID][8];  // of the parts that are joined
+  __shared__ float s_head[8][3];           // joined maxima and sum per head
+  __shared__ int s_part[2 * S::WARPS][4];  // a warp's first and last part: request (or -1), item, whether it starts / ends it
+  __shared__ int s_last;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int chunks_of = (a.group + 7) / 8, items = c.kv_heads * chunks_of;
+  const int row_chunks = c.width * S::ESZ / 16;
+
+  // Prefix sums of the requests' tiles, and zeros for the empty ones.
+  {
+    const int per = (a.batch + S::THREADS - 1) / S::THREADS, b0 = threadIdx.x * per;
+    long long own = 0;
+    for (int b = b0; b < min(a.batch, b0 + per); b++) own += (attend_length(c, a, a.first + b) + TK - 1) / TK;
+    long long before = own;
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, before, off);
+      if (lane >= off) before += v;
+    }
+    if (lane == 31) s_scan[warp] = before;
+    __syncthreads();
+    before -= own;
+    for (int w = 0; w < warp; w++) before += s_scan[w];
+    for (int b = b0; b < min(a.batch, b0 + per); b++) {
+      s_start[b] = before;
+      before += (attend_length(c, a, a.first + b) + TK - 1) / TK;
+    }
+    if (threadIdx.x == 0) {
+      long long all = 0;
+      for (int w = 0; w < S::WARPS; w++) all += s_scan[w];
+      s_start[a.batch] = all;
+    }
+    for (int i = threadIdx.x; i < 2 * S::WARPS; i += S::THREADS) s_part[i][0] = -1;
+    if (c.width != WP)  // chunks behind the row are read as zeros and never written
+      for (int i = threadIdx.x; i < S::RING / 16; i += S::THREADS) ((uint4 *)smem)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+  }
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
+    if (s_start[b] == s_start[b + 1])
+      for (int i = threadIdx.x; i < a.heads * c.width; i += S::THREADS) a.y[(a.first + b) * a.y_row + i] = 0.0f;
+
+  const long long total = s_start[a.batch] * items;
+  const int grid = (int)min((long long)gridDim.x, (total + S::WARPS - 1) / S::WARPS);
+  if ((int)blockIdx.x >= grid) return;
+  const long long block0 = total * blockIdx.x / grid, block1 = total * (blockIdx.x + 1) / grid;
+  const long long t0 = block0 + (block1 - block0) * warp / S::WARPS, t1 = block0 + (block1 - block0) * (warp + 1) / S::WARPS;
+
+  const uint32_t ring = shared_u32(smem) + warp * S::STAGES * S::TILE;
+  uint8_t *meta = s_meta + warp * S::STAGES * S::META;
+
+  Cursor load, use;
+  {
+    int lo = 0, hi = a.batch - 1;  // the last request that starts at or before t0 (the empty ones before it share its start)
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (s_start[mid] * items <= t0) lo = mid;
+      else hi = mid - 1;
+    }
+    load.b = lo;
+    load.tiles = (int)(s_start[lo + 1] - s_start[lo]);
+    load.n = attend_length(c, a, a.first + lo);
+    const long long in = t0 - s_start[lo] * items;
+    load.item = load.tiles ? (int)(in / load.tiles) : 0;
+    load.tile = load.tiles ? (int)(in % load.tiles) : 0;
+    use = load;
+  }
+  auto advance = [&](Cursor &k) {
+    if (++k.tile < k.tiles) return;
+    k.tile = 0;
+    if (++k.item < items) return;
+    k.item = 0;
+    do k.b++;
+    while (k.b < a.batch && s_start[k.b] == s_start[k.b + 1]);
+    if (k.b < a.batch) {
+      k.tiles = (int)(s_start[k.b + 1] - s_start[k.b]);
+      k.n = attend_length(c, a, a.first + k.b);
+    }
+  };
+  const int todo = (int)(t1 - t0);
+  // Page of this lane's key (lane & 15) in the tile at `load`, one tile ahead of its copies.
+  auto page_ahead = [&](bool live) {
+    const int key = load.tile * TK + (lane & 15);
+    if (!live || key >= load.n) return -2;
+    return c.tables[(size_t)(a.first + load.b) * c.blocks + key / c.page_size];
+  };
+  int issued = 0, page = page_ahead(todo > 0);
+  auto issue = [&](int stage) {
+    if (issued < todo) {
+      const int key = load.tile * TK + (lane & 15), kvh = load.item / chunks_of;
+      bool live = page != -2;
+      if (live && (unsigned)page >= (unsigned)c.pages) {
+        *c.err = DEV_BAD_INDEX;
+        live = false;
+      }
+      const int at = live ? (int)paged_row(c, page, kvh, key % c.page_size) : 0;
+      const uint32_t mask = __ballot_sync(0xffffffffu, live) & 0xffffu;
+      uint8_t *m = meta + stage * S::META;
+      if (lane == 0) *(uint32_t *)m = mask;
+      if (SCALED) m[16 + lane] = live ? c.scale[lane >> 4][at] : (uint8_t)127;
+      const uint32_t dst = ring + stage * S::TILE;
+      constexpr int PER = 32 / S::CHUNKS > 0 ? 32 / S::CHUNKS : 1;  // rows of one copy of the warp
+      constexpr int TIMES = S::CHUNKS > 32 ? S::CHUNKS / 32 : 1;
+#pragma unroll
+      for (int side = 0; side < 2; side++)
+#pragma unroll
+        for (int r0 = 0; r0 < TK; r0 += PER) {
+          const int r = r0 + (TIMES == 1 ? lane / S::CHUNKS : 0);
+          const int from = __shfl_sync(0xffffffffu, at, r);
+#pragma unroll
+          for (int i = 0; i < TIMES; i++) {
+            const int chunk = TIMES == 1 ? lane % S::CHUNKS : i * 32 + lane;
+            if (chunk < row_chunks)
+              copy16(chunk_at<S::ROW>(dst + side * TK * S::ROW, r, chunk),
+                     (const uint8_t *)c.kv[side] + ((size_t)from * row_chunks + chunk) * 16, mask >> r & 1);
+          }
+        }
+      advance(load);
+      issued++;
+      page = page_ahead(issued < todo);
+    }
+    copy_commit();
+  };
+
+  uint32_t q[STEPS][QREGS];
+  float o[NT][2], m1 = -INFINITY, m2 = -INFINITY, sum = 0.0f, unscale = 1.0f;
+
+  // q of the item at `use` into operand registers, scaled by log2(e) / sqrt(width).
+  auto load_query = [&]() {
+    const int kvh = use.item / chunks_of, head = (use.item % chunks_of) * 8 + g;
+    const bool live = head < a.group;
+    const float *row = a.q + (a.first + use.b) * a.q_row + (size_t)(kvh * a.group + head) * c.width;
+    // dimensions of this lane in step s: two pairs (F32: two single ones)
+    auto dim = [&](int s, int i) {
+      if (DTYPE == STB_F32) return s * 8 + t + 4 * i;
+      if (SCALED) return s * 16 + 4 * t + i;
+      return s * 16 + 2 * t + (i & 1) + 8 * (i >> 1);
+    };
+    constexpr int N = DTYPE == STB_F32 ? 2 : 4;
+    float factor = a.scale_log2;
+    if (HALF) {
+      float top = 0.0f;
+#pragma unroll
+      for (int s = 0; s < STEPS; s++)
+#pragma unroll
+        for (int i = 0; i < N; i++)
+          if (live && dim(s, i) < c.width) top = fmaxf(top, fabsf(row[dim(s, i)]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * a.scale_log2;
+      int e = 0;
+      if (top > 0.0f && top <= 3.402823466e38f) e = min(126, 12 - ((int)(__float_as_uint(top) >> 23) - 127));
+      unscale = scale_of((uint8_t)(127 - e));
+      const float up = scale_of((uint8_t)(127 + e));
+#pragma unroll
+      for (int s = 0; s < STEPS; s++) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = live && dim(s, i) < c.width ? row[dim(s, i)] * factor * up : 0.0f;
+        uint32_t u[2], v[2];
+        split2_pair(x[0], x[1], u);
+        split2_pair(x[2], x[3], v);
+        q[s][0] = u[0];
+        q[s][1] = u[1];
+        q[s][2] = v[0];
+        q[s][3] = v[1];
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < STEPS; s++) {
+        float x[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = live && dim(s, i) < c.width ? row[dim(s, i)] * factor : 0.0f;
+        if constexpr (DTYPE == STB_F32) {
+          split_tf32(x[0], q[s][0], q[s][1]);
+          split_tf32(x[1], q[s][2], q[s][3]);
+        } else {
+          uint16_t u[4][3];
+#pragma unroll
+          for (int i = 0; i < 4; i++) split3_bf16(x[i], u[i][0], u[i][1], u[i][2]);
+          q[s][0] = pack2(u[0][0], u[1][0]);
+          q[s][1] = pack2(u[0][1], u[1][1]);
+          q[s][2] = pack2(u[2][0], u[3][0]);
+          q[s][3] = pack2(u[2][1], u[3][1]);
+          q[s][4] = pack2(u[0][2], u[1][2]);
+          q[s][5] = pack2(u[2][2], u[3][2]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; i++) o[i][0] = o[i][1] = 0.0f;
+    m1 = m2 = -INFINITY;
+    sum = 0.0f;
+  };
+
+  // Dimension of o[i][j]: E4M3 values come in pairs of neighbouring dimensions, one per result tile.
+  auto dim_of = [&](int i, int j) { return SCALED ? (i >> 1) * 16 + 4 * t + 2 * j + (i & 1) : i * 8 + 2 * t + j; };
+
+  // The result of an item's tiles that this warp has seen: all of them to y; a part to the block's pieces (a first
+  // part, while the ring is in use) or over the warp's own ring (a last part).
+  float *const block_pieces = a.pieces + (size_t)blockIdx.x * BLOCK_PIECES;
+  float *const my_ring = (float *)(smem + warp * S::STAGES * S::TILE);
+  auto finish = [&](bool starts, bool ends) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    if (starts && ends) {
+      const int head = (use.item % chunks_of) * 8 + g;
+      if (head < a.group) {
+        float *y = a.y + (a.first + use.b) * a.y_row + (size_t)(use.item / chunks_of * a.group + head) * c.width;
+        const float f = sum != 0.0f ? (HALF ? 1.0f / P_SHIFT : 1.0f) * (SCALED ? exp2f(m2 - m1) : 1.0f) / sum : 0.0f;
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+          for (int j = 0; j < 2; j++)
+            if (dim_of(i, j) < c.width) y[dim_of(i, j)] = sum != 0.0f ? o[i][j] * f : 0.0f;
+      }
+      return;
+    }
+    float *part = (ends ? block_pieces + (2 + warp) * S::PART : my_ring) + g * (WP + 4);
+    if (t == 0) {
+      part[0] = m1;
+      part[1] = m2;
+      part[2] = sum;
+    }
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+      for (int j = 0; j < 2; j++) part[4 + dim_of(i, j)] = o[i][j];
+    if (lane == 0) {
+      int *p = s_part[2 * warp + (ends ? 0 : 1)];
+      p[0] = use.b;
+      p[1] = use.item;
+      p[2] = starts;
+      p[3] = ends;
+    }
+  };
+
+#pragma unroll
+  for (int i = 0; i < S::STAGES - 1; i++) issue(i);
+  if (todo > 0) load_query();
+  bool starts = use.tile == 0;
+  int stage = 0;
+  for (int i = 0; i < todo; i++) {
+    copy_wait<S::STAGES - 2>();
+    __syncwarp();  // every lane's copies of this tile are there, and the tile before it has been read
+    issue(stage == 0 ? S::STAGES - 1 : stage - 1);
+    const uint32_t keys = ring + stage * S::TILE, values = keys + TK * S::ROW;
+    const uint8_t *m = meta + stage * S::META;
+    const uint32_t mask = *(const uint32_t *)m;
+
+    // scores: row g (first terms of q) and row g + 8 (second terms) of both 8-key results
+    float ca[2][4] = {}, cb[2][4] = {}, cc[2][4] = {};
+    {
+      const int row = (lane & 7) + (lane >> 4) * 8, odd = (lane >> 3) & 1;
+#pragma unroll
+      for (int s = 0; s < S::CHUNKS / 2; s++) {
+        if (2 * s >= row_chunks) continue;
+        uint32_t r[4];
+        load_matrix4(r, chunk_at<S::ROW>(keys, row, 2 * s + odd));
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+          const uint32_t b0 = r[2 * n], b1 = r[2 * n + 1];
+          if constexpr (SCALED) {  // two steps of 16 dimensions, one register each
+            product<DTYPE>(ca[n], q[2 * s][0], q[2 * s][1], q[2 * s][2], q[2 * s][3], widen_pair(b0 & 0xffffu), widen_pair(b0 >> 16));
+            product<DTYPE>(cb[n], q[2 * s + 1][0], q[2 * s + 1][1], q[2 * s + 1][2], q[2 * s + 1][3], widen_pair(b1 & 0xffffu),
+                           widen_pair(b1 >> 16));
+          } else if constexpr (DTYPE == STB_F32) {
+            uint32_t h0, l0, h1, l1;
+            split_tf32(__uint_as_float(b0), h0, l0);
+            split_tf32(__uint_as_float(b1), h1, l1);
+            product<DTYPE>(s & 1 ? cb[n] : ca[n], q[s][0], q[s][1], q[s][2], q[s][3], h0, h1);
+            product<DTYPE>(cc[n], q[s][0], q[s][1], q[s][2], q[s][3], l0, l1);
+          } else {
+            product<DTYPE>(s & 1 ? cb[n] : ca[n], q[s][0], q[s][1], q[s][2], q[s][3], b0, b1);
+            if constexpr (DTYPE == STB_BF16) product<DTYPE>(cc[n], q[s][4], 0u, q[s][5], 0u, b0, b1);
+          }
+        }
+      }
+    }
+    float sc[4], ev[4], top1 = -INFINITY, top2 = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {  // key 2 t + (k & 1) + 8 (k >> 1) of the tile, head g
+      const int n = k >> 1, j = k & 1, key = 2 * t + j + 8 * n;
+      sc[k] = (ca[n][j] + cb[n][j]) + ((ca[n][2 + j] + cb[n][2 + j]) + cc[n][j]);
+      ev[k] = 0.0f;
+      if (HALF) sc[k] *= unscale;
+      if (SCALED) {
+        sc[k] *= scale_of(m[16 + key]);
+        ev[k] = (float)((int)m[32 + key] - 127);
+      }
+      if (mask >> key & 1) {
+        top1 = fmaxf(top1, sc[k]);
+        if (SCALED) top2 = fmaxf(top2, sc[k] + ev[k]);
+      }
+    }
+    top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 1));
+    top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 2));
+    if (SCALED) {
+      top2 = fmaxf(top2, __shfl_xor_sync(0xffffffffu, top2, 1));
+      top2 = fmaxf(top2, __shfl_xor_sync(0xffffffffu, top2, 2));
+    } else {
+      top2 = top1;
+    }
+    const bool move1 = top1 > m1 + LAZY, move2 = top2 > m2 + LAZY;
+    if (__any_sync(0xffffffffu, move1 || move2)) {
+      const float n1 = move1 ? top1 : m1, n2 = move2 ? top2 : m2;
+      const float f1 = move1 ? exp2f(m1 - n1) : 1.0f, f2 = move2 ? exp2f(m2 - n2) : 1.0f;
+      sum *= f1;
+#pragma unroll
+      for (int k = 0; k < NT; k++) {
+        o[k][0] *= f2;
+        o[k][1] *= f2;
+      }
+      m1 = n1;
+      m2 = n2;
+    }
+    float w[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int key = 2 * t + (k & 1) + 8 * (k >> 1);
+      const bool live = mask >> key & 1;
+      const float p = live ? exp2f(sc[k] - m1) : 0.0f;
+      sum += p;
+      w[k] = SCALED ? (live ? exp2f(sc[k] + ev[k] - m2) : 0.0f) : p;
+      if (HALF) w[k] *= P_SHIFT;
+    }
+
+    // weighted values: a fresh result per tile, its rows g and g + 8 added in Float32
+    if constexpr (DTYPE == STB_F32) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) split_tf32(w[k], hi[k], lo[k]);
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        if (2 * n >= row_chunks) continue;
+        float r[4] = {};
+        uint32_t vh[4], vl[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {  // keys 2 t, 2 t + 1 of each half as the product's slots t, t + 4
+          const int key = (k >> 1) * 8 + 2 * t + (k & 1);
+          float v;
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(chunk_at<S::ROW>(values, key, 2 * n + (g >> 2)) + (g & 3) * 4) : "memory");
+          split_tf32(v, vh[k], vl[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) product<DTYPE>(r, hi[k], lo[k], hi[k + 1], lo[k + 1], vl[k], vl[k + 1]);
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) product<DTYPE>(r, hi[k], lo[k], hi[k + 1], lo[k + 1], vh[k], vh[k + 1]);
+        o[n][0] += r[0] + r[2];
+        o[n][1] += r[1] + r[3];
+      }
+    } else {
+      uint32_t p0[3] = {}, p1[3] = {};
+      if constexpr (DTYPE == STB_BF16) {
+        split3_pair(w[0], w[1], p0);
+        split3_pair(w[2], w[3], p1);
+      } else {
+        uint32_t u[2], v[2];
+        split2_pair(w[0], w[1], u);
+        split2_pair(w[2], w[3], v);
+        p0[0] = u[0], p0[1] = u[1], p1[0] = v[0], p1[1] = v[1];
+      }
+      auto weigh = [&](float (&to)[2], uint32_t b0, uint32_t b1) {
+        float r[4] = {};
+        if constexpr (DTYPE == STB_BF16) product<DTYPE>(r, p0[2], 0u, p1[2], 0u, b0, b1);
+        product<DTYPE>(r, p0[0], p0[1], p1[0], p1[1], b0, b1);
+        to[0] += r[0] + r[2];
+        to[1] += r[1] + r[3];
+      };
+      const int row = (lane & 7) + ((lane >> 3) & 1) * 8, odd = lane >> 4;
+#pragma unroll
+      for (int s = 0; s < S::CHUNKS / 2; s++) {
+        if (2 * s >= row_chunks) continue;
+        uint32_t r[4];
+        load_matrix4_trans(r, chunk_at<S::ROW>(values, row, 2 * s + odd));
+        if constexpr (SCALED) {
+#pragma unroll
+          for (int h = 0; h < 2; h++) {  // bytes (key, dim), (key, dim + 1), (key + 1, dim), (key + 1, dim + 1)
+            const uint32_t x = __byte_perm(r[2 * h], 0, 0x3120), z = __byte_perm(r[2 * h + 1], 0, 0x3120);
+            weigh(o[4 * s + 2 * h], widen_pair(x & 0xffffu), widen_pair(z & 0xffffu));
+            weigh(o[4 * s + 2 * h + 1], widen_pair(x >> 16), widen_pair(z >> 16));
+          }
+        } else {
+          weigh(o[2 * s], r[0], r[1]);
+          weigh(o[2 * s + 1], r[2], r[3]);
+        }
+      }
+    }
+
+    if (use.tile + 1 == use.tiles) {
+      finish(starts, true);
+      advance(use);
+      starts = true;
+      if (i + 1 < todo) load_query();
+    } else if (i + 1 == todo) {
+      copy_wait<0>();
+      __syncwarp();
+      finish(starts, false);
+    } else {
+      use.tile++;
+    }
+    stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+  }
+  copy_wait<0>();
+  __syncthreads();
+
+  // Joins the parts of one item: `count` of them, part i at place(i) (`far`: written by other blocks); the result to y,
+  // or to `piece` as a part again.
+  auto join = [&](int count, auto far, auto place, int b, int item, float *piece) {
+    auto get = [](const float *p) { return decltype(far)::value ? __ldcg(p) : *p; };
+    if (threadIdx.x < 8) {
+      const int h = threadIdx.x;
+      float n1 = -INFINITY, n2 = -INFINITY, all = 0.0f;
+      for (int i = 0; i < count; i++) {
+        const float *p = place(i) + h * (WP + 4);
+        const float l = get(p + 2);
+        if (l != 0.0f) {
+          n1 = fmaxf(n1, get(p));
+          n2 = fmaxf(n2, get(p + 1));
+        }
+      }
+      for (int i = 0; i < count; i++) {
+        const float *p = place(i) + h * (WP + 4);
+        const float l = get(p + 2);
+        if (l != 0.0f) all += l * exp2f(get(p) - n1);
+        s_weight[i][h] = l != 0.0f ? exp2f(get(p + 1) - n2) : 0.0f;
+      }
+      s_head[h][0] = n1;
+      s_head[h][1] = n2;
+      s_head[h][2] = all;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 8 * WP; e += S::THREADS) {
+      const int h = e / WP, d = e % WP;
+      float v = 0.0f;
+#pragma unroll 4
+      for (int i = 0; i < count; i++) {
+        const float x = get(place(i) + h * (WP + 4) + 4 + d), f = s_weight[i][h];
+        if (f != 0.0f) v = fmaf(x, f, v);
+      }
+      const float n1 = s_head[h][0], n2 = s_head[h][1], all = s_head[h][2];
+      if (piece) {
+        piece[h * (WP + 4) + 4 + d] = v;
+        if (d < 3) piece[h * (WP + 4) + d] = s_head[h][d];
+      } else {
+        const int head = item % chunks_of * 8 + h;
+        if (head < a.group && d < c.width)
+          a.y[(a.first + b) * a.y_row + (size_t)(item / chunks_of * a.group + head) * c.width + d] =
+              all != 0.0f ? v * ((HALF ? 1.0f / P_SHIFT : 1.0f) * (SCALED ? exp2f(n2 - n1) : 1.0f) / all) : 0.0f;
+      }
+    }
+  };
+
+  for (int i = 0; i < 2 * S::WARPS;) {
+    const int b = s_part[i][0], item = s_part[i][1];
+    if (b < 0) {
+      i++;
+      continue;
+    }
+    const bool first = s_part[i][2];
+    int at[2 * S::WARPS], count = 0;
+    bool last = false;
+    for (; i < 2 * S::WARPS && (s_part[i][0] < 0 || (s_part[i][0] == b && s_part[i][1] == item)); i++)
+      if (s_part[i][0] >= 0) {
+        at[count++] = i;
+        last = s_part[i][3];
+      }
+    auto of_block = [&](int k) -> const float * {
+      return at[k] & 1 ? (const float *)(smem + (at[k] >> 1) * S::STAGES * S::TILE) : block_pieces + (2 + (at[k] >> 1)) * S::PART;
+    };
+    const long long i0 = s_start[b] * items + (long long)item * (s_start[b + 1] - s_start[b]);
+    float *piece = first && last ? nullptr : block_pieces + (block0 >= i0 ? 0 : 1) * S::PART;
+    join(count, std::false_type(), of_block, b, item, piece);
+    if (piece) {
+      const long long i1 = i0 + (s_start[b + 1] - s_start[b]);
+      const int c0 = (int)(((i0 + 1) * grid - 1) / total), c1 = (int)((i1 * grid - 1) / total);
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        s_last = atomicAdd(a.arrived + c0, 1) == c1 - c0;
+        if (s_last) a.arrived[c0] = 0;
+      }
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        auto of_blocks = [&](int k) -> const float * {
+          const long long start = total * (c0 + k) / grid;
+          return a.pieces + (size_t)(c0 + k) * BLOCK_PIECES + (start >= i0 ? 0 : 1) * S::PART;
+        };
+        join(c1 - c0 + 1, std::true_type(), of_blocks, b, item, nullptr);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <int DTYPE, int WP>
+void launch_attention(stb_session *s, const PagedView &c, AttendArgs a, int batch) {
+  using S = Shape<DTYPE, WP>;
+  {
+    static std::mutex mu;
+    static bool configured[64] = {};
+    std::lock_guard<std::mutex> lock(mu);
+    if (s->device < 0 || s->device >= 64 || !configured[s->device]) {
+      STB_CUDA(cudaFuncSetAttribute(paged_attention_kernel<DTYPE, WP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+      if (s->device >= 0 && s->device < 64) configured[s->device] = true;
+    }
+  }
+  const int grid = std::min(tc::sm_count(s->device), MAX_GRID);
+  for (a.first = 0; a.first < batch; a.first += MAX_BATCH) {
+    a.batch = std::min(MAX_BATCH, batch - a.first);
+    launch_kernel(paged_attention_kernel<DTYPE, WP>, dim3(grid), dim3(S::THREADS), (size_t)S::SMEM, s->stream, false, c, a);
+    count_launch(s);
+  }
+}
+
 }  // namespace
 }  // namespace stb
 
@@ -105,10 +776,35 @@ extern "C" int stb_op_paged_attention(stb_session *s, const stb_paged_cache *cac
     a.lengths = (const int *)lengths;
     a.heads = heads;
     a.group = heads / c.kv_heads;
+    a.batch = batch;
+    a.first = 0;
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)c.width));
+    a.pieces = nullptr;
+    a.arrived = nullptr;
+    const int esz = cache->dtype == STB_F32 ? 4 : (cache->dtype == STB_E4M3 ? 1 : 2);
+    // The copies move whole 16-byte chunks and address rows of the cache by an Int.
+    const bool chunked = c.width <= 256 && c.width * esz % 16 == 0 && cache->keys % 16 == 0 && cache->values % 16 == 0 &&
+                         (int64_t)c.pages * c.kv_heads * c.page_size <= 0x7fffffff;
+    if (!chunked) {
+      dispatch_paged(cache->dtype, [&](auto t) {
+        launch_kernel(paged_attention_any_kernel<decltype(t)::value>, dim3(heads, batch), dim3(256), 0, s->stream, false, c, a);
+      });
+      count_launch(s);
+      return;
+    }
+    const uint64_t counters = MAX_GRID * sizeof(int), bytes = counters + (uint64_t)MAX_GRID * BLOCK_PIECES * sizeof(float);
+    if (!s->paged_ws) {
+      if (capturing(s)) throw Error(STB_ERR_STATE, "a session's first paged attention cannot be captured: make a call before");
+      s->paged_ws = session_alloc(s, bytes);
+      STB_CUDA(cudaMemsetAsync((void *)s->paged_ws, 0, counters, s->stream));
+    }
+    a.arrived = (int *)s->paged_ws;
+    a.pieces = (float *)(s->paged_ws + counters);
     dispatch_paged(cache->dtype, [&](auto t) {
-      launch_kernel(paged_attention_kernel<decltype(t)::value>, dim3(heads, batch), dim3(256), 0, s->stream, false, c, a);
+      constexpr int DT = decltype(t)::value;
+      if (c.width <= 64) launch_attention<DT, 64>(s, c, a, batch);
+      else if (c.width <= 128) launch_attention<DT, 128>(s, c, a, batch);
+      else launch_attention<DT, 256>(s, c, a, batch);
     });
-    count_launch(s);
   });
 }
