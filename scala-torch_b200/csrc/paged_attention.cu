@@ -13,7 +13,7 @@
 //   * F32 cache: both sides in two TF32 terms.
 // The tensor core truncates its sums, so chains are kept short (at most 8 products) and joined by Float32 additions.
 //
-// Work: items (request, kv head, chunk of 8 query heads) are cut into tiles of 16 keys, all tiles in one line; each
+// Work: items (request, kv head, chunk of 8 query heads) are cut into tiles of 16 or 32 keys, all tiles in one line; each
 // block takes an equal stretch of the line and each of its warps an equal stretch of that (lengths are known on
 // the device only: a captured step is replayed with new ones).  A warp runs alone over its stretch, across items,
 // with a ring of cp.async stages of its own: no block barrier until its end.  Row g of a 16-row operand is
@@ -110,37 +110,46 @@ __global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedVie
 
 // ------------------------------------------------------------------ rows of whole 16-byte chunks, width <= 256
 
-constexpr int TK = 16;             // keys of a tile
 constexpr int MAX_GRID = 160;
 constexpr int BLOCK_PIECES = 20800;  // floats of a block's pieces, at most: (2 + warps) of 8 heads x (width + 4)
-constexpr int MAX_BATCH = 1024;    // requests of one launch (their prefix sums lie in shared memory)
-constexpr float LAZY = 8.0f;       // a maximum moves only when a score passes it by 2^8
-constexpr float P_SHIFT = 128.0f;  // F16 weights times 2^7: at most 2^15, and 2^-32 apart at their lowest
+constexpr int MAX_BATCH = 1024;      // requests of one launch (their prefix sums lie in shared memory)
+constexpr float LAZY = 8.0f;         // a maximum moves only when a score passes it by 2^8
+constexpr float P_SHIFT = 128.0f;    // F16 weights times 2^7: at most 2^15, and 2^-32 apart at their lowest
 
 template <int DTYPE, int WP>
 struct Shape {
   static constexpr int ESZ = DTYPE == STB_F32 ? 4 : (DTYPE == STB_E4M3 ? 1 : 2);
   static constexpr int ROW = WP * ESZ;            // bytes of a key's row in shared memory
   static constexpr int CHUNKS = ROW / 16;
+  static constexpr int TK = ROW >= 256 ? 16 : 32; // keys of a tile: 8 KB where the width allows
   static constexpr int TILE = 2 * TK * ROW;       // keys and values of a tile
   // Warps and stages that fill about 192 KB: at least two stages in flight per warp, 128 KB per SM.
-  static constexpr int WARPS = TILE <= 2048 ? 16 : (TILE <= 8192 ? 8 : (TILE <= 16384 ? 4 : 2));
+  static constexpr int WARPS = TILE <= 8192 ? 8 : (TILE <= 16384 ? 4 : 2);
   static constexpr int STAGES = 196608 / (WARPS * TILE) < 6 ? 196608 / (WARPS * TILE) : 6;
-  static constexpr int META = 64;                 // per stage: valid mask, scale bytes
+  static constexpr int META = 80;                 // per stage: valid mask, scale bytes of keys and values
   static constexpr int THREADS = WARPS * 32;
   static constexpr int RING = WARPS * STAGES * TILE;
   static constexpr int PART = 8 * (WP + 4);       // floats of a partial result: per head max, weight max, sum, -, values
-  static constexpr int SMEM = RING + WARPS * STAGES * META + (MAX_BATCH + 1) * 8 + 1024;
-  static_assert(STAGES >= 3 && SMEM <= 232448, "shared memory per block");
+  static constexpr int SMEM = RING + WARPS * STAGES * META + (2 * MAX_BATCH + 4) * 4;
+  static_assert(STAGES >= 3 && SMEM + 8192 <= 232448, "shared memory per block");
   static_assert(STAGES * TILE >= PART * 4, "a warp's last part reuses its ring");
   static_assert((2 + WARPS) * PART <= BLOCK_PIECES, "workspace");
 };
 
 __device__ __forceinline__ uint32_t shared_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-// 16 bytes of global memory to shared memory; `live` false writes zeros instead.
+// 16 bytes of global memory to shared memory; the second form writes zeros instead where `live` is false.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+// 2^x, at most 2 steps of Float32 off; results below 2^-126 are 0.
+__device__ __forceinline__ float pow2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -220,6 +229,15 @@ __device__ __forceinline__ uint32_t chunk_at(uint32_t base, int row, int chunk) 
   return base + line * 128 + ((at ^ (line & 7)) << 4);
 }
 
+// `total` tiles cut into `parts` stretches whose lengths differ by one at most: where a stretch begins, and whose tile i is.
+__device__ __forceinline__ int stretch_start(int k, int total, int parts) {
+  return k * (total / parts) + min(k, total % parts);
+}
+__device__ __forceinline__ int stretch_of(int i, int total, int parts) {
+  const int q = total / parts, r = total % parts;
+  return i < r * (q + 1) ? i / (q + 1) : r + (i - r * (q + 1)) / q;
+}
+
 // A place on the line of tiles.
 struct Cursor {
   int b, item, tile, tiles, n;  // request, its item (kv head * chunks + chunk), tile of the item, tiles and keys of the request
@@ -228,60 +246,65 @@ struct Cursor {
 template <int DTYPE, int WP>
 __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_kernel(const PagedView c, const AttendArgs a) {
   using S = Shape<DTYPE, WP>;
-  constexpr int STEP = DTYPE == STB_F32 ? 8 : 16;   // dimensions of one product
+  constexpr int TK = S::TK, NB = TK / 8, NK = 2 * NB;  // keys of a tile, 8-key results, keys of a lane
+  constexpr int STEP = DTYPE == STB_F32 ? 8 : 16;      // dimensions of one product
   constexpr int STEPS = WP / STEP, NT = WP / 8;
   constexpr int QREGS = DTYPE == STB_BF16 ? 6 : 4;  // operand registers of q per step
   constexpr bool HALF = DTYPE == STB_F16 || DTYPE == STB_E4M3, SCALED = DTYPE == STB_E4M3;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t *s_meta = smem + S::RING;
-  long long *s_start = (long long *)(s_meta + S::WARPS * S::STAGES * S::META);  // tiles before request b, per item of it
-  __shared__ long long s_scan[S::WARPS];
+  int *s_start = (int *)(s_meta + S::WARPS * S::STAGES * S::META);  // tiles before request b, of one item each
+  int *s_len = s_start + MAX_BATCH + 1;
+  __shared__ int s_scan[S::WARPS];
   __shared__ float s_weight[MAX_GRID][8];  // of the parts that are joined
-  __shared__ float s_head[8][3];           // joined maxima and sum per head
+  __shared__ __align__(16) float s_head[8][4];  // joined maxima and sum per head
   __shared__ int s_part[2 * S::WARPS][4];  // a warp's first and last part: request (or -1), item, whether it starts / ends it
+  __shared__ int s_list[2 * S::WARPS];     // entries of s_part that are joined
   __shared__ int s_last;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int chunks_of = (a.group + 7) / 8, items = c.kv_heads * chunks_of;
-  const int row_chunks = c.width * S::ESZ / 16;
+  const int row_chunks = c.width * S::ESZ / 16, row_bytes = row_chunks * 16;
 
   // Prefix sums of the requests' tiles, and zeros for the empty ones.
   {
-    const int per = (a.batch + S::THREADS - 1) / S::THREADS, b0 = threadIdx.x * per;
-    long long own = 0;
-    for (int b = b0; b < min(a.batch, b0 + per); b++) own += (attend_length(c, a, a.first + b) + TK - 1) / TK;
-    long long before = own;
+    const int per = (a.batch + S::THREADS - 1) / S::THREADS, b0 = threadIdx.x * per, b1 = min(a.batch, b0 + per);
+    int own = 0;
+    for (int b = b0; b < b1; b++) {
+      const int n = attend_length(c, a, a.first + b);
+      s_len[b] = n;
+      own += (n + TK - 1) / TK;
+    }
+    int before = own;
+#pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, before, off);
+      const int v = __shfl_up_sync(0xffffffffu, before, off);
       if (lane >= off) before += v;
     }
     if (lane == 31) s_scan[warp] = before;
-    __syncthreads();
-    before -= own;
-    for (int w = 0; w < warp; w++) before += s_scan[w];
-    for (int b = b0; b < min(a.batch, b0 + per); b++) {
-      s_start[b] = before;
-      before += (attend_length(c, a, a.first + b) + TK - 1) / TK;
-    }
-    if (threadIdx.x == 0) {
-      long long all = 0;
-      for (int w = 0; w < S::WARPS; w++) all += s_scan[w];
-      s_start[a.batch] = all;
-    }
     for (int i = threadIdx.x; i < 2 * S::WARPS; i += S::THREADS) s_part[i][0] = -1;
     if (c.width != WP)  // chunks behind the row are read as zeros and never written
       for (int i = threadIdx.x; i < S::RING / 16; i += S::THREADS) ((uint4 *)smem)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
+    before -= own;
+    for (int w = 0; w < warp; w++) before += s_scan[w];
+    for (int b = b0; b < b1; b++) {
+      s_start[b] = before;
+      before += (s_len[b] + TK - 1) / TK;
+      if (b == a.batch - 1) s_start[a.batch] = before;
+    }
+    __syncthreads();
   }
   for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
-    if (s_start[b] == s_start[b + 1])
+    if (s_len[b] == 0)
       for (int i = threadIdx.x; i < a.heads * c.width; i += S::THREADS) a.y[(a.first + b) * a.y_row + i] = 0.0f;
 
-  const long long total = s_start[a.batch] * items;
-  const int grid = (int)min((long long)gridDim.x, (total + S::WARPS - 1) / S::WARPS);
+  const int total = s_start[a.batch] * items;
+  const int grid = min((int)gridDim.x, (total + S::WARPS - 1) / S::WARPS);
   if ((int)blockIdx.x >= grid) return;
-  const long long block0 = total * blockIdx.x / grid, block1 = total * (blockIdx.x + 1) / grid;
-  const long long t0 = block0 + (block1 - block0) * warp / S::WARPS, t1 = block0 + (block1 - block0) * (warp + 1) / S::WARPS;
+  const int block0 = stretch_start(blockIdx.x, total, grid), mine = stretch_start(blockIdx.x + 1, total, grid) - block0;
+  const int t0 = block0 + stretch_start(warp, mine, S::WARPS);
+  const int todo = block0 + stretch_start(warp + 1, mine, S::WARPS) - t0;
 
   const uint32_t ring = shared_u32(smem) + warp * S::STAGES * S::TILE;
   uint8_t *meta = s_meta + warp * S::STAGES * S::META;
@@ -295,11 +318,11 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       else hi = mid - 1;
     }
     load.b = lo;
-    load.tiles = (int)(s_start[lo + 1] - s_start[lo]);
-    load.n = attend_length(c, a, a.first + lo);
-    const long long in = t0 - s_start[lo] * items;
-    load.item = load.tiles ? (int)(in / load.tiles) : 0;
-    load.tile = load.tiles ? (int)(in % load.tiles) : 0;
+    load.tiles = s_start[lo + 1] - s_start[lo];
+    load.n = s_len[lo];
+    const int in = t0 - s_start[lo] * items;
+    load.item = load.tiles ? in / load.tiles : 0;
+    load.tile = load.tiles ? in % load.tiles : 0;
     use = load;
   }
   auto advance = [&](Cursor &k) {
@@ -308,50 +331,70 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     if (++k.item < items) return;
     k.item = 0;
     do k.b++;
-    while (k.b < a.batch && s_start[k.b] == s_start[k.b + 1]);
+    while (k.b < a.batch && s_len[k.b] == 0);
     if (k.b < a.batch) {
-      k.tiles = (int)(s_start[k.b + 1] - s_start[k.b]);
-      k.n = attend_length(c, a, a.first + k.b);
+      k.tiles = s_start[k.b + 1] - s_start[k.b];
+      k.n = s_len[k.b];
     }
   };
-  const int todo = (int)(t1 - t0);
-  // Page of this lane's key (lane & 15) in the tile at `load`, one tile ahead of its copies.
+
+  // Copies of one tile: lane i looks up key i, then the warp copies whole rows, their addresses by shuffle.  The page of
+  // the next tile's key is read one tile ahead, and scale bytes are stored one tile after they are read: neither waits
+  // for memory here.
+  constexpr int PER = 32 / S::CHUNKS > 0 ? 32 / S::CHUNKS : 1;      // rows of one copy of the warp
+  constexpr int TIMES = S::CHUNKS > 32 ? S::CHUNKS / 32 : 1;        // copies of one row
+  const int my_key = lane % TK, my_row = TIMES == 1 ? lane / S::CHUNKS : 0, my_chunk = TIMES == 1 ? lane % S::CHUNKS : lane;
+  const uint8_t *const from[2] = {(const uint8_t *)c.kv[0] + my_chunk * 16, (const uint8_t *)c.kv[1] + my_chunk * 16};
+  const int page_shift = (c.page_size & (c.page_size - 1)) == 0 ? 31 - __clz(c.page_size) : -1;
   auto page_ahead = [&](bool live) {
-    const int key = load.tile * TK + (lane & 15);
+    const int key = load.tile * TK + my_key;
     if (!live || key >= load.n) return -2;
-    return c.tables[(size_t)(a.first + load.b) * c.blocks + key / c.page_size];
+    return c.tables[(size_t)(a.first + load.b) * c.blocks + (page_shift >= 0 ? key >> page_shift : key / c.page_size)];
   };
   int issued = 0, page = page_ahead(todo > 0);
+  uint32_t scales = 0;
+  uint8_t *scales_to = nullptr;
   auto issue = [&](int stage) {
+    if (SCALED && scales_to) {
+      scales_to[0] = (uint8_t)scales;
+      scales_to[TK] = (uint8_t)(scales >> 8);
+      scales_to = nullptr;
+    }
     if (issued < todo) {
-      const int key = load.tile * TK + (lane & 15), kvh = load.item / chunks_of;
+      const int key = load.tile * TK + my_key, kvh = chunks_of == 1 ? load.item : load.item / chunks_of;
       bool live = page != -2;
       if (live && (unsigned)page >= (unsigned)c.pages) {
         *c.err = DEV_BAD_INDEX;
         live = false;
       }
-      const int at = live ? (int)paged_row(c, page, kvh, key % c.page_size) : 0;
-      const uint32_t mask = __ballot_sync(0xffffffffu, live) & 0xffffu;
+      const int slot = page_shift >= 0 ? key & (c.page_size - 1) : key % c.page_size;
+      const int at = live ? (page * c.kv_heads + kvh) * c.page_size + slot : 0;
+      const uint32_t mask = __ballot_sync(0xffffffffu, live);
       uint8_t *m = meta + stage * S::META;
       if (lane == 0) *(uint32_t *)m = mask;
-      if (SCALED) m[16 + lane] = live ? c.scale[lane >> 4][at] : (uint8_t)127;
+      if (SCALED) {
+        scales = live ? c.scale[0][at] | (uint32_t)c.scale[1][at] << 8 : 0x7f7fu;
+        scales_to = m + 16 + my_key;
+      }
       const uint32_t dst = ring + stage * S::TILE;
-      constexpr int PER = 32 / S::CHUNKS > 0 ? 32 / S::CHUNKS : 1;  // rows of one copy of the warp
-      constexpr int TIMES = S::CHUNKS > 32 ? S::CHUNKS / 32 : 1;
-#pragma unroll
-      for (int side = 0; side < 2; side++)
+      auto copy = [&](auto all) {
 #pragma unroll
         for (int r0 = 0; r0 < TK; r0 += PER) {
-          const int r = r0 + (TIMES == 1 ? lane / S::CHUNKS : 0);
-          const int from = __shfl_sync(0xffffffffu, at, r);
+          const int r = r0 + my_row;
+          const size_t off = (size_t)(uint32_t)__shfl_sync(0xffffffffu, at, r) * row_bytes;
 #pragma unroll
-          for (int i = 0; i < TIMES; i++) {
-            const int chunk = TIMES == 1 ? lane % S::CHUNKS : i * 32 + lane;
-            if (chunk < row_chunks)
-              copy16(chunk_at<S::ROW>(dst + side * TK * S::ROW, r, chunk),
-                     (const uint8_t *)c.kv[side] + ((size_t)from * row_chunks + chunk) * 16, mask >> r & 1);
-          }
+          for (int side = 0; side < 2; side++)
+#pragma unroll
+            for (int i = 0; i < TIMES; i++)
+              if (S::CHUNKS == 1 || my_chunk + i * 32 < row_chunks) {
+                const uint32_t to = chunk_at<S::ROW>(dst + side * TK * S::ROW, r, my_chunk + i * 32);
+                if (decltype(all)::value) copy16(to, from[side] + off + i * 512);
+                else copy16(to, from[side] + off + i * 512, mask >> r & 1);
+              }
         }
+      };
+      if (mask == 0xffffffffu) copy(std::true_type());
+      else copy(std::false_type());
       advance(load);
       issued++;
       page = page_ahead(issued < todo);
@@ -375,13 +418,16 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     };
     constexpr int N = DTYPE == STB_F32 ? 2 : 4;
     float factor = a.scale_log2;
-    if (HALF) {
+    if (HALF) {  // the head's largest magnitude to 2^12
       float top = 0.0f;
 #pragma unroll
       for (int s = 0; s < STEPS; s++)
 #pragma unroll
-        for (int i = 0; i < N; i++)
-          if (live && dim(s, i) < c.width) top = fmaxf(top, fabsf(row[dim(s, i)]));
+        for (int i = 0; i < N; i++) {
+          const float x = live && dim(s, i) < c.width ? row[dim(s, i)] : 0.0f;
+          q[s][i] = __float_as_uint(x);
+          top = fmaxf(top, fabsf(x));
+        }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * a.scale_log2;
       int e = 0;
@@ -392,7 +438,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       for (int s = 0; s < STEPS; s++) {
         float x[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = live && dim(s, i) < c.width ? row[dim(s, i)] * factor * up : 0.0f;
+        for (int i = 0; i < 4; i++) x[i] = __uint_as_float(q[s][i]) * factor * up;
         uint32_t u[2], v[2];
         split2_pair(x[0], x[1], u);
         split2_pair(x[2], x[3], v);
@@ -453,11 +499,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       return;
     }
     float *part = (ends ? block_pieces + (2 + warp) * S::PART : my_ring) + g * (WP + 4);
-    if (t == 0) {
-      part[0] = m1;
-      part[1] = m2;
-      part[2] = sum;
-    }
+    if (t == 0) *(float4 *)part = make_float4(m1, m2, sum, 0.0f);
 #pragma unroll
     for (int i = 0; i < NT; i++)
 #pragma unroll
@@ -471,11 +513,12 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     }
   };
 
-#pragma unroll
+#pragma unroll 1
   for (int i = 0; i < S::STAGES - 1; i++) issue(i);
   if (todo > 0) load_query();
   bool starts = use.tile == 0;
   int stage = 0;
+#pragma unroll 1
   for (int i = 0; i < todo; i++) {
     copy_wait<S::STAGES - 2>();
     __syncwarp();  // every lane's copies of this tile are there, and the tile before it has been read
@@ -484,50 +527,58 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     const uint8_t *m = meta + stage * S::META;
     const uint32_t mask = *(const uint32_t *)m;
 
-    // scores: row g (first terms of q) and row g + 8 (second terms) of both 8-key results
-    float ca[2][4] = {}, cb[2][4] = {}, cc[2][4] = {};
+    // scores: row g (first terms of q) and row g + 8 (second terms) of the 8-key results
+    float ca[NB][4] = {}, cb[NB][4] = {}, cc[NB][4] = {};
     {
       const int row = (lane & 7) + (lane >> 4) * 8, odd = (lane >> 3) & 1;
 #pragma unroll
       for (int s = 0; s < S::CHUNKS / 2; s++) {
         if (2 * s >= row_chunks) continue;
-        uint32_t r[4];
-        load_matrix4(r, chunk_at<S::ROW>(keys, row, 2 * s + odd));
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-          const uint32_t b0 = r[2 * n], b1 = r[2 * n + 1];
-          if constexpr (SCALED) {  // two steps of 16 dimensions, one register each
-            product<DTYPE>(ca[n], q[2 * s][0], q[2 * s][1], q[2 * s][2], q[2 * s][3], widen_pair(b0 & 0xffffu), widen_pair(b0 >> 16));
-            product<DTYPE>(cb[n], q[2 * s + 1][0], q[2 * s + 1][1], q[2 * s + 1][2], q[2 * s + 1][3], widen_pair(b1 & 0xffffu),
-                           widen_pair(b1 >> 16));
-          } else if constexpr (DTYPE == STB_F32) {
-            uint32_t h0, l0, h1, l1;
-            split_tf32(__uint_as_float(b0), h0, l0);
-            split_tf32(__uint_as_float(b1), h1, l1);
-            product<DTYPE>(s & 1 ? cb[n] : ca[n], q[s][0], q[s][1], q[s][2], q[s][3], h0, h1);
-            product<DTYPE>(cc[n], q[s][0], q[s][1], q[s][2], q[s][3], l0, l1);
-          } else {
-            product<DTYPE>(s & 1 ? cb[n] : ca[n], q[s][0], q[s][1], q[s][2], q[s][3], b0, b1);
-            if constexpr (DTYPE == STB_BF16) product<DTYPE>(cc[n], q[s][4], 0u, q[s][5], 0u, b0, b1);
+        for (int n0 = 0; n0 < NB; n0 += 2) {
+          uint32_t r[4];
+          load_matrix4(r, chunk_at<S::ROW>(keys, row + n0 * 8, 2 * s + odd));
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const int n = n0 + h;
+            const uint32_t b0 = r[2 * h], b1 = r[2 * h + 1];
+            if constexpr (SCALED) {  // two steps of 16 dimensions, one register each
+              product<DTYPE>(ca[n], q[2 * s][0], q[2 * s][1], q[2 * s][2], q[2 * s][3], widen_pair(b0 & 0xffffu), widen_pair(b0 >> 16));
+              product<DTYPE>(cb[n], q[2 * s + 1][0], q[2 * s + 1][1], q[2 * s + 1][2], q[2 * s + 1][3], widen_pair(b1 & 0xffffu),
+                             widen_pair(b1 >> 16));
+            } else if constexpr (DTYPE == STB_F32) {
+              uint32_t h0, l0, h1, l1;
+              split_tf32(__uint_as_float(b0), h0, l0);
+              split_tf32(__uint_as_float(b1), h1, l1);
+              product<DTYPE>(s & 1 ? cb[n] : ca[n], q[s][0], q[s][1], q[s][2], q[s][3], h0, h1);
+              product<DTYPE>(cc[n], q[s][0], q[s][1], q[s][2], q[s][3], l0, l1);
+            } else {
+              product<DTYPE>(s & 1 ? cb[n] : ca[n], q[s][0], q[s][1], q[s][2], q[s][3], b0, b1);
+              if constexpr (DTYPE == STB_BF16) product<DTYPE>(cc[n], q[s][4], 0u, q[s][5], 0u, b0, b1);
+            }
           }
         }
       }
     }
-    float sc[4], ev[4], top1 = -INFINITY, top2 = -INFINITY;
+    float sc[NK], sw[SCALED ? NK : 1], top1 = -INFINITY, top2 = -INFINITY;
+    const uint32_t live = mask >> (2 * t);  // bit (k & 1) + 8 (k >> 1): key 2 t + (k & 1) + 8 (k >> 1) of the tile
 #pragma unroll
-    for (int k = 0; k < 4; k++) {  // key 2 t + (k & 1) + 8 (k >> 1) of the tile, head g
-      const int n = k >> 1, j = k & 1, key = 2 * t + j + 8 * n;
+    for (int k = 0; k < NK; k++) {
+      const int n = k >> 1, j = k & 1;
       sc[k] = (ca[n][j] + cb[n][j]) + ((ca[n][2 + j] + cb[n][2 + j]) + cc[n][j]);
-      ev[k] = 0.0f;
-      if (HALF) sc[k] *= unscale;
       if (SCALED) {
-        sc[k] *= scale_of(m[16 + key]);
-        ev[k] = (float)((int)m[32 + key] - 127);
+        const int key = 2 * t + j + 8 * n;
+        sc[k] *= unscale * scale_of(m[16 + key]);
+        sw[k] = sc[k] + (float)((int)m[16 + TK + key] - 127);
+      } else if (HALF) {
+        sc[k] *= unscale;
       }
-      if (mask >> key & 1) {
-        top1 = fmaxf(top1, sc[k]);
-        if (SCALED) top2 = fmaxf(top2, sc[k] + ev[k]);
+      if (!(live >> (j + 8 * n) & 1)) {
+        sc[k] = -INFINITY;
+        if (SCALED) sw[k] = -INFINITY;
       }
+      top1 = fmaxf(top1, sc[k]);
+      if (SCALED) top2 = fmaxf(top2, sw[k]);
     }
     top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 1));
     top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 2));
@@ -540,7 +591,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     const bool move1 = top1 > m1 + LAZY, move2 = top2 > m2 + LAZY;
     if (__any_sync(0xffffffffu, move1 || move2)) {
       const float n1 = move1 ? top1 : m1, n2 = move2 ? top2 : m2;
-      const float f1 = move1 ? exp2f(m1 - n1) : 1.0f, f2 = move2 ? exp2f(m2 - n2) : 1.0f;
+      const float f1 = move1 ? pow2(m1 - n1) : 1.0f, f2 = move2 ? pow2(m2 - n2) : 1.0f;
       sum *= f1;
 #pragma unroll
       for (int k = 0; k < NT; k++) {
@@ -550,14 +601,14 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       m1 = n1;
       m2 = n2;
     }
-    float w[4];
+    // Weights; a maximum of -inf means that no key has counted yet, and none does here (their scores are -inf).
+    const float base1 = m1 == -INFINITY ? 0.0f : m1, base2 = m2 == -INFINITY ? 0.0f : m2;
+    float w[NK];
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const int key = 2 * t + (k & 1) + 8 * (k >> 1);
-      const bool live = mask >> key & 1;
-      const float p = live ? exp2f(sc[k] - m1) : 0.0f;
+    for (int k = 0; k < NK; k++) {
+      const float p = pow2(sc[k] - base1);
       sum += p;
-      w[k] = SCALED ? (live ? exp2f(sc[k] + ev[k] - m2) : 0.0f) : p;
+      w[k] = SCALED ? pow2(sw[k] - base2) : p;
       if (HALF) w[k] *= P_SHIFT;
     }
 
@@ -586,39 +637,43 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
         o[n][1] += r[1] + r[3];
       }
     } else {
-      uint32_t p0[3] = {}, p1[3] = {};
-      if constexpr (DTYPE == STB_BF16) {
-        split3_pair(w[0], w[1], p0);
-        split3_pair(w[2], w[3], p1);
-      } else {
-        uint32_t u[2], v[2];
-        split2_pair(w[0], w[1], u);
-        split2_pair(w[2], w[3], v);
-        p0[0] = u[0], p0[1] = u[1], p1[0] = v[0], p1[1] = v[1];
+      constexpr int TERMS = DTYPE == STB_BF16 ? 3 : 2;
+      uint32_t p[NB][TERMS];  // keys 8 n + 2 t, + 1 of each term
+#pragma unroll
+      for (int n = 0; n < NB; n++) {
+        if constexpr (DTYPE == STB_BF16) split3_pair(w[2 * n], w[2 * n + 1], p[n]);
+        else split2_pair(w[2 * n], w[2 * n + 1], p[n]);
       }
-      auto weigh = [&](float (&to)[2], uint32_t b0, uint32_t b1) {
-        float r[4] = {};
-        if constexpr (DTYPE == STB_BF16) product<DTYPE>(r, p0[2], 0u, p1[2], 0u, b0, b1);
-        product<DTYPE>(r, p0[0], p0[1], p1[0], p1[1], b0, b1);
-        to[0] += r[0] + r[2];
-        to[1] += r[1] + r[3];
-      };
       const int row = (lane & 7) + ((lane >> 3) & 1) * 8, odd = lane >> 4;
+      constexpr int PAIR = SCALED ? 4 : 2;  // result tiles of two chunks
 #pragma unroll
       for (int s = 0; s < S::CHUNKS / 2; s++) {
         if (2 * s >= row_chunks) continue;
-        uint32_t r[4];
-        load_matrix4_trans(r, chunk_at<S::ROW>(values, row, 2 * s + odd));
-        if constexpr (SCALED) {
+        float r[PAIR][4] = {};
 #pragma unroll
-          for (int h = 0; h < 2; h++) {  // bytes (key, dim), (key, dim + 1), (key + 1, dim), (key + 1, dim + 1)
-            const uint32_t x = __byte_perm(r[2 * h], 0, 0x3120), z = __byte_perm(r[2 * h + 1], 0, 0x3120);
-            weigh(o[4 * s + 2 * h], widen_pair(x & 0xffffu), widen_pair(z & 0xffffu));
-            weigh(o[4 * s + 2 * h + 1], widen_pair(x >> 16), widen_pair(z >> 16));
+        for (int n = 0; n < NB; n += 2) {
+          auto weigh = [&](float (&to)[4], uint32_t b0, uint32_t b1) {
+            if constexpr (DTYPE == STB_BF16) product<DTYPE>(to, p[n][2], 0u, p[n + 1][2], 0u, b0, b1);
+            product<DTYPE>(to, p[n][0], p[n][1], p[n + 1][0], p[n + 1][1], b0, b1);
+          };
+          uint32_t v[4];
+          load_matrix4_trans(v, chunk_at<S::ROW>(values, row + n * 8, 2 * s + odd));
+          if constexpr (SCALED) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {  // bytes (key, dim), (key, dim + 1), (key + 1, dim), (key + 1, dim + 1)
+              const uint32_t x = __byte_perm(v[2 * h], 0, 0x3120), z = __byte_perm(v[2 * h + 1], 0, 0x3120);
+              weigh(r[2 * h], widen_pair(x & 0xffffu), widen_pair(z & 0xffffu));
+              weigh(r[2 * h + 1], widen_pair(x >> 16), widen_pair(z >> 16));
+            }
+          } else {
+            weigh(r[0], v[0], v[1]);
+            weigh(r[1], v[2], v[3]);
           }
-        } else {
-          weigh(o[2 * s], r[0], r[1]);
-          weigh(o[2 * s + 1], r[2], r[3]);
+        }
+#pragma unroll
+        for (int k = 0; k < PAIR; k++) {
+          o[PAIR * s + k][0] += r[k][0] + r[k][2];
+          o[PAIR * s + k][1] += r[k][1] + r[k][3];
         }
       }
     }
@@ -643,47 +698,65 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
   // Joins the parts of one item: `count` of them, part i at place(i) (`far`: written by other blocks); the result to y,
   // or to `piece` as a part again.
   auto join = [&](int count, auto far, auto place, int b, int item, float *piece) {
-    auto get = [](const float *p) { return decltype(far)::value ? __ldcg(p) : *p; };
-    if (threadIdx.x < 8) {
-      const int h = threadIdx.x;
+    auto get = [](const float *p) { return decltype(far)::value ? __ldcg((const float4 *)p) : *(const float4 *)p; };
+    constexpr int MOST = decltype(far)::value ? MAX_GRID / 32 : (2 * S::WARPS + 31) / 32;
+    for (int h = warp; h < 8; h += S::WARPS) {  // a warp per head, a lane per part
+      float4 part[MOST];
       float n1 = -INFINITY, n2 = -INFINITY, all = 0.0f;
-      for (int i = 0; i < count; i++) {
-        const float *p = place(i) + h * (WP + 4);
-        const float l = get(p + 2);
-        if (l != 0.0f) {
-          n1 = fmaxf(n1, get(p));
-          n2 = fmaxf(n2, get(p + 1));
+#pragma unroll
+      for (int k = 0; k < MOST; k++) {
+        part[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (k * 32 + lane < count) part[k] = get(place(k * 32 + lane) + h * (WP + 4));
+      }
+#pragma unroll
+      for (int k = 0; k < MOST; k++)
+        if (part[k].z != 0.0f) {
+          n1 = fmaxf(n1, part[k].x);
+          n2 = fmaxf(n2, part[k].y);
         }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) {
+        n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, off));
+        n2 = fmaxf(n2, __shfl_xor_sync(0xffffffffu, n2, off));
       }
-      for (int i = 0; i < count; i++) {
-        const float *p = place(i) + h * (WP + 4);
-        const float l = get(p + 2);
-        if (l != 0.0f) all += l * exp2f(get(p) - n1);
-        s_weight[i][h] = l != 0.0f ? exp2f(get(p + 1) - n2) : 0.0f;
+#pragma unroll
+      for (int k = 0; k < MOST; k++) {
+        if (part[k].z != 0.0f) all += part[k].z * exp2f(part[k].x - n1);
+        if (k * 32 + lane < count) s_weight[k * 32 + lane][h] = part[k].z != 0.0f ? exp2f(part[k].y - n2) : 0.0f;
       }
-      s_head[h][0] = n1;
-      s_head[h][1] = n2;
-      s_head[h][2] = all;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
+      if (lane == 0) *(float4 *)s_head[h] = make_float4(n1, n2, all, 0.0f);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < 8 * WP; e += S::THREADS) {
-      const int h = e / WP, d = e % WP;
-      float v = 0.0f;
-#pragma unroll 4
+    for (int e = threadIdx.x; e < 2 * WP; e += S::THREADS) {
+      const int h = e / (WP / 4), d = e % (WP / 4) * 4;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
       for (int i = 0; i < count; i++) {
-        const float x = get(place(i) + h * (WP + 4) + 4 + d), f = s_weight[i][h];
-        if (f != 0.0f) v = fmaf(x, f, v);
+        const float4 x = get(place(i) + h * (WP + 4) + 4 + d);
+        const float f = s_weight[i][h];
+        if (f != 0.0f) {  // a part without a key may hold anything
+          v.x = fmaf(x.x, f, v.x);
+          v.y = fmaf(x.y, f, v.y);
+          v.z = fmaf(x.z, f, v.z);
+          v.w = fmaf(x.w, f, v.w);
+        }
       }
-      const float n1 = s_head[h][0], n2 = s_head[h][1], all = s_head[h][2];
+      const float4 top = *(const float4 *)s_head[h];
       if (piece) {
-        piece[h * (WP + 4) + 4 + d] = v;
-        if (d < 3) piece[h * (WP + 4) + d] = s_head[h][d];
-      } else {
-        const int head = item % chunks_of * 8 + h;
-        if (head < a.group && d < c.width)
-          a.y[(a.first + b) * a.y_row + (size_t)(item / chunks_of * a.group + head) * c.width + d] =
-              all != 0.0f ? v * ((HALF ? 1.0f / P_SHIFT : 1.0f) * (SCALED ? exp2f(n2 - n1) : 1.0f) / all) : 0.0f;
+        *(float4 *)(piece + h * (WP + 4) + 4 + d) = v;
+        if (d == 0) *(float4 *)(piece + h * (WP + 4)) = top;
+        continue;
       }
+      const int head = item % chunks_of * 8 + h;
+      if (head >= a.group) continue;
+      float *y = a.y + (a.first + b) * a.y_row + (size_t)(item / chunks_of * a.group + head) * c.width + d;
+      const float f = top.z != 0.0f ? (HALF ? 1.0f / P_SHIFT : 1.0f) * (SCALED ? exp2f(top.y - top.x) : 1.0f) / top.z : 0.0f;
+      if (d < c.width) y[0] = f != 0.0f ? v.x * f : 0.0f;
+      if (d + 1 < c.width) y[1] = f != 0.0f ? v.y * f : 0.0f;
+      if (d + 2 < c.width) y[2] = f != 0.0f ? v.z * f : 0.0f;
+      if (d + 3 < c.width) y[3] = f != 0.0f ? v.w * f : 0.0f;
     }
   };
 
@@ -694,22 +767,26 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       continue;
     }
     const bool first = s_part[i][2];
-    int at[2 * S::WARPS], count = 0;
+    int count = 0;
     bool last = false;
+    uint32_t which = 0;  // entries of this item
     for (; i < 2 * S::WARPS && (s_part[i][0] < 0 || (s_part[i][0] == b && s_part[i][1] == item)); i++)
       if (s_part[i][0] >= 0) {
-        at[count++] = i;
+        which |= 1u << i;
+        count++;
         last = s_part[i][3];
       }
+    if (threadIdx.x < 2 * S::WARPS && (which >> threadIdx.x & 1)) s_list[__popc(which & ((1u << threadIdx.x) - 1))] = threadIdx.x;
+    __syncthreads();
     auto of_block = [&](int k) -> const float * {
-      return at[k] & 1 ? (const float *)(smem + (at[k] >> 1) * S::STAGES * S::TILE) : block_pieces + (2 + (at[k] >> 1)) * S::PART;
+      const int i = s_list[k];
+      return i & 1 ? (const float *)(smem + (i >> 1) * S::STAGES * S::TILE) : block_pieces + (2 + (i >> 1)) * S::PART;
     };
-    const long long i0 = s_start[b] * items + (long long)item * (s_start[b + 1] - s_start[b]);
+    const int tiles = s_start[b + 1] - s_start[b], i0 = s_start[b] * items + item * tiles;
     float *piece = first && last ? nullptr : block_pieces + (block0 >= i0 ? 0 : 1) * S::PART;
     join(count, std::false_type(), of_block, b, item, piece);
     if (piece) {
-      const long long i1 = i0 + (s_start[b + 1] - s_start[b]);
-      const int c0 = (int)(((i0 + 1) * grid - 1) / total), c1 = (int)((i1 * grid - 1) / total);
+      const int c0 = stretch_of(i0, total, grid), c1 = stretch_of(i0 + tiles - 1, total, grid);
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) {
@@ -720,8 +797,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       if (s_last) {
         __threadfence();
         auto of_blocks = [&](int k) -> const float * {
-          const long long start = total * (c0 + k) / grid;
-          return a.pieces + (size_t)(c0 + k) * BLOCK_PIECES + (start >= i0 ? 0 : 1) * S::PART;
+          return a.pieces + (size_t)(c0 + k) * BLOCK_PIECES + (stretch_start(c0 + k, total, grid) >= i0 ? 0 : 1) * S::PART;
         };
         join(c1 - c0 + 1, std::true_type(), of_blocks, b, item, nullptr);
       }
@@ -731,7 +807,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
 }
 
 template <int DTYPE, int WP>
-void launch_attention(stb_session *s, const PagedView &c, AttendArgs a, int batch) {
+void launch_attention(stb_session *s, const PagedView &c, AttendArgs a, int batch, int at_once) {
   using S = Shape<DTYPE, WP>;
   {
     static std::mutex mu;
@@ -743,8 +819,8 @@ void launch_attention(stb_session *s, const PagedView &c, AttendArgs a, int batc
     }
   }
   const int grid = std::min(tc::sm_count(s->device), MAX_GRID);
-  for (a.first = 0; a.first < batch; a.first += MAX_BATCH) {
-    a.batch = std::min(MAX_BATCH, batch - a.first);
+  for (a.first = 0; a.first < batch; a.first += at_once) {
+    a.batch = std::min(at_once, batch - a.first);
     launch_kernel(paged_attention_kernel<DTYPE, WP>, dim3(grid), dim3(S::THREADS), (size_t)S::SMEM, s->stream, false, c, a);
     count_launch(s);
   }
@@ -782,9 +858,12 @@ extern "C" int stb_op_paged_attention(stb_session *s, const stb_paged_cache *cac
     a.pieces = nullptr;
     a.arrived = nullptr;
     const int esz = cache->dtype == STB_F32 ? 4 : (cache->dtype == STB_E4M3 ? 1 : 2);
+    // Requests of one launch whose tiles (16 keys at least) an Int can count, whatever their lengths.
+    const int64_t tiles = ((int64_t)c.blocks * c.page_size / 16 + 1) * c.kv_heads * ((a.group + 7) / 8);
+    const int at_once = (int)std::min<int64_t>(MAX_BATCH, 0x7fffffff / tiles);
     // The copies move whole 16-byte chunks and address rows of the cache by an Int.
     const bool chunked = c.width <= 256 && c.width * esz % 16 == 0 && cache->keys % 16 == 0 && cache->values % 16 == 0 &&
-                         (int64_t)c.pages * c.kv_heads * c.page_size <= 0x7fffffff;
+                         (int64_t)c.pages * c.kv_heads * c.page_size <= 0x7fffffff && at_once > 0;
     if (!chunked) {
       dispatch_paged(cache->dtype, [&](auto t) {
         launch_kernel(paged_attention_any_kernel<decltype(t)::value>, dim3(heads, batch), dim3(256), 0, s->stream, false, c, a);
@@ -802,9 +881,9 @@ extern "C" int stb_op_paged_attention(stb_session *s, const stb_paged_cache *cac
     a.pieces = (float *)(s->paged_ws + counters);
     dispatch_paged(cache->dtype, [&](auto t) {
       constexpr int DT = decltype(t)::value;
-      if (c.width <= 64) launch_attention<DT, 64>(s, c, a, batch);
-      else if (c.width <= 128) launch_attention<DT, 128>(s, c, a, batch);
-      else launch_attention<DT, 256>(s, c, a, batch);
+      if (c.width <= 64) launch_attention<DT, 64>(s, c, a, batch, at_once);
+      else if (c.width <= 128) launch_attention<DT, 128>(s, c, a, batch, at_once);
+      else launch_attention<DT, 256>(s, c, a, batch, at_once);
     });
   });
 }
