@@ -5,7 +5,7 @@
 // What bounds it: every cached byte is read once, 4 * group flops per element: HBM, as long as the arithmetic keeps
 // out of the way.  With 8 query heads on a kv head, Float32 FMAs would take 8 flops per BF16 byte (52 TFLOP/s at the
 // copy rate of 6.5 TB/s, near the SM's FP32 peak) and twice that for E4M3, so both products run on the tensor
-// cores (mma.sync: a 16-row operand is all there is to multiply, the 128-row tiles of tcgen05 would be padding), with
+// cores (mma.sync, fed by each warp's own ring: with 8 columns there is no reuse that larger tiles could find), with
 // Float32 accuracy kept by splitting the Float32 side into terms that the products take exactly:
 //   * BF16 cache: q and p in three BF16 terms (24 bits);
 //   * F16 and E4M3 cache (E4M3 widens to F16 exactly): two F16 terms (22 bits), after a power of two that puts the
@@ -16,10 +16,9 @@
 // Work: items (request, kv head, chunk of 8 query heads) are cut into tiles of 16 or 32 keys, all tiles in one line; each
 // block takes an equal stretch of the line and each of its warps an equal stretch of that (lengths are known on
 // the device only: a captured step is replayed with new ones).  A warp runs alone over its stretch, across items,
-// with a ring of cp.async stages of its own: no block barrier until its end.  Row g of a 16-row operand is
-// query head g in its first term, row g + 8 the same head's second term, so a lane (g, t) of a product's result
-// holds head g at keys (dimensions) 2t, 2t + 1 and its lower terms: the running maximum needs two shuffles, and
-// weights become the next product's operand without moving.  Items that a block covers only in part are joined
+// with a ring of cp.async stages of its own: no block barrier until its end.  The cache is the 16-row operand of
+// both products (keys, then dimensions, as rows), the 8 heads are the columns, a product per term: no row of the
+// tensor core's tile is padding.  Maxima move only when a score passes them by 2^8, which one vote per tile sees.  Items that a block covers only in part are joined
 // first among its warps in shared memory, then by the last block to arrive, always in the order of the keys.
 #include <algorithm>
 #include <cmath>
@@ -160,32 +159,35 @@ __device__ __forceinline__ void copy_wait() {
 __device__ __forceinline__ void load_matrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 __device__ __forceinline__ void load_matrix4_trans(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
+}
+// Transpose of an 8 x 8 matrix of 16-bit elements, two neighbours of row lane / 4 per lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 // c += a . b, 16 x 8 results; a 16 x 16 (BF16, F16) or 16 x 8 (F32 taken as TF32).
 template <int DTYPE>
-__device__ __forceinline__ void product(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
+__device__ __forceinline__ void product(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (DTYPE == STB_F32)
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else if constexpr (DTYPE == STB_BF16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // x = hi + lo in two TF32 values: hi rounded to 11 bits (half a step up, then cut), lo the exact rest, rounded likewise.
@@ -246,10 +248,10 @@ struct Cursor {
 template <int DTYPE, int WP>
 __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_kernel(const PagedView c, const AttendArgs a) {
   using S = Shape<DTYPE, WP>;
-  constexpr int TK = S::TK, NB = TK / 8, NK = 2 * NB;  // keys of a tile, 8-key results, keys of a lane
-  constexpr int STEP = DTYPE == STB_F32 ? 8 : 16;      // dimensions of one product
-  constexpr int STEPS = WP / STEP, NT = WP / 8;
-  constexpr int QREGS = DTYPE == STB_BF16 ? 6 : 4;  // operand registers of q per step
+  constexpr int TK = S::TK, MB = TK / 16;          // keys of a tile, its 16-key results
+  constexpr int STEP = DTYPE == STB_F32 ? 8 : 16;  // dimensions of one product
+  constexpr int STEPS = WP / STEP, NT = WP / 16;
+  constexpr int TERMS = DTYPE == STB_BF16 ? 3 : 2;  // of q and of the weights
   constexpr bool HALF = DTYPE == STB_F16 || DTYPE == STB_E4M3, SCALED = DTYPE == STB_E4M3;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t *s_meta = smem + S::RING;
@@ -402,8 +404,8 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     copy_commit();
   };
 
-  uint32_t q[STEPS][QREGS];
-  float o[NT][2], m1 = -INFINITY, m2 = -INFINITY, sum = 0.0f, unscale = 1.0f;
+  uint32_t q[STEPS][2 * TERMS];
+  float o[NT][4], m1[2], m2[2], sum[2], unscale[2] = {1.0f, 1.0f};
 
   // q of the item at `use` into operand registers, scaled by log2(e) / sqrt(width).
   auto load_query = [&]() {
@@ -417,93 +419,94 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       return s * 16 + 2 * t + (i & 1) + 8 * (i >> 1);
     };
     constexpr int N = DTYPE == STB_F32 ? 2 : 4;
-    float factor = a.scale_log2;
+#pragma unroll
+    for (int s = 0; s < STEPS; s++)
+#pragma unroll
+      for (int i = 0; i < N; i++) q[s][i] = __float_as_uint(live && dim(s, i) < c.width ? row[dim(s, i)] : 0.0f);
+    float up = 1.0f;
     if (HALF) {  // the head's largest magnitude to 2^12
       float top = 0.0f;
 #pragma unroll
       for (int s = 0; s < STEPS; s++)
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-          const float x = live && dim(s, i) < c.width ? row[dim(s, i)] : 0.0f;
-          q[s][i] = __float_as_uint(x);
-          top = fmaxf(top, fabsf(x));
-        }
+        for (int i = 0; i < N; i++) top = fmaxf(top, fabsf(__uint_as_float(q[s][i])));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * a.scale_log2;
       int e = 0;
       if (top > 0.0f && top <= 3.402823466e38f) e = min(126, 12 - ((int)(__float_as_uint(top) >> 23) - 127));
-      unscale = scale_of((uint8_t)(127 - e));
-      const float up = scale_of((uint8_t)(127 + e));
+      up = scale_of((uint8_t)(127 + e));
+      const float down = scale_of((uint8_t)(127 - e));
+      unscale[0] = __shfl_sync(0xffffffffu, down, 8 * t);
+      unscale[1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+    }
 #pragma unroll
-      for (int s = 0; s < STEPS; s++) {
-        float x[4];
+    for (int s = 0; s < STEPS; s++) {
+      float x[N];
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = __uint_as_float(q[s][i]) * factor * up;
+      for (int i = 0; i < N; i++) x[i] = __uint_as_float(q[s][i]) * a.scale_log2 * up;
+      if constexpr (DTYPE == STB_F32) {  // hi, hi, lo, lo
+        split_tf32(x[0], q[s][0], q[s][2]);
+        split_tf32(x[1], q[s][1], q[s][3]);
+      } else if constexpr (DTYPE == STB_BF16) {  // pairs of the first, second and third terms
+        uint16_t u[4][3];
+#pragma unroll
+        for (int i = 0; i < 4; i++) split3_bf16(x[i], u[i][0], u[i][1], u[i][2]);
+#pragma unroll
+        for (int k = 0; k < 3; k++) {
+          q[s][2 * k] = pack2(u[0][k], u[1][k]);
+          q[s][2 * k + 1] = pack2(u[2][k], u[3][k]);
+        }
+      } else {
         uint32_t u[2], v[2];
         split2_pair(x[0], x[1], u);
         split2_pair(x[2], x[3], v);
         q[s][0] = u[0];
-        q[s][1] = u[1];
-        q[s][2] = v[0];
+        q[s][1] = v[0];
+        q[s][2] = u[1];
         q[s][3] = v[1];
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < STEPS; s++) {
-        float x[N];
-#pragma unroll
-        for (int i = 0; i < N; i++) x[i] = live && dim(s, i) < c.width ? row[dim(s, i)] * factor : 0.0f;
-        if constexpr (DTYPE == STB_F32) {
-          split_tf32(x[0], q[s][0], q[s][1]);
-          split_tf32(x[1], q[s][2], q[s][3]);
-        } else {
-          uint16_t u[4][3];
-#pragma unroll
-          for (int i = 0; i < 4; i++) split3_bf16(x[i], u[i][0], u[i][1], u[i][2]);
-          q[s][0] = pack2(u[0][0], u[1][0]);
-          q[s][1] = pack2(u[0][1], u[1][1]);
-          q[s][2] = pack2(u[2][0], u[3][0]);
-          q[s][3] = pack2(u[2][1], u[3][1]);
-          q[s][4] = pack2(u[0][2], u[1][2]);
-          q[s][5] = pack2(u[2][2], u[3][2]);
-        }
       }
     }
 #pragma unroll
-    for (int i = 0; i < NT; i++) o[i][0] = o[i][1] = 0.0f;
-    m1 = m2 = -INFINITY;
-    sum = 0.0f;
+    for (int i = 0; i < NT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+    m1[0] = m1[1] = m2[0] = m2[1] = -INFINITY;
+    sum[0] = sum[1] = 0.0f;
   };
 
-  // Dimension of o[i][j]: E4M3 values come in pairs of neighbouring dimensions, one per result tile.
-  auto dim_of = [&](int i, int j) { return SCALED ? (i >> 1) * 16 + 4 * t + 2 * j + (i & 1) : i * 8 + 2 * t + j; };
+  // o[i][j + 2 k]: head 2 t + j at this dimension (E4M3 values come in pairs of neighbouring dimensions).
+  auto dim_of = [&](int i, int k) { return SCALED ? i * 16 + 2 * g + k : i * 16 + g + 8 * k; };
 
   // The result of an item's tiles that this warp has seen: all of them to y; a part to the block's pieces (a first
   // part, while the ring is in use) or over the warp's own ring (a last part).
   float *const block_pieces = a.pieces + (size_t)blockIdx.x * BLOCK_PIECES;
   float *const my_ring = (float *)(smem + warp * S::STAGES * S::TILE);
   auto finish = [&](bool starts, bool ends) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    if (starts && ends) {
-      const int head = (use.item % chunks_of) * 8 + g;
-      if (head < a.group) {
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], off);
+    float *part = ends ? block_pieces + (2 + warp) * S::PART : my_ring;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const int in_chunk = 2 * t + j, head = (use.item % chunks_of) * 8 + in_chunk;
+      if (starts && ends) {
+        if (head >= a.group) continue;
         float *y = a.y + (a.first + use.b) * a.y_row + (size_t)(use.item / chunks_of * a.group + head) * c.width;
-        const float f = sum != 0.0f ? (HALF ? 1.0f / P_SHIFT : 1.0f) * (SCALED ? exp2f(m2 - m1) : 1.0f) / sum : 0.0f;
+        const float f = (HALF ? 1.0f / P_SHIFT : 1.0f) * (SCALED ? exp2f(m2[j] - m1[j]) : 1.0f) / sum[j];
 #pragma unroll
         for (int i = 0; i < NT; i++)
 #pragma unroll
-          for (int j = 0; j < 2; j++)
-            if (dim_of(i, j) < c.width) y[dim_of(i, j)] = sum != 0.0f ? o[i][j] * f : 0.0f;
+          for (int k = 0; k < 2; k++)
+            if (dim_of(i, k) < c.width) y[dim_of(i, k)] = sum[j] != 0.0f ? o[i][j + 2 * k] * f : 0.0f;
+        continue;
       }
-      return;
+      float *p = part + in_chunk * (WP + 4);
+      if (g == 0) *(float4 *)p = make_float4(m1[j], m2[j], sum[j], 0.0f);
+#pragma unroll
+      for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int k = 0; k < 2; k++) p[4 + dim_of(i, k)] = o[i][j + 2 * k];
     }
-    float *part = (ends ? block_pieces + (2 + warp) * S::PART : my_ring) + g * (WP + 4);
-    if (t == 0) *(float4 *)part = make_float4(m1, m2, sum, 0.0f);
-#pragma unroll
-    for (int i = 0; i < NT; i++)
-#pragma unroll
-      for (int j = 0; j < 2; j++) part[4 + dim_of(i, j)] = o[i][j];
+    if (starts && ends) return;
     if (lane == 0) {
       int *p = s_part[2 * warp + (ends ? 0 : 1)];
       p[0] = use.b;
@@ -527,154 +530,174 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     const uint8_t *m = meta + stage * S::META;
     const uint32_t mask = *(const uint32_t *)m;
 
-    // scores: row g (first terms of q) and row g + 8 (second terms) of the 8-key results
-    float ca[NB][4] = {}, cb[NB][4] = {}, cc[NB][4] = {};
+    // scores: keys as rows, heads as columns; an accumulator per term of q and per parity of the step
+    constexpr int PRODUCTS = DTYPE == STB_F32 ? 3 : TERMS;
+    float acc[MB][PRODUCTS][2][4] = {};
     {
+      const int row = (lane & 7) + ((lane >> 3) & 1) * 8, odd = lane >> 4;
+#pragma unroll
+      for (int s = 0; s < S::CHUNKS / 2; s++)
+#pragma unroll
+        for (int b = 0; b < MB; b++) {
+          uint32_t r[4];
+          load_matrix4(r, chunk_at<S::ROW>(keys, row + 16 * b, 2 * s + odd));
+          if constexpr (SCALED) {  // two steps of 16 dimensions
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              const uint32_t x = r[2 * h], y = r[2 * h + 1];
+              const uint32_t k[4] = {widen_pair(x & 0xffffu), widen_pair(y & 0xffffu), widen_pair(x >> 16), widen_pair(y >> 16)};
+#pragma unroll
+              for (int i = 0; i < 2; i++) product<DTYPE>(acc[b][i][h], k, q[2 * s + h][2 * i], q[2 * s + h][2 * i + 1]);
+            }
+          } else if constexpr (DTYPE == STB_F32) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) split_tf32(__uint_as_float(r[i]), hi[i], lo[i]);
+            product<DTYPE>(acc[b][0][s & 1], hi, q[s][0], q[s][1]);
+            product<DTYPE>(acc[b][1][s & 1], hi, q[s][2], q[s][3]);
+            product<DTYPE>(acc[b][2][s & 1], lo, q[s][0], q[s][1]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < TERMS; i++) product<DTYPE>(acc[b][i][s & 1], r, q[s][2 * i], q[s][2 * i + 1]);
+          }
+        }
+    }
+    float sc[MB][4], sw[SCALED ? MB : 1][4];  // [2 k + j]: key g + 8 k, head 2 t + j
+    bool move = false;
+#pragma unroll
+    for (int b = 0; b < MB; b++)
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const int key = 16 * b + 8 * k + g;
+        const bool live = mask >> key & 1;
+        const float scale = SCALED ? scale_of(m[16 + key]) : 1.0f, up = SCALED ? (float)((int)m[16 + TK + key] - 127) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const int i = 2 * k + j;
+          float x = acc[b][PRODUCTS - 1][0][i] + acc[b][PRODUCTS - 1][1][i];
+#pragma unroll
+          for (int n = PRODUCTS - 2; n >= 0; n--) x += acc[b][n][0][i] + acc[b][n][1][i];
+          if (HALF) x *= unscale[j];
+          if (SCALED) x *= scale;
+          sc[b][i] = live ? x : -INFINITY;
+          move |= sc[b][i] > m1[j] + LAZY;
+          if (SCALED) {
+            sw[b][i] = sc[b][i] + up;
+            move |= sw[b][i] > m2[j] + LAZY;
+          }
+        }
+      }
+    if (__any_sync(0xffffffffu, move)) {  // some score passed its maximum by far: move the heads' maxima
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        float n1 = m1[j], n2 = m2[j];
+#pragma unroll
+        for (int b = 0; b < MB; b++) {
+          n1 = fmaxf(n1, fmaxf(sc[b][j], sc[b][2 + j]));
+          if (SCALED) n2 = fmaxf(n2, fmaxf(sw[b][j], sw[b][2 + j]));
+        }
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, off));
+          if (SCALED) n2 = fmaxf(n2, __shfl_xor_sync(0xffffffffu, n2, off));
+        }
+        if (!SCALED) n2 = n1;
+        const float f1 = n1 == m1[j] ? 1.0f : pow2(m1[j] - n1), f2 = n2 == m2[j] ? 1.0f : pow2(m2[j] - n2);
+        sum[j] *= f1;
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+          o[i][j] *= f2;
+          o[i][2 + j] *= f2;
+        }
+        m1[j] = n1;
+        m2[j] = n2;
+      }
+    }
+    // Weights; a maximum of -inf means that no key has counted yet, and none does here (their scores are -inf).
+    float w[MB][4];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const float base1 = m1[j] == -INFINITY ? 0.0f : m1[j], base2 = m2[j] == -INFINITY ? 0.0f : m2[j];
+#pragma unroll
+      for (int b = 0; b < MB; b++)
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const float p = pow2(sc[b][2 * k + j] - base1);
+          sum[j] += p;
+          w[b][2 * k + j] = SCALED ? pow2(sw[b][2 * k + j] - base2) : p;
+          if (HALF) w[b][2 * k + j] *= P_SHIFT;
+        }
+    }
+
+    // weighted values: dimensions as rows, heads as columns, a fresh result per tile added in Float32
+    if constexpr (DTYPE == STB_F32) {
+      uint32_t hi[2][2], lo[2][2];  // [8-key half][key 2 t + i] of head g
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const int from = (2 * t + i) * 4 + (g >> 1);
+          const float x = __shfl_sync(0xffffffffu, w[0][2 * k], from), y = __shfl_sync(0xffffffffu, w[0][2 * k + 1], from);
+          split_tf32(g & 1 ? y : x, hi[k][i], lo[k][i]);
+        }
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        float r[4] = {};
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          uint32_t vh[4], vl[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {  // dimension g + 8 (i & 1), key 2 t + (i >> 1): the product's slots t and t + 4
+            float v;
+            asm volatile("ld.shared.f32 %0, [%1];"
+                         : "=f"(v)
+                         : "r"(chunk_at<S::ROW>(values, 8 * k + 2 * t + (i >> 1), 4 * n + 2 * (i & 1) + (g >> 2)) + (g & 3) * 4));
+            split_tf32(v, vh[i], vl[i]);
+          }
+          product<DTYPE>(r, vl, hi[k][0], hi[k][1]);
+          product<DTYPE>(r, vh, lo[k][0], lo[k][1]);
+          product<DTYPE>(r, vh, hi[k][0], hi[k][1]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[n][i] += r[i];
+      }
+    } else {
+      uint32_t p[MB][2][TERMS];  // [8-key half] of each term: keys 2 t, 2 t + 1 of head g
+#pragma unroll
+      for (int b = 0; b < MB; b++)
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          if constexpr (DTYPE == STB_BF16) split3_pair(w[b][2 * k], w[b][2 * k + 1], p[b][k]);
+          else split2_pair(w[b][2 * k], w[b][2 * k + 1], p[b][k]);
+#pragma unroll
+          for (int i = 0; i < TERMS; i++) p[b][k][i] = transpose8(p[b][k][i]);
+        }
       const int row = (lane & 7) + (lane >> 4) * 8, odd = (lane >> 3) & 1;
 #pragma unroll
       for (int s = 0; s < S::CHUNKS / 2; s++) {
-        if (2 * s >= row_chunks) continue;
-#pragma unroll
-        for (int n0 = 0; n0 < NB; n0 += 2) {
-          uint32_t r[4];
-          load_matrix4(r, chunk_at<S::ROW>(keys, row + n0 * 8, 2 * s + odd));
-#pragma unroll
-          for (int h = 0; h < 2; h++) {
-            const int n = n0 + h;
-            const uint32_t b0 = r[2 * h], b1 = r[2 * h + 1];
-            if constexpr (SCALED) {  // two steps of 16 dimensions, one register each
-              product<DTYPE>(ca[n], q[2 * s][0], q[2 * s][1], q[2 * s][2], q[2 * s][3], widen_pair(b0 & 0xffffu), widen_pair(b0 >> 16));
-              product<DTYPE>(cb[n], q[2 * s + 1][0], q[2 * s + 1][1], q[2 * s + 1][2], q[2 * s + 1][3], widen_pair(b1 & 0xffffu),
-                             widen_pair(b1 >> 16));
-            } else if constexpr (DTYPE == STB_F32) {
-              uint32_t h0, l0, h1, l1;
-              split_tf32(__uint_as_float(b0), h0, l0);
-              split_tf32(__uint_as_float(b1), h1, l1);
-              product<DTYPE>(s & 1 ? cb[n] : ca[n], q[s][0], q[s][1], q[s][2], q[s][3], h0, h1);
-              product<DTYPE>(cc[n], q[s][0], q[s][1], q[s][2], q[s][3], l0, l1);
-            } else {
-              product<DTYPE>(s & 1 ? cb[n] : ca[n], q[s][0], q[s][1], q[s][2], q[s][3], b0, b1);
-              if constexpr (DTYPE == STB_BF16) product<DTYPE>(cc[n], q[s][4], 0u, q[s][5], 0u, b0, b1);
-            }
-          }
-        }
-      }
-    }
-    float sc[NK], sw[SCALED ? NK : 1], top1 = -INFINITY, top2 = -INFINITY;
-    const uint32_t live = mask >> (2 * t);  // bit (k & 1) + 8 (k >> 1): key 2 t + (k & 1) + 8 (k >> 1) of the tile
-#pragma unroll
-    for (int k = 0; k < NK; k++) {
-      const int n = k >> 1, j = k & 1;
-      sc[k] = (ca[n][j] + cb[n][j]) + ((ca[n][2 + j] + cb[n][2 + j]) + cc[n][j]);
-      if (SCALED) {
-        const int key = 2 * t + j + 8 * n;
-        sc[k] *= unscale * scale_of(m[16 + key]);
-        sw[k] = sc[k] + (float)((int)m[16 + TK + key] - 127);
-      } else if (HALF) {
-        sc[k] *= unscale;
-      }
-      if (!(live >> (j + 8 * n) & 1)) {
-        sc[k] = -INFINITY;
-        if (SCALED) sw[k] = -INFINITY;
-      }
-      top1 = fmaxf(top1, sc[k]);
-      if (SCALED) top2 = fmaxf(top2, sw[k]);
-    }
-    top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 1));
-    top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 2));
-    if (SCALED) {
-      top2 = fmaxf(top2, __shfl_xor_sync(0xffffffffu, top2, 1));
-      top2 = fmaxf(top2, __shfl_xor_sync(0xffffffffu, top2, 2));
-    } else {
-      top2 = top1;
-    }
-    const bool move1 = top1 > m1 + LAZY, move2 = top2 > m2 + LAZY;
-    if (__any_sync(0xffffffffu, move1 || move2)) {
-      const float n1 = move1 ? top1 : m1, n2 = move2 ? top2 : m2;
-      const float f1 = move1 ? pow2(m1 - n1) : 1.0f, f2 = move2 ? pow2(m2 - n2) : 1.0f;
-      sum *= f1;
-#pragma unroll
-      for (int k = 0; k < NT; k++) {
-        o[k][0] *= f2;
-        o[k][1] *= f2;
-      }
-      m1 = n1;
-      m2 = n2;
-    }
-    // Weights; a maximum of -inf means that no key has counted yet, and none does here (their scores are -inf).
-    const float base1 = m1 == -INFINITY ? 0.0f : m1, base2 = m2 == -INFINITY ? 0.0f : m2;
-    float w[NK];
-#pragma unroll
-    for (int k = 0; k < NK; k++) {
-      const float p = pow2(sc[k] - base1);
-      sum += p;
-      w[k] = SCALED ? pow2(sw[k] - base2) : p;
-      if (HALF) w[k] *= P_SHIFT;
-    }
-
-    // weighted values: a fresh result per tile, its rows g and g + 8 added in Float32
-    if constexpr (DTYPE == STB_F32) {
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int k = 0; k < 4; k++) split_tf32(w[k], hi[k], lo[k]);
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-        if (2 * n >= row_chunks) continue;
-        float r[4] = {};
-        uint32_t vh[4], vl[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) {  // keys 2 t, 2 t + 1 of each half as the product's slots t, t + 4
-          const int key = (k >> 1) * 8 + 2 * t + (k & 1);
-          float v;
-          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(chunk_at<S::ROW>(values, key, 2 * n + (g >> 2)) + (g & 3) * 4) : "memory");
-          split_tf32(v, vh[k], vl[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; k += 2) product<DTYPE>(r, hi[k], lo[k], hi[k + 1], lo[k + 1], vl[k], vl[k + 1]);
-#pragma unroll
-        for (int k = 0; k < 4; k += 2) product<DTYPE>(r, hi[k], lo[k], hi[k + 1], lo[k + 1], vh[k], vh[k + 1]);
-        o[n][0] += r[0] + r[2];
-        o[n][1] += r[1] + r[3];
-      }
-    } else {
-      constexpr int TERMS = DTYPE == STB_BF16 ? 3 : 2;
-      uint32_t p[NB][TERMS];  // keys 8 n + 2 t, + 1 of each term
-#pragma unroll
-      for (int n = 0; n < NB; n++) {
-        if constexpr (DTYPE == STB_BF16) split3_pair(w[2 * n], w[2 * n + 1], p[n]);
-        else split2_pair(w[2 * n], w[2 * n + 1], p[n]);
-      }
-      const int row = (lane & 7) + ((lane >> 3) & 1) * 8, odd = lane >> 4;
-      constexpr int PAIR = SCALED ? 4 : 2;  // result tiles of two chunks
-#pragma unroll
-      for (int s = 0; s < S::CHUNKS / 2; s++) {
-        if (2 * s >= row_chunks) continue;
+        constexpr int PAIR = SCALED ? 2 : 1;  // 16-dimension results of two chunks
         float r[PAIR][4] = {};
 #pragma unroll
-        for (int n = 0; n < NB; n += 2) {
-          auto weigh = [&](float (&to)[4], uint32_t b0, uint32_t b1) {
-            if constexpr (DTYPE == STB_BF16) product<DTYPE>(to, p[n][2], 0u, p[n + 1][2], 0u, b0, b1);
-            product<DTYPE>(to, p[n][0], p[n][1], p[n + 1][0], p[n + 1][1], b0, b1);
-          };
+        for (int b = 0; b < MB; b++) {
           uint32_t v[4];
-          load_matrix4_trans(v, chunk_at<S::ROW>(values, row + n * 8, 2 * s + odd));
+          load_matrix4_trans(v, chunk_at<S::ROW>(values, row + 16 * b, 2 * s + odd));
           if constexpr (SCALED) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {  // bytes (key, dim), (key, dim + 1), (key + 1, dim), (key + 1, dim + 1)
-              const uint32_t x = __byte_perm(v[2 * h], 0, 0x3120), z = __byte_perm(v[2 * h + 1], 0, 0x3120);
-              weigh(r[2 * h], widen_pair(x & 0xffffu), widen_pair(z & 0xffffu));
-              weigh(r[2 * h + 1], widen_pair(x >> 16), widen_pair(z >> 16));
+              const uint32_t x = __byte_perm(v[h], 0, 0x3120), z = __byte_perm(v[2 + h], 0, 0x3120);
+              const uint32_t u[4] = {widen_pair(x & 0xffffu), widen_pair(x >> 16), widen_pair(z & 0xffffu), widen_pair(z >> 16)};
+#pragma unroll
+              for (int i = TERMS - 1; i >= 0; i--) product<DTYPE>(r[h], u, p[b][0][i], p[b][1][i]);
             }
           } else {
-            weigh(r[0], v[0], v[1]);
-            weigh(r[1], v[2], v[3]);
+#pragma unroll
+            for (int i = TERMS - 1; i >= 0; i--) product<DTYPE>(r[0], v, p[b][0][i], p[b][1][i]);
           }
         }
 #pragma unroll
-        for (int k = 0; k < PAIR; k++) {
-          o[PAIR * s + k][0] += r[k][0] + r[k][2];
-          o[PAIR * s + k][1] += r[k][1] + r[k][3];
-        }
+        for (int h = 0; h < PAIR; h++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) o[PAIR * s + h][i] += r[h][i];
       }
     }
 
