@@ -39,7 +39,7 @@ struct AttendArgs {
   int heads, group, batch, first;  // requests first .. first + batch - 1 of the call
   float scale_log2;                // log2(e) / sqrt(width)
   float *pieces;                   // per block: two of its own, then one per warp
-  int *arrived;                    // per block, zero between calls
+  int *arrived;                    // per block and head, zero between calls
 };
 
 __device__ __forceinline__ int attend_length(const PagedView &c, const AttendArgs &a, int b) {
@@ -258,11 +258,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
   int *s_start = (int *)(s_meta + S::WARPS * S::STAGES * S::META);  // tiles before request b, of one item each
   int *s_len = s_start + MAX_BATCH + 1;
   __shared__ int s_scan[S::WARPS];
-  __shared__ float s_weight[MAX_GRID][8];  // of the parts that are joined
-  __shared__ __align__(16) float s_head[8][4];  // joined maxima and sum per head
   __shared__ int s_part[2 * S::WARPS][4];  // a warp's first and last part: request (or -1), item, whether it starts / ends it
-  __shared__ int s_list[2 * S::WARPS];     // entries of s_part that are joined
-  __shared__ int s_last;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int chunks_of = (a.group + 7) / 8, items = c.kv_heads * chunks_of;
@@ -397,8 +393,15 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       };
       if (mask == 0xffffffffu) copy(std::true_type());
       else copy(std::false_type());
+      const int item = load.item, b = load.b;
       advance(load);
       issued++;
+      if ((load.item != item || load.b != b) && issued < todo) {  // the next item's q to L1, ahead of its use
+        const int chunk = load.item % chunks_of;
+        const float *row = a.q + (a.first + load.b) * a.q_row + (size_t)(load.item / chunks_of * a.group + chunk * 8) * c.width;
+        for (int i = lane * 32; i < min(8, a.group - chunk * 8) * c.width; i += 1024)
+          asm volatile("prefetch.global.L1 [%0];" ::"l"(row + i));
+      }
       page = page_ahead(issued < todo);
     }
     copy_commit();
@@ -407,22 +410,24 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
   uint32_t q[STEPS][2 * TERMS];
   float o[NT][4], m1[2], m2[2], sum[2], unscale[2] = {1.0f, 1.0f};
 
-  // q of the item at `use` into operand registers, scaled by log2(e) / sqrt(width).
+  // q of the item at `use` into registers: dimensions of this lane in step s, two pairs (F32: two single ones).
+  constexpr int N = DTYPE == STB_F32 ? 2 : 4;
   auto load_query = [&]() {
     const int kvh = use.item / chunks_of, head = (use.item % chunks_of) * 8 + g;
     const bool live = head < a.group;
     const float *row = a.q + (a.first + use.b) * a.q_row + (size_t)(kvh * a.group + head) * c.width;
-    // dimensions of this lane in step s: two pairs (F32: two single ones)
     auto dim = [&](int s, int i) {
       if (DTYPE == STB_F32) return s * 8 + t + 4 * i;
       if (SCALED) return s * 16 + 4 * t + i;
       return s * 16 + 2 * t + (i & 1) + 8 * (i >> 1);
     };
-    constexpr int N = DTYPE == STB_F32 ? 2 : 4;
 #pragma unroll
     for (int s = 0; s < STEPS; s++)
 #pragma unroll
       for (int i = 0; i < N; i++) q[s][i] = __float_as_uint(live && dim(s, i) < c.width ? row[dim(s, i)] : 0.0f);
+  };
+  // Its operand terms, scaled by log2(e) / sqrt(width), and a fresh state.
+  auto start_item = [&]() {
     float up = 1.0f;
     if (HALF) {  // the head's largest magnitude to 2^12
       float top = 0.0f;
@@ -516,9 +521,10 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     }
   };
 
+  if (todo > 0) load_query();  // before the copies: its loads would queue behind them
 #pragma unroll 1
   for (int i = 0; i < S::STAGES - 1; i++) issue(i);
-  if (todo > 0) load_query();
+  start_item();
   bool starts = use.tile == 0;
   int stage = 0;
 #pragma unroll 1
@@ -705,7 +711,10 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       finish(starts, true);
       advance(use);
       starts = true;
-      if (i + 1 < todo) load_query();
+      if (i + 1 < todo) {
+        load_query();
+        start_item();
+      }
     } else if (i + 1 == todo) {
       copy_wait<0>();
       __syncwarp();
@@ -718,114 +727,128 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
   copy_wait<0>();
   __syncthreads();
 
-  // Joins the parts of one item: `count` of them, part i at place(i) (`far`: written by other blocks); the result to y,
-  // or to `piece` as a part again.
-  auto join = [&](int count, auto far, auto place, int b, int item, float *piece) {
-    auto get = [](const float *p) { return decltype(far)::value ? __ldcg((const float4 *)p) : *(const float4 *)p; };
-    constexpr int MOST = decltype(far)::value ? MAX_GRID / 32 : (2 * S::WARPS + 31) / 32;
-    for (int h = warp; h < 8; h += S::WARPS) {  // a warp per head, a lane per part
-      float4 part[MOST];
-      float n1 = -INFINITY, n2 = -INFINITY, all = 0.0f;
+  // Joins the parts of the items that this block covers in part, a warp per head, without another block barrier.
+  constexpr int FAR = MAX_GRID / 32;
+  auto write = [&](int b, int item, int h, int d, float4 v, float n1, float n2, float all) {
+    const int head = item % chunks_of * 8 + h;
+    if (head >= a.group) return;
+    float *y = a.y + (a.first + b) * a.y_row + (size_t)(item / chunks_of * a.group + head) * c.width + d;
+    const float f = (HALF ? 1.0f / P_SHIFT : 1.0f) * (SCALED ? exp2f(n2 - n1) : 1.0f) / all;
+    const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int k = 0; k < MOST; k++) {
-        part[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (k * 32 + lane < count) part[k] = get(place(k * 32 + lane) + h * (WP + 4));
+    for (int i = 0; i < 4; i++)
+      if (d + i < c.width) y[i] = all != 0.0f ? x[i] * f : 0.0f;
+  };
+  auto add = [](float4 &v, const float4 &x, float f) {
+    if (f == 0.0f) return;  // a part without a key may hold anything
+    v.x = fmaf(x.x, f, v.x);
+    v.y = fmaf(x.y, f, v.y);
+    v.z = fmaf(x.z, f, v.z);
+    v.w = fmaf(x.w, f, v.w);
+  };
+  auto most = [](float x) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
+    return x;
+  };
+  auto total_of = [](float x) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+    return x;
+  };
+  constexpr int WIDE = (WP + 127) / 128;  // float4 of a lane
+  const int mine_b = lane < 2 * S::WARPS ? s_part[lane][0] : -1, mine_item = lane < 2 * S::WARPS ? s_part[lane][1] : -1;
+  // the part of entry `lane`
+  const float *const mine_at = lane & 1 ? (const float *)(smem + (lane >> 1) * S::STAGES * S::TILE) : block_pieces + (2 + (lane >> 1)) * S::PART;
+  uint32_t left = __ballot_sync(0xffffffffu, mine_b >= 0);
+#pragma unroll 1
+  while (left) {
+    const int i0 = __ffs(left) - 1;
+    const int b = __shfl_sync(0xffffffffu, mine_b, i0), item = __shfl_sync(0xffffffffu, mine_item, i0);
+    const uint32_t which = __ballot_sync(0xffffffffu, mine_b == b && mine_item == item);
+    left &= ~which;
+    const bool whole = s_part[i0][2] && s_part[31 - __clz(which)][3];
+    const int tiles = s_start[b + 1] - s_start[b], first = s_start[b] * items + item * tiles;
+    float *piece = block_pieces + (block0 >= first ? 0 : 1) * S::PART;
+    const int c0 = whole ? 0 : stretch_of(first, total, grid), c1 = whole ? 0 : stretch_of(first + tiles - 1, total, grid);
+#pragma unroll 1
+    for (int h = warp; h < 8; h += S::WARPS) {
+      const int row = h * (WP + 4);
+      const bool has = which >> lane & 1;
+      float4 part = has ? *(const float4 *)(mine_at + row) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float n1 = most(part.z != 0.0f ? part.x : -INFINITY), n2 = most(part.z != 0.0f ? part.y : -INFINITY);
+      float all = total_of(part.z != 0.0f ? part.z * exp2f(part.x - n1) : 0.0f);
+      const float factor = part.z != 0.0f ? exp2f(part.y - n2) : 0.0f;
+      float4 v[WIDE] = {};
+      for (uint32_t m = which; m; m &= m - 1) {
+        const int i = __ffs(m) - 1;
+        const float f = __shfl_sync(0xffffffffu, factor, i);
+        const float *at = i & 1 ? (const float *)(smem + (i >> 1) * S::STAGES * S::TILE) : block_pieces + (2 + (i >> 1)) * S::PART;
+#pragma unroll
+        for (int k = 0; k < WIDE; k++)
+          if (k * 128 + lane * 4 < WP) add(v[k], *(const float4 *)(at + row + 4 + k * 128 + lane * 4), f);
       }
+      if (whole) {
 #pragma unroll
-      for (int k = 0; k < MOST; k++)
-        if (part[k].z != 0.0f) {
-          n1 = fmaxf(n1, part[k].x);
-          n2 = fmaxf(n2, part[k].y);
-        }
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) {
-        n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, off));
-        n2 = fmaxf(n2, __shfl_xor_sync(0xffffffffu, n2, off));
-      }
-#pragma unroll
-      for (int k = 0; k < MOST; k++) {
-        if (part[k].z != 0.0f) all += part[k].z * exp2f(part[k].x - n1);
-        if (k * 32 + lane < count) s_weight[k * 32 + lane][h] = part[k].z != 0.0f ? exp2f(part[k].y - n2) : 0.0f;
-      }
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
-      if (lane == 0) *(float4 *)s_head[h] = make_float4(n1, n2, all, 0.0f);
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < 2 * WP; e += S::THREADS) {
-      const int h = e / (WP / 4), d = e % (WP / 4) * 4;
-      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-      for (int i = 0; i < count; i++) {
-        const float4 x = get(place(i) + h * (WP + 4) + 4 + d);
-        const float f = s_weight[i][h];
-        if (f != 0.0f) {  // a part without a key may hold anything
-          v.x = fmaf(x.x, f, v.x);
-          v.y = fmaf(x.y, f, v.y);
-          v.z = fmaf(x.z, f, v.z);
-          v.w = fmaf(x.w, f, v.w);
-        }
-      }
-      const float4 top = *(const float4 *)s_head[h];
-      if (piece) {
-        *(float4 *)(piece + h * (WP + 4) + 4 + d) = v;
-        if (d == 0) *(float4 *)(piece + h * (WP + 4)) = top;
+        for (int k = 0; k < WIDE; k++)
+          if (k * 128 + lane * 4 < WP) write(b, item, h, k * 128 + lane * 4, v[k], n1, n2, all);
         continue;
       }
-      const int head = item % chunks_of * 8 + h;
-      if (head >= a.group) continue;
-      float *y = a.y + (a.first + b) * a.y_row + (size_t)(item / chunks_of * a.group + head) * c.width + d;
-      const float f = top.z != 0.0f ? (HALF ? 1.0f / P_SHIFT : 1.0f) * (SCALED ? exp2f(top.y - top.x) : 1.0f) / top.z : 0.0f;
-      if (d < c.width) y[0] = f != 0.0f ? v.x * f : 0.0f;
-      if (d + 1 < c.width) y[1] = f != 0.0f ? v.y * f : 0.0f;
-      if (d + 2 < c.width) y[2] = f != 0.0f ? v.z * f : 0.0f;
-      if (d + 3 < c.width) y[3] = f != 0.0f ? v.w * f : 0.0f;
-    }
-  };
-
-  for (int i = 0; i < 2 * S::WARPS;) {
-    const int b = s_part[i][0], item = s_part[i][1];
-    if (b < 0) {
-      i++;
-      continue;
-    }
-    const bool first = s_part[i][2];
-    int count = 0;
-    bool last = false;
-    uint32_t which = 0;  // entries of this item
-    for (; i < 2 * S::WARPS && (s_part[i][0] < 0 || (s_part[i][0] == b && s_part[i][1] == item)); i++)
-      if (s_part[i][0] >= 0) {
-        which |= 1u << i;
-        count++;
-        last = s_part[i][3];
-      }
-    if (threadIdx.x < 2 * S::WARPS && (which >> threadIdx.x & 1)) s_list[__popc(which & ((1u << threadIdx.x) - 1))] = threadIdx.x;
-    __syncthreads();
-    auto of_block = [&](int k) -> const float * {
-      const int i = s_list[k];
-      return i & 1 ? (const float *)(smem + (i >> 1) * S::STAGES * S::TILE) : block_pieces + (2 + (i >> 1)) * S::PART;
-    };
-    const int tiles = s_start[b + 1] - s_start[b], i0 = s_start[b] * items + item * tiles;
-    float *piece = first && last ? nullptr : block_pieces + (block0 >= i0 ? 0 : 1) * S::PART;
-    join(count, std::false_type(), of_block, b, item, piece);
-    if (piece) {
-      const int c0 = stretch_of(i0, total, grid), c1 = stretch_of(i0 + tiles - 1, total, grid);
+      if (lane == 0) *(float4 *)(piece + row) = make_float4(n1, n2, all, 0.0f);
+#pragma unroll
+      for (int k = 0; k < WIDE; k++)
+        if (k * 128 + lane * 4 < WP) *(float4 *)(piece + row + 4 + k * 128 + lane * 4) = v[k];
       __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        s_last = atomicAdd(a.arrived + c0, 1) == c1 - c0;
-        if (s_last) a.arrived[c0] = 0;
+      __syncwarp();
+      int last = 0;
+      if (lane == 0) {  // the head's counter of the item's first block; the last block to arrive joins, and clears it
+        last = atomicAdd(a.arrived + c0 * 8 + h, 1) == c1 - c0;
+        if (last) a.arrived[c0 * 8 + h] = 0;
       }
-      __syncthreads();
-      if (s_last) {
-        __threadfence();
-        auto of_blocks = [&](int k) -> const float * {
-          return a.pieces + (size_t)(c0 + k) * BLOCK_PIECES + (stretch_start(c0 + k, total, grid) >= i0 ? 0 : 1) * S::PART;
-        };
-        join(c1 - c0 + 1, std::true_type(), of_blocks, b, item, nullptr);
+      if (!__shfl_sync(0xffffffffu, last, 0)) continue;
+      __threadfence();
+      const int count = c1 - c0 + 1;
+      auto piece_of = [&](int k) {
+        return a.pieces + (size_t)(c0 + k) * BLOCK_PIECES + (stretch_start(c0 + k, total, grid) >= first ? 0 : 1) * S::PART + row;
+      };
+      float4 far[FAR];
+      n1 = n2 = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < FAR; k++) {
+        far[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (k * 32 + lane < count) far[k] = __ldcg((const float4 *)piece_of(k * 32 + lane));
       }
+#pragma unroll
+      for (int k = 0; k < FAR; k++)
+        if (far[k].z != 0.0f) {
+          n1 = fmaxf(n1, far[k].x);
+          n2 = fmaxf(n2, far[k].y);
+        }
+      n1 = most(n1);
+      n2 = most(n2);
+      all = 0.0f;
+#pragma unroll
+      for (int k = 0; k < FAR; k++) {
+        if (far[k].z != 0.0f) all += far[k].z * exp2f(far[k].x - n1);
+        far[k].w = far[k].z != 0.0f ? exp2f(far[k].y - n2) : 0.0f;
+      }
+      all = total_of(all);
+#pragma unroll
+      for (int k = 0; k < WIDE; k++) v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int r = 0; r < FAR; r++)
+#pragma unroll 8
+        for (int i = 0; i < min(32, count - r * 32); i++) {
+          const float f = __shfl_sync(0xffffffffu, far[r].w, i);
+          const float *at = piece_of(r * 32 + i) + 4;
+#pragma unroll
+          for (int k = 0; k < WIDE; k++)
+            if (k * 128 + lane * 4 < WP) add(v[k], __ldcg((const float4 *)(at + k * 128 + lane * 4)), f);
+        }
+#pragma unroll
+      for (int k = 0; k < WIDE; k++)
+        if (k * 128 + lane * 4 < WP) write(b, item, h, k * 128 + lane * 4, v[k], n1, n2, all);
     }
-    __syncthreads();
   }
 }
 
@@ -894,7 +917,7 @@ extern "C" int stb_op_paged_attention(stb_session *s, const stb_paged_cache *cac
       count_launch(s);
       return;
     }
-    const uint64_t counters = MAX_GRID * sizeof(int), bytes = counters + (uint64_t)MAX_GRID * BLOCK_PIECES * sizeof(float);
+    const uint64_t counters = MAX_GRID * 8 * sizeof(int), bytes = counters + (uint64_t)MAX_GRID * BLOCK_PIECES * sizeof(float);
     if (!s->paged_ws) {
       if (capturing(s)) throw Error(STB_ERR_STATE, "a session's first paged attention cannot be captured: make a call before");
       s->paged_ws = session_alloc(s, bytes);
