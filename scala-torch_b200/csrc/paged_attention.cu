@@ -110,10 +110,11 @@ __global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedVie
 // ------------------------------------------------------------------ rows of whole 16-byte chunks, width <= 256
 
 constexpr int MAX_GRID = 160;
+constexpr int DIRECT_TILES = 64;     // most tiles of an item that one block takes alone
 constexpr int BLOCK_PIECES = 20800;  // floats of a block's pieces, at most: (2 + warps) of 8 heads x (width + 4)
 constexpr int MAX_BATCH = 1024;      // requests of one launch (their prefix sums lie in shared memory)
 constexpr float LAZY = 8.0f;         // a maximum moves only when a score passes it by 2^8
-constexpr float P_SHIFT = 128.0f;    // F16 weights times 2^7: at most 2^15, and 2^-32 apart at their lowest
+constexpr float P_SHIFT = 7.0f, P_SCALE = 128.0f;  // F16 weights times 2^7: at most 2^15, and 2^-32 apart at their lowest
 
 template <int DTYPE, int WP>
 struct Shape {
@@ -123,14 +124,15 @@ struct Shape {
   static constexpr int TK = ROW >= 256 ? 16 : 32; // keys of a tile: 8 KB where the width allows
   static constexpr int TILE = 2 * TK * ROW;       // keys and values of a tile
   // Warps and stages that fill about 192 KB: at least two stages in flight per warp, 128 KB per SM.
-  static constexpr int WARPS = TILE <= 8192 ? 8 : (TILE <= 16384 ? 4 : 2);
+  // E4M3 has the most arithmetic per byte: twelve warps of two stages (three warps per scheduler to fill).
+  static constexpr int WARPS = TILE <= 8192 ? (DTYPE == STB_E4M3 && WP == 128 ? 12 : 8) : (TILE <= 16384 ? 4 : 2);
   static constexpr int STAGES = 196608 / (WARPS * TILE) < 6 ? 196608 / (WARPS * TILE) : 6;
-  static constexpr int META = 80;                 // per stage: valid mask, scale bytes of keys and values
+  static constexpr int META = 16 + (DTYPE == STB_E4M3 ? TK * 8 : 0);  // per stage: valid mask, scales of keys and values
   static constexpr int THREADS = WARPS * 32;
   static constexpr int RING = WARPS * STAGES * TILE;
   static constexpr int PART = 8 * (WP + 4);       // floats of a partial result: per head max, weight max, sum, -, values
   static constexpr int SMEM = RING + WARPS * STAGES * META + (2 * MAX_BATCH + 4) * 4;
-  static_assert(STAGES >= 3 && SMEM + 8192 <= 232448, "shared memory per block");
+  static_assert(STAGES >= 2 && SMEM + 1024 <= 232448, "shared memory per block");
   static_assert(STAGES * TILE >= PART * 4, "a warp's last part reuses its ring");
   static_assert((2 + WARPS) * PART <= BLOCK_PIECES, "workspace");
 };
@@ -196,9 +198,7 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) 
   lo = (__float_as_uint(x - __uint_as_float(hi)) + 0x1000u) & 0xffffe000u;
 }
 
-__device__ __forceinline__ uint32_t pack2(uint16_t lo, uint16_t hi) { return (uint32_t)lo | ((uint32_t)hi << 16); }
-
-// Three BF16 terms of two finite weights >= 0: rounded, rest rounded, rest rounded (rests are exact).
+// Three BF16 terms of two values: rounded, rest rounded, rest rounded (rests are exact).
 __device__ __forceinline__ void split3_pair(float x, float y, uint32_t (&t)[3]) {
 #pragma unroll
   for (int i = 0; i < 3; i++) {
@@ -264,8 +264,37 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
   const int chunks_of = (a.group + 7) / 8, items = c.kv_heads * chunks_of;
   const int row_chunks = c.width * S::ESZ / 16, row_bytes = row_chunks * 16;
 
-  // Prefix sums of the requests' tiles, and zeros for the empty ones.
-  {
+  for (int i = threadIdx.x; i < 2 * S::WARPS; i += S::THREADS) s_part[i][0] = -1;
+  if (c.width != WP)  // chunks behind the row are read as zeros and never written
+    for (int i = threadIdx.x; i < S::RING / 16; i += S::THREADS) ((uint4 *)smem)[i] = make_uint4(0, 0, 0, 0);
+
+  // Few short items: one block each, no line, nothing to join between blocks (`direct`).
+  bool direct = false;
+  if (a.batch * items <= (int)gridDim.x) {
+    bool deep = false;
+    for (int b = threadIdx.x; b < a.batch; b += S::THREADS) deep |= a.lengths[a.first + b] > DIRECT_TILES * TK;
+    direct = !__syncthreads_or(deep);
+  }
+  Cursor load, use;
+  int total = 0, grid = 0, block0 = 0, t0, todo;
+  if (direct) {
+    if ((int)blockIdx.x >= a.batch * items) return;
+    load.b = blockIdx.x / items;
+    load.item = blockIdx.x % items;
+    load.n = attend_length(c, a, a.first + load.b);
+    load.tiles = (load.n + TK - 1) / TK;
+    if (load.n == 0) {
+      for (int h = load.item % chunks_of * 8; h < min(a.group, (load.item % chunks_of + 1) * 8); h++)
+        for (int i = threadIdx.x; i < c.width; i += S::THREADS)
+          a.y[(a.first + load.b) * a.y_row + (size_t)(load.item / chunks_of * a.group + h) * c.width + i] = 0.0f;
+      return;
+    }
+    const int warps = min(S::WARPS, (load.tiles + 1) / 2);  // two tiles cost less than a join
+    t0 = stretch_start(min(warp, warps), load.tiles, warps);
+    todo = stretch_start(min(warp + 1, warps), load.tiles, warps) - t0;
+    load.tile = t0;
+  } else {
+    // Prefix sums of the requests' tiles, and zeros for the empty ones.
     const int per = (a.batch + S::THREADS - 1) / S::THREADS, b0 = threadIdx.x * per, b1 = min(a.batch, b0 + per);
     int own = 0;
     for (int b = b0; b < b1; b++) {
@@ -280,9 +309,6 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       if (lane >= off) before += v;
     }
     if (lane == 31) s_scan[warp] = before;
-    for (int i = threadIdx.x; i < 2 * S::WARPS; i += S::THREADS) s_part[i][0] = -1;
-    if (c.width != WP)  // chunks behind the row are read as zeros and never written
-      for (int i = threadIdx.x; i < S::RING / 16; i += S::THREADS) ((uint4 *)smem)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     before -= own;
     for (int w = 0; w < warp; w++) before += s_scan[w];
@@ -292,23 +318,17 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       if (b == a.batch - 1) s_start[a.batch] = before;
     }
     __syncthreads();
-  }
-  for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
-    if (s_len[b] == 0)
-      for (int i = threadIdx.x; i < a.heads * c.width; i += S::THREADS) a.y[(a.first + b) * a.y_row + i] = 0.0f;
+    for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
+      if (s_len[b] == 0)
+        for (int i = threadIdx.x; i < a.heads * c.width; i += S::THREADS) a.y[(a.first + b) * a.y_row + i] = 0.0f;
 
-  const int total = s_start[a.batch] * items;
-  const int grid = min((int)gridDim.x, (total + S::WARPS - 1) / S::WARPS);
-  if ((int)blockIdx.x >= grid) return;
-  const int block0 = stretch_start(blockIdx.x, total, grid), mine = stretch_start(blockIdx.x + 1, total, grid) - block0;
-  const int t0 = block0 + stretch_start(warp, mine, S::WARPS);
-  const int todo = block0 + stretch_start(warp + 1, mine, S::WARPS) - t0;
-
-  const uint32_t ring = shared_u32(smem) + warp * S::STAGES * S::TILE;
-  uint8_t *meta = s_meta + warp * S::STAGES * S::META;
-
-  Cursor load, use;
-  {
+    total = s_start[a.batch] * items;
+    grid = min((int)gridDim.x, (total + 2 * S::WARPS - 1) / (2 * S::WARPS));
+    if ((int)blockIdx.x >= grid) return;
+    block0 = stretch_start(blockIdx.x, total, grid);
+    const int mine = stretch_start(blockIdx.x + 1, total, grid) - block0;
+    t0 = block0 + stretch_start(warp, mine, S::WARPS);
+    todo = block0 + stretch_start(warp + 1, mine, S::WARPS) - t0;
     int lo = 0, hi = a.batch - 1;  // the last request that starts at or before t0 (the empty ones before it share its start)
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -321,10 +341,13 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     const int in = t0 - s_start[lo] * items;
     load.item = load.tiles ? in / load.tiles : 0;
     load.tile = load.tiles ? in % load.tiles : 0;
-    use = load;
   }
+  use = load;
+
+  const uint32_t ring = shared_u32(smem) + warp * S::STAGES * S::TILE;
+  uint8_t *meta = s_meta + warp * S::STAGES * S::META;
   auto advance = [&](Cursor &k) {
-    if (++k.tile < k.tiles) return;
+    if (++k.tile < k.tiles || direct) return;
     k.tile = 0;
     if (++k.item < items) return;
     k.item = 0;
@@ -350,12 +373,11 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     return c.tables[(size_t)(a.first + load.b) * c.blocks + (page_shift >= 0 ? key >> page_shift : key / c.page_size)];
   };
   int issued = 0, page = page_ahead(todo > 0);
-  uint32_t scales = 0;
-  uint8_t *scales_to = nullptr;
+  int key_scale = 0, value_scale = 0;
+  float2 *scales_to = nullptr;
   auto issue = [&](int stage) {
     if (SCALED && scales_to) {
-      scales_to[0] = (uint8_t)scales;
-      scales_to[TK] = (uint8_t)(scales >> 8);
+      *scales_to = make_float2(scale_of((uint8_t)key_scale), (float)(value_scale - 127));
       scales_to = nullptr;
     }
     if (issued < todo) {
@@ -371,8 +393,9 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       uint8_t *m = meta + stage * S::META;
       if (lane == 0) *(uint32_t *)m = mask;
       if (SCALED) {
-        scales = live ? c.scale[0][at] | (uint32_t)c.scale[1][at] << 8 : 0x7f7fu;
-        scales_to = m + 16 + my_key;
+        key_scale = live ? c.scale[0][at] : 127;
+        value_scale = live ? c.scale[1][at] : 127;
+        scales_to = (float2 *)(m + 16) + my_key;
       }
       const uint32_t dst = ring + stage * S::TILE;
       auto copy = [&](auto all) {
@@ -453,13 +476,13 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
         split_tf32(x[0], q[s][0], q[s][2]);
         split_tf32(x[1], q[s][1], q[s][3]);
       } else if constexpr (DTYPE == STB_BF16) {  // pairs of the first, second and third terms
-        uint16_t u[4][3];
-#pragma unroll
-        for (int i = 0; i < 4; i++) split3_bf16(x[i], u[i][0], u[i][1], u[i][2]);
+        uint32_t u[3], v[3];
+        split3_pair(x[0], x[1], u);
+        split3_pair(x[2], x[3], v);
 #pragma unroll
         for (int k = 0; k < 3; k++) {
-          q[s][2 * k] = pack2(u[0][k], u[1][k]);
-          q[s][2 * k + 1] = pack2(u[2][k], u[3][k]);
+          q[s][2 * k] = u[k];
+          q[s][2 * k + 1] = v[k];
         }
       } else {
         uint32_t u[2], v[2];
@@ -496,7 +519,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       if (starts && ends) {
         if (head >= a.group) continue;
         float *y = a.y + (a.first + use.b) * a.y_row + (size_t)(use.item / chunks_of * a.group + head) * c.width;
-        const float f = (HALF ? 1.0f / P_SHIFT : 1.0f) * (SCALED ? exp2f(m2[j] - m1[j]) : 1.0f) / sum[j];
+        const float f = (HALF ? 1.0f / P_SCALE : 1.0f) * (SCALED ? exp2f(m2[j] - m1[j]) : 1.0f) / sum[j];
 #pragma unroll
         for (int i = 0; i < NT; i++)
 #pragma unroll
@@ -521,17 +544,29 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     }
   };
 
-  if (todo > 0) load_query();  // before the copies: its loads would queue behind them
-#pragma unroll 1
-  for (int i = 0; i < S::STAGES - 1; i++) issue(i);
-  start_item();
+  // One loop for the first copies (i < 0) and the tiles: every long piece of code stands once, for the sake of the
+  // instruction cache -- a short call runs all of it cold.
   bool starts = use.tile == 0;
-  int stage = 0;
+  int want = 2;  // 2: q of the item at `use` has to be read, 1: it is on its way
+  int stage = 0, next = 0;
 #pragma unroll 1
-  for (int i = 0; i < todo; i++) {
-    copy_wait<S::STAGES - 2>();
-    __syncwarp();  // every lane's copies of this tile are there, and the tile before it has been read
-    issue(stage == 0 ? S::STAGES - 1 : stage - 1);
+  for (int i = todo > 0 ? 1 - S::STAGES : 0; i < todo; i++) {
+    if (want == 2) {  // before the copies: these loads would queue behind them
+      load_query();
+      want = 1;
+    }
+    if (i >= 0) {
+      copy_wait<S::STAGES - 2>();
+      __syncwarp();  // every lane's copies of this tile are there, and the tile before it has been read
+    }
+    issue(next);
+    next = next + 1 == S::STAGES ? 0 : next + 1;
+    if (i < 0) continue;
+    if (SCALED && S::STAGES == 2) __syncwarp();  // the tile's scales, stored just now
+    if (want == 1) {
+      start_item();
+      want = 0;
+    }
     const uint32_t keys = ring + stage * S::TILE, values = keys + TK * S::ROW;
     const uint8_t *m = meta + stage * S::META;
     const uint32_t mask = *(const uint32_t *)m;
@@ -574,24 +609,33 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     for (int b = 0; b < MB; b++)
 #pragma unroll
       for (int k = 0; k < 2; k++) {
-        const int key = 16 * b + 8 * k + g;
-        const bool live = mask >> key & 1;
-        const float scale = SCALED ? scale_of(m[16 + key]) : 1.0f, up = SCALED ? (float)((int)m[16 + TK + key] - 127) : 0.0f;
+        float2 scale = make_float2(1.0f, 0.0f);
+        if (SCALED) scale = ((const float2 *)(m + 16))[16 * b + 8 * k + g];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
           const int i = 2 * k + j;
           float x = acc[b][PRODUCTS - 1][0][i] + acc[b][PRODUCTS - 1][1][i];
 #pragma unroll
           for (int n = PRODUCTS - 2; n >= 0; n--) x += acc[b][n][0][i] + acc[b][n][1][i];
-          if (HALF) x *= unscale[j];
-          if (SCALED) x *= scale;
-          sc[b][i] = live ? x : -INFINITY;
-          move |= sc[b][i] > m1[j] + LAZY;
-          if (SCALED) {
-            sw[b][i] = sc[b][i] + up;
-            move |= sw[b][i] > m2[j] + LAZY;
-          }
+          if (HALF) x *= SCALED ? unscale[j] * scale.x : unscale[j];
+          sc[b][i] = x;
+          if (SCALED) sw[b][i] = x + scale.y;
         }
+      }
+    if (mask != 0xffffffffu) {
+#pragma unroll
+      for (int b = 0; b < MB; b++)
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+          if (!(mask >> (16 * b + 8 * k + g) & 1))
+            sc[b][2 * k] = sc[b][2 * k + 1] = sw[SCALED ? b : 0][2 * k] = sw[SCALED ? b : 0][2 * k + 1] = -INFINITY;
+    }
+#pragma unroll
+    for (int b = 0; b < MB; b++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        move |= sc[b][i] > m1[i & 1] + LAZY;
+        if (SCALED) move |= sw[b][i] > m2[i & 1] + LAZY;
       }
     if (__any_sync(0xffffffffu, move)) {  // some score passed its maximum by far: move the heads' maxima
 #pragma unroll
@@ -623,15 +667,14 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     float w[MB][4];
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-      const float base1 = m1[j] == -INFINITY ? 0.0f : m1[j], base2 = m2[j] == -INFINITY ? 0.0f : m2[j];
+      const float base1 = m1[j] == -INFINITY ? 0.0f : m1[j], base2 = m2[j] == -INFINITY ? 0.0f : m2[j] - P_SHIFT;
 #pragma unroll
       for (int b = 0; b < MB; b++)
 #pragma unroll
         for (int k = 0; k < 2; k++) {
           const float p = pow2(sc[b][2 * k + j] - base1);
           sum[j] += p;
-          w[b][2 * k + j] = SCALED ? pow2(sw[b][2 * k + j] - base2) : p;
-          if (HALF) w[b][2 * k + j] *= P_SHIFT;
+          w[b][2 * k + j] = SCALED ? pow2(sw[b][2 * k + j] - base2) : (HALF ? p * P_SCALE : p);
         }
     }
 
@@ -707,21 +750,17 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       }
     }
 
-    if (use.tile + 1 == use.tiles) {
-      finish(starts, true);
-      advance(use);
-      starts = true;
-      if (i + 1 < todo) {
-        load_query();
-        start_item();
+    const bool ends = use.tile + 1 == use.tiles;
+    if (ends || i + 1 == todo) {
+      if (!ends) {  // the part goes over the ring
+        copy_wait<0>();
+        __syncwarp();
       }
-    } else if (i + 1 == todo) {
-      copy_wait<0>();
-      __syncwarp();
-      finish(starts, false);
-    } else {
-      use.tile++;
+      finish(starts, ends);
+      starts = true;
+      want = 2;
     }
+    advance(use);
     stage = stage + 1 == S::STAGES ? 0 : stage + 1;
   }
   copy_wait<0>();
@@ -733,7 +772,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     const int head = item % chunks_of * 8 + h;
     if (head >= a.group) return;
     float *y = a.y + (a.first + b) * a.y_row + (size_t)(item / chunks_of * a.group + head) * c.width + d;
-    const float f = (HALF ? 1.0f / P_SHIFT : 1.0f) * (SCALED ? exp2f(n2 - n1) : 1.0f) / all;
+    const float f = (HALF ? 1.0f / P_SCALE : 1.0f) * (SCALED ? exp2f(n2 - n1) : 1.0f) / all;
     const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -768,7 +807,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     const uint32_t which = __ballot_sync(0xffffffffu, mine_b == b && mine_item == item);
     left &= ~which;
     const bool whole = s_part[i0][2] && s_part[31 - __clz(which)][3];
-    const int tiles = s_start[b + 1] - s_start[b], first = s_start[b] * items + item * tiles;
+    const int tiles = whole ? 0 : s_start[b + 1] - s_start[b], first = whole ? 0 : s_start[b] * items + item * tiles;
     float *piece = block_pieces + (block0 >= first ? 0 : 1) * S::PART;
     const int c0 = whole ? 0 : stretch_of(first, total, grid), c1 = whole ? 0 : stretch_of(first + tiles - 1, total, grid);
 #pragma unroll 1
