@@ -12,9 +12,6 @@
 
 namespace stb {
 
-void linear(stb_session *s, uint64_t x, int ldx, uint64_t w, int w_dtype, uint64_t bias, uint64_t y, int ldy,
-            int M, int N, int K);
-
 namespace {
 
 __global__ void adapter_down_kernel(const float *x, const float *a, float *t, int M, int r, int K) {

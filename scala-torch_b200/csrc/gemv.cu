@@ -146,7 +146,7 @@ __global__ void fill_bias_kernel(float *y, int ldy, const float *bias, int M, in
 }
 
 void linear(stb_session *s, uint64_t x, int ldx, uint64_t w, int w_dtype, uint64_t bias, uint64_t y, int ldy,
-            int M, int N, int K) {
+            int M, int N, int K, bool pdl) {
   STB_REQUIRE(M >= 0 && N >= 0 && K >= 0, "Linear dimensions must be nonnegative");
   STB_REQUIRE(w_dtype == STB_F32 || w_dtype == STB_BF16 || w_dtype == STB_F16, "unsupported weight dtype");
   if (M == 0 || N == 0) return;
@@ -189,6 +189,7 @@ void linear(stb_session *s, uint64_t x, int ldx, uint64_t w, int w_dtype, uint64
   p.y = (float *)y;
   p.ldy = ldy;
   p.bias = (const float *)bias;
+  p.pdl = pdl;
   if (skinny_eligible(M, N, K, w_dtype, (const void *)w)) {
     // 2+ token rows: tensor cores with the activations split into three BF16 terms, 64-row blocks
     const uint64_t bytes = skinny_scratch_bytes(M, N, K, s->device);
@@ -210,7 +211,7 @@ int stb_linear_ld(stb_session *s, uint64_t x, int ldx, uint64_t w, int w_dtype, 
                   int ldy, int M, int N, int K) {
   return guarded([&] {
     enter(s);
-    linear(s, x, ldx, w, w_dtype, bias, y, ldy, M, N, K);
+    linear(s, x, ldx, w, w_dtype, bias, y, ldy, M, N, K, false);
   });
 }
 
@@ -218,7 +219,7 @@ int stb_linear(stb_session *s, uint64_t x, uint64_t w, int w_dtype, uint64_t bia
                int K) {
   return guarded([&] {
     enter(s);
-    linear(s, x, K, w, w_dtype, bias, y, N, M, N, K);
+    linear(s, x, K, w, w_dtype, bias, y, N, M, N, K, false);
   });
 }
 
@@ -240,7 +241,7 @@ int stb_linear_host(stb_session *s, const float *x_host, uint64_t w, int w_dtype
         s->io_bytes = xr + yb;
       }
       upload(s, x_host, xb, s->io_buf);
-      linear(s, s->io_buf, K, w, w_dtype, bias, s->io_buf + xr, N, M, N, K);
+      linear(s, s->io_buf, K, w, w_dtype, bias, s->io_buf + xr, N, M, N, K, false);
       download(s, s->io_buf + xr, y_host, yb);
       return;
     }
@@ -249,7 +250,7 @@ int stb_linear_host(stb_session *s, const float *x_host, uint64_t w, int w_dtype
       dx = session_alloc(s, xb);
       dy = session_alloc(s, yb);
       upload(s, x_host, xb, dx);
-      linear(s, dx, K, w, w_dtype, bias, dy, N, M, N, K);
+      linear(s, dx, K, w, w_dtype, bias, dy, N, M, N, K, false);
       download(s, dy, y_host, yb);
     } catch (...) {
       if (dy) session_free(s, dy);

@@ -487,4 +487,8 @@ int skinny_nt(int M);
 // Whether a residual projection of N outputs can do the next projection's RMSNorm prologue (SkinnyNext).
 bool skinny_norm_fusable(int N);
 
+// stb_linear (gemv.cu).  pdl: the first kernel is launched as a programmatic dependent of the one before it.
+void linear(stb_session *s, uint64_t x, int ldx, uint64_t w, int w_dtype, uint64_t bias, uint64_t y, int ldy,
+            int M, int N, int K, bool pdl = false);
+
 }  // namespace stb
