@@ -3,18 +3,22 @@
 // the shared product and bias as stb_linear does them, the thin products by two kernels around it.
 //
 // What bounds them: the factors of every slot in use, read once (the rows of a slot go through them 16 at a time), and the
-// launches.  One block serves one slot: the block of the slot's first row, which finds the others in `rows`; blocks of
-// other rows leave at once.  Both products run on the tensor cores in TF32 terms (the 16 rows are the product's rows):
-// BF16 and F16 factors are TF32 values already, Float32 factors and the activations are split into two terms, so the
-// result keeps 22 bits; sums of 32 products are joined in Float32.  A lane reads whole 16-byte pieces of a factor's row:
-// the order of the summed index within 32 is the lanes', the same in both operands.
-//   1. down: thin[s][m][j] = x[m] . A_t[j] over the s-th stretch of K (split so that the blocks cover the SMs even
-//      for a single row), by warps in turn, joined in shared memory;
+// launches.  Every block plans the rows by slot for itself and takes units of the plan in turn.  Both products run on the
+// tensor cores in TF32 terms (the rows of a slot are the product's 16 rows): BF16 and F16 factors are TF32 values
+// already, Float32 factors and the activations are split into two terms, so the result keeps 22 bits; sums of 32 products
+// are joined in Float32.  A lane reads whole 16-byte pieces of a factor's row: the order of the summed index within 32
+// is the lanes', the same in both operands.
+//   1. down: thin[s][m][j] = x[m] . A_t[j] over the s-th stretch of K; beside it the shared product's own prologue, the
+//      three BF16 terms of x, where the product takes the skinny tensor-core form;
 //   2. the shared product, launched as a dependent (its weights stream in while the first kernel drains);
-//   3. up: adds the stretches in order, multiplies by B_t, adds to y.  Its factors are read before it waits for y.
+//   3. up: adds the stretches in order, multiplies by B_t; it also adds up the skinny form's pieces of the shared
+//      product (or reads y), and the bias.  Its factors are read before it waits.
+// Rows go through in blocks of 64, the skinny form's.
 #include <algorithm>
+#include <mutex>
 
 #include "gemv.cuh"
+#include "tc_common.cuh"
 #include "tf32.cuh"
 
 namespace stb {
@@ -29,48 +33,60 @@ struct Pool {
   int *err;
 };
 
-constexpr int DOWN_RANKS = 32;   // ranks of a block of the first kernel
-constexpr int UP_COLUMNS = 256;  // outputs of a block of the second
+constexpr int DOWN_RANKS = 32;     // ranks of a unit of the first kernel
+constexpr int DOWN_COLUMNS = 512;  // columns of it: 32 for each of 16 warps
+constexpr int UP_COLUMNS = 256;    // outputs of a unit of the second
 constexpr int MAX_RANK = 256;
+constexpr int WINDOW = 64;         // rows of one launch
 
-__device__ __forceinline__ int rank_of(const Pool &p, int t) { return max(0, min(p.ranks[t], p.max_rank)); }
+// The launch's rows by slot: groups of up to 16 rows that name the same slot (or none).
+struct Plan {
+  int slots[WINDOW];   // per row: -1 without a slot, -2 behind the last row
+  uint32_t starts[2];  // rows that start a group
+  int groups;
+  int slot[WINDOW], rank[WINDOW], count[WINDOW];  // per group
+  signed char rows[WINDOW][16];
+};
 
-// The slot that this block serves (for rows m and later), or -1: a row without one, or not the slot's first row.
-__device__ __forceinline__ int slot_served(const Pool &p, int m) {
-  const int t = p.rows[m];
-  if (t < 0) return -1;
-  if (t >= p.slots) {
-    *p.err = DEV_BAD_INDEX + 2;
-    return -1;
-  }
-  bool before = false;
-  for (int i = threadIdx.x; i < m; i += blockDim.x) before |= p.rows[i] == t;
-  return __syncthreads_or(before) ? -1 : t;
-}
-
-// The next 16 rows of slot t from row `from` on, -1 behind the last; returns where to go on.  Ends with a barrier.
-__device__ __forceinline__ int gather_rows(const Pool &p, int t, int from, int M, int (&s_rows)[16], int &s_next) {
-  if (threadIdx.x < 32) {
-    const int lane = threadIdx.x;
-    if (lane < 16) s_rows[lane] = -1;
-    __syncwarp();
-    int count = 0, next = M;
-    for (int i = from; i < M; i += 32) {
-      const bool has = i + lane < M && p.rows[i + lane] == t;
-      const uint32_t which = __ballot_sync(0xffffffffu, has);
-      const int at = count + __popc(which & ((1u << lane) - 1));
-      if (has && at < 16) s_rows[at] = i + lane;
-      const uint32_t over = __ballot_sync(0xffffffffu, has && at >= 16);
-      count += __popc(which);
-      if (over) {
-        next = i + __ffs(over) - 1;
-        break;
-      }
+// A thread per row compares its slot with the others'.  Ends with a barrier.
+__device__ __forceinline__ void make_plan(const Pool &p, int M, Plan &s) {
+  const int i = threadIdx.x;
+  if (i < WINDOW) {
+    int t = -2;
+    if (i < M) {
+      t = p.rows[i];
+      if (t >= p.slots) *p.err = DEV_BAD_INDEX + 2;
+      if (t < 0 || t >= p.slots) t = -1;
     }
-    if (lane == 0) s_next = next;
+    s.slots[i] = t;
   }
   __syncthreads();
-  return s_next;
+  uint64_t same = 0;
+  int t = -2, at = 0, rank = 0;
+  if (i < WINDOW) {
+    t = s.slots[i];
+    if (t >= 0) rank = max(0, min(p.ranks[t], p.max_rank));
+#pragma unroll
+    for (int k = 0; k < WINDOW; k++) same |= (uint64_t)(s.slots[k] == t) << k;
+    at = __popcll(same & ((1ull << i) - 1));  // its place in the slot's rows
+    const uint32_t starts = __ballot_sync(0xffffffffu, t != -2 && at % 16 == 0);
+    if ((i & 31) == 0) s.starts[i >> 5] = starts;
+  }
+  __syncthreads();
+  if (i < WINDOW && t != -2) {
+    const uint64_t starts = (uint64_t)s.starts[1] << 32 | s.starts[0];
+    uint64_t mine = same & starts;  // its group starts at the (at / 16)-th of these
+    for (int k = 0; k < at / 16; k++) mine &= mine - 1;
+    const int group = __popcll(starts & ((1ull << (__ffsll((long long)mine) - 1)) - 1));
+    s.rows[group][at % 16] = (signed char)i;
+    if (at % 16 == 0) {
+      s.slot[group] = t;
+      s.rank[group] = rank;
+      s.count[group] = min(16, __popcll(same) - at);
+    }
+    if (i == 0) s.groups = __popcll(starts);
+  }
+  __syncthreads();
 }
 
 // Eight neighbouring factor elements from index `at`, the first `live` of them (the others are zero).  VEC: 16-byte loads.
@@ -131,111 +147,245 @@ __device__ __forceinline__ void eight_products(float (&c)[4], const uint32_t (&h
   }
 }
 
-// thin[blockIdx.y][m][j] for the rows of one slot, ranks 32 blockIdx.z .. + 31, columns blockIdx.y * stretch .. + stretch - 1
-// (a multiple of 256).  VEC: x and A have rows of whole 16-byte pieces.
-template <int DTYPE, bool VEC>
-__global__ void __launch_bounds__(256) pool_down_kernel(const Pool p, const float *x, float *thin, int M, int K, int stretch) {
-  constexpr int NT = DOWN_RANKS / 8;
-  __shared__ float s_sum[8][16][DOWN_RANKS + 1];
-  __shared__ int s_rows[16], s_next;
-  const int m = blockIdx.x, j0 = blockIdx.z * DOWN_RANKS;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  pdl_trigger();
-  const int t = slot_served(p, m);
-  if (t < 0) return;
-  const int rank = rank_of(p, t) - j0;
-  if (rank <= 0) return;
-  const int k0 = blockIdx.y * stretch + warp * 32 + t4 * 8, k1 = min(K, (int)(blockIdx.y + 1) * stretch);
-  for (int next = m; next < M;) {
-    next = gather_rows(p, t, next, M, s_rows, s_next);
-    const int m0 = s_rows[g], m1 = s_rows[g + 8];
-    Eight<DTYPE, VEC> f[NT];
-    Eight<STB_F32, VEC> x0, x1;
-    auto read = [&](int k) {
-      const int live = min(8, k1 - k);
+// The skinny form's terms x3 [3][NT][K] of four neighbouring values (zeros for rows M and behind).
+__device__ __forceinline__ void write_terms(float4 v, uint16_t *x3, int m, int NT, int K, int k) {
+  const float f[4] = {v.x, v.y, v.z, v.w};
+  uint16_t h[3][4];
 #pragma unroll
-      for (int n = 0; n < NT; n++)
-        f[n].load(p.a, ((size_t)t * p.max_rank + j0 + n * 8 + g) * K + k, n * 8 + g < rank ? live : 0);
-      x0.load(x, (size_t)max(m0, 0) * K + k, m0 >= 0 ? live : 0);
-      x1.load(x, (size_t)max(m1, 0) * K + k, m1 >= 0 ? live : 0);
-    };
-    float acc[NT][4] = {};
-    read(k0);
-#pragma unroll 1
-    for (int k = k0 - t4 * 8; k < k1; k += 256) {
-      uint32_t hi[4][4], lo[4][4];
+  for (int e = 0; e < 4; e++) split3_bf16(f[e], h[0][e], h[1][e], h[2][e]);
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          split_tf32(x0.get(2 * j + i), hi[j][2 * i], lo[j][2 * i]);
-          split_tf32(x1.get(2 * j + i), hi[j][2 * i + 1], lo[j][2 * i + 1]);
-        }
-      Eight<DTYPE, VEC> now[NT];
-#pragma unroll
-      for (int n = 0; n < NT; n++) now[n] = f[n];
-      read(k + 256 + t4 * 8);
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-        if (n * 8 >= rank) continue;
-        float c[4] = {};
-        eight_products<DTYPE>(c, hi, lo, now[n]);
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[n][i] += c[i];
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) s_sum[warp][g + 8 * (i >> 1)][n * 8 + 2 * t4 + (i & 1)] = acc[n][i];
-    __syncthreads();
-    for (int e = threadIdx.x; e < 16 * DOWN_RANKS; e += 256) {
-      const int i = e / DOWN_RANKS, j = e % DOWN_RANKS;
-      if (s_rows[i] < 0 || j >= rank) continue;
-      float v = 0.0f;
-#pragma unroll
-      for (int w = 0; w < 8; w++) v += s_sum[w][i][j];
-      thin[((size_t)blockIdx.y * M + s_rows[i]) * p.max_rank + j0 + j] = v;
-    }
-    __syncthreads();
+  for (int i = 0; i < 3; i++) {
+    uint2 u;
+    u.x = (uint32_t)h[i][0] | ((uint32_t)h[i][1] << 16);
+    u.y = (uint32_t)h[i][2] | ((uint32_t)h[i][3] << 16);
+    *(uint2 *)(x3 + ((size_t)i * NT + m) * K + k) = u;
   }
 }
 
-// y[m][n] += scale_t thin[m] . B_t[n] for the rows of one slot, columns 256 blockIdx.y .. + 255; `stretches` partial sums
-// of thin.  VEC: B has rows of whole 16-byte pieces.
+template <int DTYPE>
+struct Down {
+  static constexpr int ESZ = DTYPE == STB_F32 ? 4 : 2;
+  static constexpr int A_ROW = DOWN_COLUMNS * ESZ, X_ROW = DOWN_COLUMNS * 4;
+  static constexpr int SLOT = DOWN_RANKS * A_ROW + 16 * X_ROW;
+  static constexpr int SLOTS = 196608 / SLOT;
+  static_assert(SLOTS >= 2 && 16 * 16 * (DOWN_RANKS + 1) * 4 <= SLOT, "shared memory");
+};
+
+__device__ __forceinline__ void copy16_async(void *dst, const void *src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+               "r"(live ? 16 : 0)
+               : "memory");
+}
+
+// thin[s][m][j] for all rows: units (group of rows, s-th stretch of 512 columns, chunk of 32 ranks) in turn over the blocks,
+// one block per SM; with x3 the blocks also write the terms of x.  The factors come from memory that nothing has touched
+// lately (2 to 3 us away, behind the shared product's weights), so a block sends for all that its shared memory holds (three
+// units, 192 KB) before it waits for the first.  VEC: x and A have rows of whole 16-byte pieces (plain loads otherwise).
 template <int DTYPE, bool VEC>
-__global__ void __launch_bounds__(256) pool_up_kernel(const Pool p, const float *thin, float *y, int M, int N, int stretches) {
-  constexpr int NT = UP_COLUMNS / 64;  // 8-column results of a warp
-  __shared__ float s_thin[16][MAX_RANK + 4];
-  __shared__ int s_rows[16], s_next;
-  const int m = blockIdx.x;
+__global__ void __launch_bounds__(512, 1) pool_down_kernel(const Pool p, const float *x, float *thin, int M, int K, int stretches,
+                                                           int chunks, uint16_t *x3, int terms_rows) {
+  using D = Down<DTYPE>;
+  constexpr int NT = DOWN_RANKS / 8, ESZ = D::ESZ;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ Plan s_plan;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  const int n0 = blockIdx.y * UP_COLUMNS + warp * (UP_COLUMNS / 8);
-  const int t = slot_served(p, m);
-  const int rank = t >= 0 ? rank_of(p, t) : 0;
-  if (rank == 0) return;
-  const int blocks = (rank + 31) / 32;  // of 32 ranks
-  const float scale = p.scales[t];
-  Eight<DTYPE, VEC> f[NT];
-  auto read = [&](int kb) {
-    const int j = kb * 32 + t4 * 8;
+  pdl_trigger();
+  make_plan(p, M, s_plan);
+  const int groups = s_plan.groups, units = groups * stretches * chunks;
+
+  // The next unit of this block from u on that has work (ranks left in its chunk).
+  auto find = [&](int u) {
+    for (; u < units; u += gridDim.x)
+      if (s_plan.slot[u % groups] >= 0 && s_plan.rank[u % groups] > u / groups / stretches * DOWN_RANKS) break;
+    return u;
+  };
+  // 16-byte chunk c of row r: XORed so that the chunks that eight rows read at once lie in different banks.
+  auto a_at = [&](uint8_t *slot, int r, int c) {
+    return slot + r * D::A_ROW + ((c ^ (ESZ == 4 ? r & 7 : (r & 1) << 2 | (r >> 1 & 3))) << 4);
+  };
+  auto x_at = [&](uint8_t *slot, int r, int c) { return slot + DOWN_RANKS * D::A_ROW + r * D::X_ROW + ((c ^ (r & 7)) << 4); };
+  auto send = [&](int u, uint8_t *slot) {
+    if (u < units) {
+      const int e = u % groups, s = u / groups % stretches, j0 = u / groups / stretches * DOWN_RANKS;
+      const int live = min(DOWN_RANKS, s_plan.rank[e] - j0), rows = (live + 7) / 8 * 8, k0 = s * DOWN_COLUMNS;
+      const size_t base = ((size_t)s_plan.slot[e] * p.max_rank + j0) * K + k0;
+      constexpr int AC = D::A_ROW / 16, XC = D::X_ROW / 16, PER = 16 / ESZ;
+      for (int i = threadIdx.x; i < rows * AC; i += 512) {
+        const int r = i / AC, c = i % AC, k = c * PER;
+        if (VEC) {
+          const bool in = r < live && k0 + k < K;
+          copy16_async(a_at(slot, r, c), (const uint8_t *)p.a + (base + (in ? (size_t)r * K + k : 0)) * ESZ, in);
+        } else {
+          uint8_t *to = a_at(slot, r, c);
+          for (int h = 0; h < PER; h++) {
+            const bool in = r < live && k0 + k + h < K;
+            if (ESZ == 4) ((uint32_t *)to)[h] = in ? ((const uint32_t *)p.a)[base + (size_t)r * K + k + h] : 0u;
+            else ((uint16_t *)to)[h] = in ? ((const uint16_t *)p.a)[base + (size_t)r * K + k + h] : (uint16_t)0;
+          }
+        }
+      }
+      for (int i = threadIdx.x; i < s_plan.count[e] * XC; i += 512) {
+        const int r = i / XC, c = i % XC, k = c * 4;
+        const float *from = x + (size_t)s_plan.rows[e][r] * K + k0;
+        if (VEC) {
+          copy16_async(x_at(slot, r, c), from + (k0 + k < K ? k : 0), k0 + k < K);
+        } else {
+          for (int h = 0; h < 4; h++) ((float *)x_at(slot, r, c))[h] = k0 + k + h < K ? from[k + h] : 0.0f;
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+
+  int ahead = find(blockIdx.x), unit = ahead;
+#pragma unroll 1
+  for (int i = 0; i < D::SLOTS; i++) {
+    send(ahead, smem + i * D::SLOT);
+    if (ahead < units) ahead = find(ahead + gridDim.x);
+  }
+  if (x3) {
+    const int quads = K / 4, all = terms_rows * quads, step = gridDim.x * 512;
+    for (int i = blockIdx.x * 512 + threadIdx.x; i < all; i += 2 * step) {  // two in flight
+      float4 v[2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int e = i + h * step;
+        v[h] = e < M * quads ? *(const float4 *)(x + (size_t)e * 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int e = i + h * step;
+        if (e < all) write_terms(v[h], x3, e / quads, terms_rows, K, e % quads * 4);
+      }
+    }
+  }
+  int in = 0;
+  for (; unit < units; unit = find(unit + gridDim.x)) {
+    const int e = unit % groups, s = unit / groups % stretches, j0 = unit / groups / stretches * DOWN_RANKS;
+    const int rank = s_plan.rank[e] - j0, count = s_plan.count[e];
+    uint8_t *slot = smem + in * D::SLOT;
+    asm volatile("cp.async.wait_group %0;" ::"n"(D::SLOTS - 1) : "memory");
+    __syncthreads();
+    uint32_t hi[4][4], lo[4][4];  // the rows' eight values of this lane, in both terms
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int r = g + 8 * h;
+      const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const float4 u = r < count ? *(const float4 *)x_at(slot, r, warp * 8 + t4 * 2) : zero;
+      const float4 v = r < count ? *(const float4 *)x_at(slot, r, warp * 8 + t4 * 2 + 1) : zero;
+      const float f[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) split_tf32(f[2 * j + i], hi[j][2 * i + h], lo[j][2 * i + h]);
+    }
+    float acc[NT][4] = {};
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      if (n * 8 >= rank) continue;
+      Eight<DTYPE, true> f;
+#pragma unroll
+      for (int i = 0; i < ESZ / 2; i++) f.raw[i] = *(const uint4 *)a_at(slot, n * 8 + g, (warp * 4 + t4) * (ESZ / 2) + i);
+      eight_products<DTYPE>(acc[n], hi, lo, f);
+    }
+    __syncthreads();  // the unit has been read: the warps' sums go over it
+    float(*sums)[16][DOWN_RANKS + 1] = (float(*)[16][DOWN_RANKS + 1]) slot;
 #pragma unroll
     for (int n = 0; n < NT; n++)
-      f[n].load(p.b, ((size_t)t * N + n0 + n * 8 + g) * p.max_rank + j, n0 + n * 8 + g < N ? min(8, rank - j) : 0);
-  };
-  read(0);
-  int next = gather_rows(p, t, m, M, s_rows, s_next);
-  pdl_wait();  // thin, and the shared product in y
-  while (true) {
-    for (int e = threadIdx.x; e < 16 * blocks * 32; e += 256) {
-      const int i = e / (blocks * 32), j = e % (blocks * 32), row = s_rows[i];
-      float v = 0.0f;
-      if (row >= 0 && j < rank) {
-        const float *at = thin + (size_t)row * p.max_rank + j;
-#pragma unroll 8
-        for (int s = 0; s < stretches; s++) v += __ldcg(at + (size_t)s * M * p.max_rank);
+#pragma unroll
+      for (int i = 0; i < 4; i++) sums[warp][g + 8 * (i >> 1)][n * 8 + 2 * t4 + (i & 1)] = acc[n][i];
+    __syncthreads();
+    float v = 0.0f;  // a warp per row, a lane per rank
+#pragma unroll
+    for (int w = 0; w < 16; w++) v += sums[w][warp][lane];
+    if (warp < count && lane < rank) thin[((size_t)s * M + s_plan.rows[e][warp]) * p.max_rank + j0 + lane] = v;
+    __syncthreads();
+    send(ahead, slot);
+    if (ahead < units) ahead = find(ahead + gridDim.x);
+    in = in + 1 == D::SLOTS ? 0 : in + 1;
+  }
+}
+
+// y[m][n] = base + scale_t thin[m] . B_t[n] + bias[n]: units (group of rows, 256 columns) in turn over the blocks;
+// `stretches` partial sums of thin.  base: the skinny form's pieces (PIECES), or y itself, its bias already in.  VEC: B has
+// rows of whole 16-byte pieces.
+template <int DTYPE, bool VEC, bool PIECES>
+__global__ void __launch_bounds__(256, DTYPE == STB_F32 ? 1 : 2) pool_up_kernel(const Pool p, const float *thin, float *y, int M,
+                                                                               int N, int stretches, const SkinnyParts parts,
+                                                                               const float *bias) {
+  constexpr int NT = UP_COLUMNS / 64;  // 8-column results of a warp
+  __shared__ float s_thin[16][MAX_RANK + 4];
+  __shared__ Plan s_plan;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  pdl_trigger();
+  make_plan(p, M, s_plan);
+  const int groups = s_plan.groups, columns = (N + UP_COLUMNS - 1) / UP_COLUMNS;
+  bool waited = false;
+  for (int u = blockIdx.x; u < groups * columns; u += gridDim.x) {
+    const int e = u % groups, t = s_plan.slot[e], rank = s_plan.rank[e], count = s_plan.count[e];
+    const int n0 = u / groups * UP_COLUMNS + warp * (UP_COLUMNS / 8);
+    if (!PIECES && rank == 0) continue;
+    const int blocks = (rank + 31) / 32;  // of 32 ranks
+    const float scale = t >= 0 ? p.scales[t] : 0.0f;
+    Eight<DTYPE, VEC> f[NT];
+    auto read = [&](int kb) {
+      const int j = kb * 32 + t4 * 8;
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+        f[n].load(p.b, ((size_t)t * N + n0 + n * 8 + g) * p.max_rank + j, n0 + n * 8 + g < N ? min(8, rank - j) : 0);
+    };
+    if (rank) read(0);
+    // pieces of the tile of 128 columns that this warp's 32 lie in
+    int pieces = 0;
+    const float *at_piece = nullptr;
+    if (PIECES && n0 < N) {
+      const int tile = n0 / 128;
+      pieces = skinny_cta_of((long long)(tile + 1) * parts.kbs - 1, parts.T, parts.G) -
+               skinny_cta_of((long long)tile * parts.kbs, parts.T, parts.G) + 1;
+      at_piece = parts.part + (size_t)tile * parts.pmax * parts.M * 128 + n0 % 128 + 2 * t4;
+    }
+    if (!waited) pdl_wait();  // thin, and the shared product
+    waited = true;
+    float2 base[2][NT];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+#pragma unroll
+      for (int n = 0; n < NT; n++) base[h][n] = make_float2(0.0f, 0.0f);
+      if (g + 8 * h >= count) continue;
+      const int r = s_plan.rows[e][g + 8 * h];
+      if (PIECES) {
+#pragma unroll 4
+        for (int i = 0; i < pieces; i++)
+#pragma unroll
+          for (int n = 0; n < NT; n++) {
+            const float2 v = __ldcg((const float2 *)(at_piece + ((size_t)i * parts.M + r) * 128 + n * 8));
+            base[h][n].x += v.x;
+            base[h][n].y += v.y;
+          }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          const int col = n0 + n * 8 + 2 * t4;
+          if (col < N) base[h][n].x = y[(size_t)r * N + col];
+          if (col + 1 < N) base[h][n].y = y[(size_t)r * N + col + 1];
+        }
       }
-      s_thin[i][j] = v;
+    }
+    const int wide = blocks * 32;
+    for (int i = warp * 32; i < count * wide; i += 256) {  // 32 ranks of one row
+      const int j = i % wide + lane;
+      float v = 0.0f;
+      if (j < rank) {
+        const float *at = thin + (size_t)s_plan.rows[e][i / wide] * p.max_rank + j;
+        for (int s = 0; s < stretches; s += 16) {
+          float w[16];
+#pragma unroll
+          for (int k = 0; k < 16; k++) w[k] = s + k < stretches ? __ldcg(at + (size_t)(s + k) * M * p.max_rank) : 0.0f;
+#pragma unroll
+          for (int k = 0; k < 16; k++) v += w[k];
+        }
+      }
+      s_thin[i / wide][j] = v;
     }
     __syncthreads();
     float acc[NT][4] = {};
@@ -247,13 +397,13 @@ __global__ void __launch_bounds__(256) pool_up_kernel(const Pool p, const float 
 #pragma unroll
         for (int i = 0; i < 2; i++) {
           const int at = kb * 32 + t4 * 8 + 2 * j + i;
-          split_tf32(s_thin[g][at], hi[j][2 * i], lo[j][2 * i]);
-          split_tf32(s_thin[g + 8][at], hi[j][2 * i + 1], lo[j][2 * i + 1]);
+          split_tf32(g < count ? s_thin[g][at] : 0.0f, hi[j][2 * i], lo[j][2 * i]);
+          split_tf32(g + 8 < count ? s_thin[g + 8][at] : 0.0f, hi[j][2 * i + 1], lo[j][2 * i + 1]);
         }
       Eight<DTYPE, VEC> now[NT];
 #pragma unroll
       for (int n = 0; n < NT; n++) now[n] = f[n];
-      if (kb + 1 < blocks || next < M) read(kb + 1 < blocks ? kb + 1 : 0);
+      if (kb + 1 < blocks) read(kb + 1);
 #pragma unroll
       for (int n = 0; n < NT; n++) {
         float c[4] = {};
@@ -263,22 +413,40 @@ __global__ void __launch_bounds__(256) pool_up_kernel(const Pool p, const float 
       }
     }
 #pragma unroll
-    for (int half = 0; half < 2; half++) {
-      const int row = s_rows[g + 8 * half];
-      if (row < 0) continue;
-      float *to = y + (size_t)row * N;
+    for (int h = 0; h < 2; h++) {
+      if (g + 8 * h >= count) continue;
+      float *to = y + (size_t)s_plan.rows[e][g + 8 * h] * N;
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int i = 0; i < 2; i++) {
           const int col = n0 + n * 8 + 2 * t4 + i;
-          if (col < N) to[col] += scale * acc[n][2 * half + i];
+          if (col >= N) continue;
+          float v = i ? base[h][n].y : base[h][n].x;
+          if (rank) v += scale * acc[n][2 * h + i];
+          if (PIECES && bias) v += bias[col];
+          to[col] = v;
         }
     }
-    if (next >= M) return;
-    __syncthreads();
-    next = gather_rows(p, t, next, M, s_rows, s_next);
+    __syncthreads();  // before thin's sums are replaced
   }
+}
+
+template <int DTYPE, bool VEC>
+void launch_down(stb_session *s, int grid, const Pool &p, const float *x, float *thin, int M, int K, int stretches, int chunks,
+                 uint16_t *x3, int terms_rows) {
+  constexpr int SMEM = Down<DTYPE>::SLOTS * Down<DTYPE>::SLOT;
+  {
+    static std::mutex mu;
+    static bool configured[64] = {};
+    std::lock_guard<std::mutex> lock(mu);
+    if (s->device < 0 || s->device >= 64 || !configured[s->device]) {
+      STB_CUDA(cudaFuncSetAttribute(pool_down_kernel<DTYPE, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+      if (s->device >= 0 && s->device < 64) configured[s->device] = true;
+    }
+  }
+  launch_kernel(pool_down_kernel<DTYPE, VEC>, dim3(grid), dim3(512), (size_t)SMEM, s->stream, false, p, x, thin, M, K, stretches,
+                chunks, x3, terms_rows);
 }
 
 }  // namespace
@@ -313,32 +481,55 @@ extern "C" int stb_linear_pool(stb_session *s, uint64_t x, uint64_t w, int w_dty
     p.scales = (const float *)pool->scales;
     p.slots = pool->slots;
     p.max_rank = pool->max_rank;
-    p.rows = (const int *)rows;
     p.err = session_error_word(s);
-    // About 1200 blocks of the first kernel were every row of a slot of its own, at least 256 columns each (measured at
-    // 32 rows of 12 slots, K = 14336, rank 64: 1024 columns).
-    const int chunks = (p.max_rank + DOWN_RANKS - 1) / DOWN_RANKS;
-    const int64_t want = std::max<int64_t>(1, 1184 / ((int64_t)M * chunks));
-    const int stretch = (int)(((K + want - 1) / want + 255) / 256 * 256);
-    const int stretches = (K + stretch - 1) / stretch;
-    const int columns = (N + UP_COLUMNS - 1) / UP_COLUMNS;
-    STB_REQUIRE(columns <= 65535, "adapted Linear too wide");
+    const int chunks = (p.max_rank + DOWN_RANKS - 1) / DOWN_RANKS, most = std::min(M, WINDOW);
+    const int stretches = (K + DOWN_COLUMNS - 1) / DOWN_COLUMNS, columns = (N + UP_COLUMNS - 1) / UP_COLUMNS;
+    STB_REQUIRE((int64_t)WINDOW * stretches * chunks <= 0x7fffffff && (int64_t)WINDOW * columns <= 0x7fffffff, "adapted Linear too large");
+    const int sms = tc::sm_count(s->device), resident = (pool->dtype == STB_F32 ? 1 : 2) * sms;  // blocks of `up` at once
+    const bool skinny = K % 8 == 0 && x % 16 == 0 && skinny_eligible(M, N, K, w_dtype, (const void *)w);
     // The partial sums lie behind the shared product's own scratch.
-    const uint64_t base = (skinny_eligible(M, N, K, w_dtype, (const void *)w) ? skinny_scratch_bytes(M, N, K, s->device) : 0) + 255 & ~255ull;
-    float *thin = (float *)(session_scratch(s, base + (uint64_t)stretches * M * p.max_rank * sizeof(float)) + base);
+    const uint64_t base = ((skinny ? skinny_scratch_bytes(M, N, K, s->device) : 0) + 255) & ~255ull;
+    const uint64_t scratch = session_scratch(s, base + (uint64_t)stretches * most * p.max_rank * sizeof(float));
+    float *thin = (float *)(scratch + base);
     const bool vec_down = K % 8 == 0 && x % 16 == 0 && pool->a % 16 == 0;
     const bool vec_up = p.max_rank % 8 == 0 && pool->b % 16 == 0;
     auto go = [&](auto type) {
       constexpr int DT = decltype(type)::value;
-      launch_kernel(vec_down ? pool_down_kernel<DT, true> : pool_down_kernel<DT, false>, dim3(M, stretches, chunks), dim3(256), 0,
-                    s->stream, false, p, (const float *)x, thin, M, K, stretch);
-      linear(s, x, K, w, w_dtype, bias, y, N, M, N, K, true);
-      launch_kernel(vec_up ? pool_up_kernel<DT, true> : pool_up_kernel<DT, false>, dim3(M, columns), dim3(256), 0, s->stream, true, p,
-                    (const float *)thin, (float *)y, M, N, stretches);
+      for (int m0 = 0; m0 < M; m0 += WINDOW) {
+        const int mb = std::min(WINDOW, M - m0), terms_rows = skinny ? skinny_nt(mb) : 0;
+        const float *xb = (const float *)x + (size_t)m0 * K;
+        float *yb = (float *)y + (size_t)m0 * N;
+        uint16_t *terms = skinny ? (uint16_t *)scratch : nullptr;
+        p.rows = (const int *)rows + m0;
+        const int down_grid = skinny ? sms : (int)std::min<int64_t>(sms, (int64_t)mb * stretches * chunks);
+        const int up_grid = (int)std::min<int64_t>(resident, (int64_t)mb * columns);
+        if (vec_down) launch_down<DT, true>(s, down_grid, p, xb, thin, mb, K, stretches, chunks, terms, terms_rows);
+        else launch_down<DT, false>(s, down_grid, p, xb, thin, mb, K, stretches, chunks, terms, terms_rows);
+        SkinnyParts parts;
+        if (skinny) {
+          GemvParams g;
+          g.x = xb;
+          g.ldx = K;
+          g.w = (const void *)w;
+          g.M = mb;
+          g.N = N;
+          g.K = K;
+          g.y = yb;
+          g.ldy = N;
+          g.pdl = true;
+          count_launch(s, skinny_launch<EPI_PLAIN>(g, (void *)scratch, base, p.err, s->device, s->stream, terms, nullptr, &parts));
+          launch_kernel(vec_up ? pool_up_kernel<DT, true, true> : pool_up_kernel<DT, false, true>, dim3(up_grid), dim3(256), 0,
+                        s->stream, true, p, (const float *)thin, yb, mb, N, stretches, parts, (const float *)bias);
+        } else {
+          linear(s, (uint64_t)xb, K, w, w_dtype, bias, (uint64_t)yb, N, mb, N, K, true);
+          launch_kernel(vec_up ? pool_up_kernel<DT, true, false> : pool_up_kernel<DT, false, false>, dim3(up_grid), dim3(256), 0,
+                        s->stream, true, p, (const float *)thin, yb, mb, N, stretches, parts, (const float *)bias);
+        }
+        count_launch(s, 2);
+      }
     };
     if (pool->dtype == STB_F32) go(std::integral_constant<int, STB_F32>());
     else if (pool->dtype == STB_BF16) go(std::integral_constant<int, STB_BF16>());
     else go(std::integral_constant<int, STB_F16>());
-    count_launch(s, 2);
   });
 }
