@@ -42,15 +42,23 @@ constexpr int WINDOW = 64;         // rows of one launch
 // The launch's rows by slot: groups of up to 16 rows that name the same slot (or none).
 struct Plan {
   int slots[WINDOW];   // per row: -1 without a slot, -2 behind the last row
+  short ranks[WINDOW * 2];  // of a small pool's slots, clamped
   uint32_t starts[2];  // rows that start a group
   int groups;
-  int slot[WINDOW], rank[WINDOW], count[WINDOW];  // per group
+  int slot[WINDOW];                     // per group
+  short rank[WINDOW], count[WINDOW], first[WINDOW];
   signed char rows[WINDOW][16];
+  // (group, chunk of 32 ranks) pairs, and into how many parts each one's columns are split: as many as give every block
+  // of the first kernel one (both kernels plan alike).
+  int chunks[2], pairs, parts, per;  // per: stretches of 512 columns in a part
+  signed char group_of[WINDOW * (MAX_RANK / DOWN_RANKS)];
 };
 
 // A thread per row compares its slot with the others'.  Ends with a barrier.
-__device__ __forceinline__ void make_plan(const Pool &p, int M, Plan &s) {
+__device__ __forceinline__ void make_plan(const Pool &p, int M, int stretches, int blocks, Plan &s) {
   const int i = threadIdx.x;
+  const bool small = p.slots <= WINDOW * 2;  // all ranks at once, beside the rows rather than behind them
+  if (small && i < p.slots) s.ranks[i] = (short)max(0, min(p.ranks[i], p.max_rank));
   if (i < WINDOW) {
     int t = -2;
     if (i < M) {
@@ -65,7 +73,7 @@ __device__ __forceinline__ void make_plan(const Pool &p, int M, Plan &s) {
   int t = -2, at = 0, rank = 0;
   if (i < WINDOW) {
     t = s.slots[i];
-    if (t >= 0) rank = max(0, min(p.ranks[t], p.max_rank));
+    if (t >= 0) rank = small ? s.ranks[t] : max(0, min(p.ranks[t], p.max_rank));
 #pragma unroll
     for (int k = 0; k < WINDOW; k++) same |= (uint64_t)(s.slots[k] == t) << k;
     at = __popcll(same & ((1ull << i) - 1));  // its place in the slot's rows
@@ -81,15 +89,40 @@ __device__ __forceinline__ void make_plan(const Pool &p, int M, Plan &s) {
     s.rows[group][at % 16] = (signed char)i;
     if (at % 16 == 0) {
       s.slot[group] = t;
-      s.rank[group] = rank;
-      s.count[group] = min(16, __popcll(same) - at);
+      s.rank[group] = (short)rank;
+      s.count[group] = (short)min(16, __popcll(same) - at);
     }
     if (i == 0) s.groups = __popcll(starts);
   }
   __syncthreads();
+  int chunks = 0, before = 0;
+  if (i < WINDOW) {
+    if (i < s.groups && s.slot[i] >= 0) chunks = (s.rank[i] + DOWN_RANKS - 1) / DOWN_RANKS;
+    before = chunks;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, before, off);
+      if ((i & 31) >= off) before += v;
+    }
+    if ((i & 31) == 31) s.chunks[i >> 5] = before;
+  }
+  __syncthreads();
+  if (i < WINDOW) {
+    before += (i >= 32 ? s.chunks[0] : 0) - chunks;
+    s.first[i] = (short)before;
+    for (int k = 0; k < chunks; k++) s.group_of[before + k] = (signed char)i;
+    if (i == 0) {
+      s.pairs = s.chunks[0] + s.chunks[1];
+      const int parts = max(1, min(stretches, blocks / max(1, s.pairs)));
+      s.per = (stretches + parts - 1) / parts;
+      s.parts = (stretches + s.per - 1) / s.per;
+    }
+  }
+  __syncthreads();
 }
 
-// Eight neighbouring factor elements from index `at`, the first `live` of them (the others are zero).  VEC: 16-byte loads.
+// Eight neighbouring factor elements from index `at`, the first `live` of them at least (all of a piece that has one, with
+// VEC: 16-byte loads).
 template <int DTYPE, bool VEC>
 struct Eight {
   uint4 raw[DTYPE == STB_F32 ? 2 : 1];
@@ -97,17 +130,11 @@ struct Eight {
   __device__ __forceinline__ void load(const void *base, size_t at, int live) {
 #pragma unroll
     for (int i = 0; i < (DTYPE == STB_F32 ? 2 : 1); i++) raw[i] = make_uint4(0, 0, 0, 0);
-    if (live <= 0) return;
     if (VEC) {
       const uint4 *p = (const uint4 *)((const char *)base + at * (DTYPE == STB_F32 ? 4 : 2));
+      if (live > 0) {
 #pragma unroll
-      for (int i = 0; i < (DTYPE == STB_F32 ? 2 : 1); i++) raw[i] = __ldg(p + i);
-      if (live >= 8) return;
-      uint32_t *w = (uint32_t *)raw;
-#pragma unroll
-      for (int i = 0; i < (DTYPE == STB_F32 ? 8 : 4); i++) {
-        if (DTYPE == STB_F32) w[i] = i < live ? w[i] : 0u;
-        else w[i] = 2 * i + 1 < live ? w[i] : (2 * i < live ? w[i] & 0xffffu : 0u);
+        for (int i = 0; i < (DTYPE == STB_F32 ? 2 : 1); i++) raw[i] = __ldg(p + i);
       }
     } else {
       uint32_t *w = (uint32_t *)raw;
@@ -117,6 +144,15 @@ struct Eight {
           if (DTYPE == STB_F32) w[i] = ((const uint32_t *)base)[at + i];
           else w[i / 2] |= (uint32_t)((const uint16_t *)base)[at + i] << (16 * (i & 1));
         }
+    }
+  }
+  // Zeros behind the first `live` elements, which may hold anything: at the use, a load would have to be waited for.
+  __device__ __forceinline__ void trim(int live) {
+    uint32_t *w = (uint32_t *)raw;
+#pragma unroll
+    for (int i = 0; i < (DTYPE == STB_F32 ? 8 : 4); i++) {
+      if (DTYPE == STB_F32) w[i] = i < live ? w[i] : 0u;
+      else w[i] = 2 * i + 1 < live ? w[i] : (2 * i < live ? w[i] & 0xffffu : 0u);
     }
   }
   __device__ __forceinline__ float get(int i) const {
@@ -168,7 +204,8 @@ struct Down {
   static constexpr int A_ROW = DOWN_COLUMNS * ESZ, X_ROW = DOWN_COLUMNS * 4;
   static constexpr int SLOT = DOWN_RANKS * A_ROW + 16 * X_ROW;
   static constexpr int SLOTS = 196608 / SLOT;
-  static_assert(SLOTS >= 2 && 16 * 16 * (DOWN_RANKS + 1) * 4 <= SLOT, "shared memory");
+  static constexpr int SMEM = SLOTS * SLOT + 16 * 16 * DOWN_RANKS * 4;  // the ring, then the warps' sums
+  static_assert(SLOTS >= 2 && SMEM + sizeof(Plan) <= 232448, "shared memory");
 };
 
 __device__ __forceinline__ void copy16_async(void *dst, const void *src, bool live) {
@@ -177,38 +214,41 @@ __device__ __forceinline__ void copy16_async(void *dst, const void *src, bool li
                : "memory");
 }
 
-// thin[s][m][j] for all rows: units (group of rows, s-th stretch of 512 columns, chunk of 32 ranks) in turn over the blocks,
-// one block per SM; with x3 the blocks also write the terms of x.  The factors come from memory that nothing has touched
-// lately (2 to 3 us away, behind the shared product's weights), so a block sends for all that its shared memory holds (three
-// units, 192 KB) before it waits for the first.  VEC: x and A have rows of whole 16-byte pieces (plain loads otherwise).
+// thin[part][m][j] for all rows: units (pair of a group of rows and a chunk of 32 ranks, part of the columns), one block per
+// SM and, where the plan can, one unit per block; with x3 the blocks also write the terms of x.  The factors come from
+// memory that nothing has touched lately (2 to 3 us away, behind the shared product's weights), so a block sends for all
+// that its shared memory holds (three stretches of 512 columns, 192 KB) before it waits for the first.  VEC: x and A have
+// rows of whole 16-byte pieces (plain loads otherwise).
 template <int DTYPE, bool VEC>
 __global__ void __launch_bounds__(512, 1) pool_down_kernel(const Pool p, const float *x, float *thin, int M, int K, int stretches,
-                                                           int chunks, uint16_t *x3, int terms_rows) {
+                                                           uint16_t *x3, int terms_rows) {
   using D = Down<DTYPE>;
   constexpr int NT = DOWN_RANKS / 8, ESZ = D::ESZ;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Plan s_plan;
+  float(*s_sum)[16][DOWN_RANKS] = (float(*)[16][DOWN_RANKS])(smem + D::SLOTS * D::SLOT);  // row r turned by 8 (r & 3)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   pdl_trigger();
-  make_plan(p, M, s_plan);
-  const int groups = s_plan.groups, units = groups * stretches * chunks;
+  make_plan(p, M, stretches, gridDim.x, s_plan);
+  const int units = s_plan.pairs * s_plan.parts, per = s_plan.per;
 
-  // The next unit of this block from u on that has work (ranks left in its chunk).
-  auto find = [&](int u) {
-    for (; u < units; u += gridDim.x)
-      if (s_plan.slot[u % groups] >= 0 && s_plan.rank[u % groups] > u / groups / stretches * DOWN_RANKS) break;
-    return u;
-  };
   // 16-byte chunk c of row r: XORed so that the chunks that eight rows read at once lie in different banks.
   auto a_at = [&](uint8_t *slot, int r, int c) {
     return slot + r * D::A_ROW + ((c ^ (ESZ == 4 ? r & 7 : (r & 1) << 2 | (r >> 1 & 3))) << 4);
   };
   auto x_at = [&](uint8_t *slot, int r, int c) { return slot + DOWN_RANKS * D::A_ROW + r * D::X_ROW + ((c ^ (r & 7)) << 4); };
-  auto send = [&](int u, uint8_t *slot) {
-    if (u < units) {
-      const int e = u % groups, s = u / groups % stretches, j0 = u / groups / stretches * DOWN_RANKS;
-      const int live = min(DOWN_RANKS, s_plan.rank[e] - j0), rows = (live + 7) / 8 * 8, k0 = s * DOWN_COLUMNS;
+  // One stretch s of unit u, and the next one to send for.
+  int ahead = blockIdx.x, ahead_s = 0;
+  auto send = [&](uint8_t *slot) {
+    if (ahead < units) {
+      const int pair = ahead / s_plan.parts, e = s_plan.group_of[pair], j0 = (pair - s_plan.first[e]) * DOWN_RANKS;
+      const int s0 = ahead % s_plan.parts * per, s = s0 + ahead_s;
+      const int live = min(DOWN_RANKS, (int)s_plan.rank[e] - j0), rows = (live + 7) / 8 * 8, k0 = s * DOWN_COLUMNS;
       const size_t base = ((size_t)s_plan.slot[e] * p.max_rank + j0) * K + k0;
+      if (++ahead_s == per || s + 1 == stretches) {
+        ahead_s = 0;
+        ahead += gridDim.x;
+      }
       constexpr int AC = D::A_ROW / 16, XC = D::X_ROW / 16, PER = 16 / ESZ;
       for (int i = threadIdx.x; i < rows * AC; i += 512) {
         const int r = i / AC, c = i % AC, k = c * PER;
@@ -237,12 +277,8 @@ __global__ void __launch_bounds__(512, 1) pool_down_kernel(const Pool p, const f
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
-  int ahead = find(blockIdx.x), unit = ahead;
 #pragma unroll 1
-  for (int i = 0; i < D::SLOTS; i++) {
-    send(ahead, smem + i * D::SLOT);
-    if (ahead < units) ahead = find(ahead + gridDim.x);
-  }
+  for (int i = 0; i < D::SLOTS; i++) send(smem + i * D::SLOT);
   if (x3) {
     const int quads = K / 4, all = terms_rows * quads, step = gridDim.x * 512;
     for (int i = blockIdx.x * 512 + threadIdx.x; i < all; i += 2 * step) {  // two in flight
@@ -260,49 +296,53 @@ __global__ void __launch_bounds__(512, 1) pool_down_kernel(const Pool p, const f
     }
   }
   int in = 0;
-  for (; unit < units; unit = find(unit + gridDim.x)) {
-    const int e = unit % groups, s = unit / groups % stretches, j0 = unit / groups / stretches * DOWN_RANKS;
-    const int rank = s_plan.rank[e] - j0, count = s_plan.count[e];
-    uint8_t *slot = smem + in * D::SLOT;
-    asm volatile("cp.async.wait_group %0;" ::"n"(D::SLOTS - 1) : "memory");
-    __syncthreads();
-    uint32_t hi[4][4], lo[4][4];  // the rows' eight values of this lane, in both terms
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int r = g + 8 * h;
-      const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      const float4 u = r < count ? *(const float4 *)x_at(slot, r, warp * 8 + t4 * 2) : zero;
-      const float4 v = r < count ? *(const float4 *)x_at(slot, r, warp * 8 + t4 * 2 + 1) : zero;
-      const float f[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-#pragma unroll
-        for (int i = 0; i < 2; i++) split_tf32(f[2 * j + i], hi[j][2 * i + h], lo[j][2 * i + h]);
-    }
+  for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int pair = unit / s_plan.parts, part = unit % s_plan.parts, e = s_plan.group_of[pair];
+    const int j0 = (pair - s_plan.first[e]) * DOWN_RANKS, rank = s_plan.rank[e] - j0, count = s_plan.count[e];
     float acc[NT][4] = {};
+    const int end = min(per, stretches - part * per);
+#pragma unroll 1
+    for (int s = 0; s < end; s++) {
+      uint8_t *slot = smem + in * D::SLOT;
+      asm volatile("cp.async.wait_group %0;" ::"n"(D::SLOTS - 1) : "memory");
+      __syncthreads();
+      uint32_t hi[4][4], lo[4][4];  // the rows' eight values of this lane, in both terms
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-      if (n * 8 >= rank) continue;
-      Eight<DTYPE, true> f;
+      for (int h = 0; h < 2; h++) {
+        const int r = g + 8 * h;
+        const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const float4 u = r < count ? *(const float4 *)x_at(slot, r, warp * 8 + t4 * 2) : zero;
+        const float4 v = r < count ? *(const float4 *)x_at(slot, r, warp * 8 + t4 * 2 + 1) : zero;
+        const float f[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < ESZ / 2; i++) f.raw[i] = *(const uint4 *)a_at(slot, n * 8 + g, (warp * 4 + t4) * (ESZ / 2) + i);
-      eight_products<DTYPE>(acc[n], hi, lo, f);
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int i = 0; i < 2; i++) split_tf32(f[2 * j + i], hi[j][2 * i + h], lo[j][2 * i + h]);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        Eight<DTYPE, true> f;  // ranks behind the last hold anything, and go nowhere
+#pragma unroll
+        for (int i = 0; i < ESZ / 2; i++) f.raw[i] = *(const uint4 *)a_at(slot, n * 8 + g, (warp * 4 + t4) * (ESZ / 2) + i);
+        float c[4] = {};
+        eight_products<DTYPE>(c, hi, lo, f);
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[n][i] += c[i];
+      }
+      __syncthreads();  // the stretch has been read
+      send(slot);
+      in = in + 1 == D::SLOTS ? 0 : in + 1;
     }
-    __syncthreads();  // the unit has been read: the warps' sums go over it
-    float(*sums)[16][DOWN_RANKS + 1] = (float(*)[16][DOWN_RANKS + 1]) slot;
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) sums[warp][g + 8 * (i >> 1)][n * 8 + 2 * t4 + (i & 1)] = acc[n][i];
+      for (int i = 0; i < 4; i++) s_sum[warp][g + 8 * (i >> 1)][(n * 8 + 2 * t4 + (i & 1) + 8 * (g & 3)) & 31] = acc[n][i];
     __syncthreads();
     float v = 0.0f;  // a warp per row, a lane per rank
 #pragma unroll
-    for (int w = 0; w < 16; w++) v += sums[w][warp][lane];
-    if (warp < count && lane < rank) thin[((size_t)s * M + s_plan.rows[e][warp]) * p.max_rank + j0 + lane] = v;
+    for (int w = 0; w < 16; w++) v += s_sum[w][warp][(lane + 8 * (warp & 3)) & 31];
+    if (warp < count && lane < rank) thin[((size_t)part * M + s_plan.rows[e][warp]) * p.max_rank + j0 + lane] = v;
     __syncthreads();
-    send(ahead, slot);
-    if (ahead < units) ahead = find(ahead + gridDim.x);
-    in = in + 1 == D::SLOTS ? 0 : in + 1;
   }
 }
 
@@ -311,14 +351,14 @@ __global__ void __launch_bounds__(512, 1) pool_down_kernel(const Pool p, const f
 // rows of whole 16-byte pieces.
 template <int DTYPE, bool VEC, bool PIECES>
 __global__ void __launch_bounds__(256, DTYPE == STB_F32 ? 1 : 2) pool_up_kernel(const Pool p, const float *thin, float *y, int M,
-                                                                               int N, int stretches, const SkinnyParts parts,
+                                                                               int N, int stretches, int down_blocks, const SkinnyParts parts,
                                                                                const float *bias) {
   constexpr int NT = UP_COLUMNS / 64;  // 8-column results of a warp
   __shared__ float s_thin[16][MAX_RANK + 4];
   __shared__ Plan s_plan;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   pdl_trigger();
-  make_plan(p, M, s_plan);
+  make_plan(p, M, stretches, down_blocks, s_plan);
   const int groups = s_plan.groups, columns = (N + UP_COLUMNS - 1) / UP_COLUMNS;
   bool waited = false;
   for (int u = blockIdx.x; u < groups * columns; u += gridDim.x) {
@@ -327,14 +367,18 @@ __global__ void __launch_bounds__(256, DTYPE == STB_F32 ? 1 : 2) pool_up_kernel(
     if (!PIECES && rank == 0) continue;
     const int blocks = (rank + 31) / 32;  // of 32 ranks
     const float scale = t >= 0 ? p.scales[t] : 0.0f;
-    Eight<DTYPE, VEC> f[NT];
-    auto read = [&](int kb) {
+    const int wide = blocks * 32;
+    Eight<DTYPE, VEC> f[2][NT];  // of 32 ranks each: the first 64 are read before the wait
+    auto read = [&](int kb, Eight<DTYPE, VEC> (&f)[NT]) {
       const int j = kb * 32 + t4 * 8;
 #pragma unroll
       for (int n = 0; n < NT; n++)
         f[n].load(p.b, ((size_t)t * N + n0 + n * 8 + g) * p.max_rank + j, n0 + n * 8 + g < N ? min(8, rank - j) : 0);
     };
-    if (rank) read(0);
+    if (rank) {
+      read(0, f[0]);
+      read(1, f[1]);
+    }
     // pieces of the tile of 128 columns that this warp's 32 lie in
     int pieces = 0;
     const float *at_piece = nullptr;
@@ -346,6 +390,13 @@ __global__ void __launch_bounds__(256, DTYPE == STB_F32 ? 1 : 2) pool_up_kernel(
     }
     if (!waited) pdl_wait();  // thin, and the shared product
     waited = true;
+    // thin's first parts for this warp's first 32 ranks, on their way together with the pieces
+    auto thin_at = [&](int i) { return thin + (size_t)s_plan.rows[e][i / wide] * p.max_rank + i % wide + lane; };
+    auto thin_in = [&](int i) { return i < count * wide && i % wide + lane < rank; };
+    float w[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      w[k] = thin_in(warp * 32) && k < s_plan.parts ? __ldcg(thin_at(warp * 32) + (size_t)k * M * p.max_rank) : 0.0f;
     float2 base[2][NT];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
@@ -371,21 +422,20 @@ __global__ void __launch_bounds__(256, DTYPE == STB_F32 ? 1 : 2) pool_up_kernel(
         }
       }
     }
-    const int wide = blocks * 32;
     for (int i = warp * 32; i < count * wide; i += 256) {  // 32 ranks of one row
-      const int j = i % wide + lane;
       float v = 0.0f;
-      if (j < rank) {
-        const float *at = thin + (size_t)s_plan.rows[e][i / wide] * p.max_rank + j;
-        for (int s = 0; s < stretches; s += 16) {
-          float w[16];
+      if (i == warp * 32) {
 #pragma unroll
-          for (int k = 0; k < 16; k++) w[k] = s + k < stretches ? __ldcg(at + (size_t)(s + k) * M * p.max_rank) : 0.0f;
-#pragma unroll
-          for (int k = 0; k < 16; k++) v += w[k];
-        }
+        for (int k = 0; k < 8; k++) v += w[k];
       }
-      s_thin[i / wide][j] = v;
+      for (int s = i == warp * 32 ? 8 : 0; s < s_plan.parts; s += 8) {
+        float u[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) u[k] = thin_in(i) && s + k < s_plan.parts ? __ldcg(thin_at(i) + (size_t)(s + k) * M * p.max_rank) : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) v += u[k];
+      }
+      s_thin[i / wide][i % wide + lane] = v;
     }
     __syncthreads();
     float acc[NT][4] = {};
@@ -400,17 +450,17 @@ __global__ void __launch_bounds__(256, DTYPE == STB_F32 ? 1 : 2) pool_up_kernel(
           split_tf32(g < count ? s_thin[g][at] : 0.0f, hi[j][2 * i], lo[j][2 * i]);
           split_tf32(g + 8 < count ? s_thin[g + 8][at] : 0.0f, hi[j][2 * i + 1], lo[j][2 * i + 1]);
         }
-      Eight<DTYPE, VEC> now[NT];
-#pragma unroll
-      for (int n = 0; n < NT; n++) now[n] = f[n];
-      if (kb + 1 < blocks) read(kb + 1);
+      const int live = rank - (kb * 32 + t4 * 8);
 #pragma unroll
       for (int n = 0; n < NT; n++) {
+        if (VEC && live < 8) f[0][n].trim(live);
         float c[4] = {};
-        eight_products<DTYPE>(c, hi, lo, now[n]);
+        eight_products<DTYPE>(c, hi, lo, f[0][n]);
 #pragma unroll
         for (int i = 0; i < 4; i++) acc[n][i] += c[i];
+        f[0][n] = f[1][n];
       }
+      if (kb + 2 < blocks) read(kb + 2, f[1]);
     }
 #pragma unroll
     for (int h = 0; h < 2; h++) {
@@ -433,9 +483,9 @@ __global__ void __launch_bounds__(256, DTYPE == STB_F32 ? 1 : 2) pool_up_kernel(
 }
 
 template <int DTYPE, bool VEC>
-void launch_down(stb_session *s, int grid, const Pool &p, const float *x, float *thin, int M, int K, int stretches, int chunks,
+void launch_down(stb_session *s, int grid, const Pool &p, const float *x, float *thin, int M, int K, int stretches,
                  uint16_t *x3, int terms_rows) {
-  constexpr int SMEM = Down<DTYPE>::SLOTS * Down<DTYPE>::SLOT;
+  constexpr int SMEM = Down<DTYPE>::SMEM;
   {
     static std::mutex mu;
     static bool configured[64] = {};
@@ -446,7 +496,7 @@ void launch_down(stb_session *s, int grid, const Pool &p, const float *x, float 
     }
   }
   launch_kernel(pool_down_kernel<DTYPE, VEC>, dim3(grid), dim3(512), (size_t)SMEM, s->stream, false, p, x, thin, M, K, stretches,
-                chunks, x3, terms_rows);
+                x3, terms_rows);
 }
 
 }  // namespace
@@ -503,8 +553,8 @@ extern "C" int stb_linear_pool(stb_session *s, uint64_t x, uint64_t w, int w_dty
         p.rows = (const int *)rows + m0;
         const int down_grid = skinny ? sms : (int)std::min<int64_t>(sms, (int64_t)mb * stretches * chunks);
         const int up_grid = (int)std::min<int64_t>(resident, (int64_t)mb * columns);
-        if (vec_down) launch_down<DT, true>(s, down_grid, p, xb, thin, mb, K, stretches, chunks, terms, terms_rows);
-        else launch_down<DT, false>(s, down_grid, p, xb, thin, mb, K, stretches, chunks, terms, terms_rows);
+        if (vec_down) launch_down<DT, true>(s, down_grid, p, xb, thin, mb, K, stretches, terms, terms_rows);
+        else launch_down<DT, false>(s, down_grid, p, xb, thin, mb, K, stretches, terms, terms_rows);
         SkinnyParts parts;
         if (skinny) {
           GemvParams g;
@@ -519,11 +569,11 @@ extern "C" int stb_linear_pool(stb_session *s, uint64_t x, uint64_t w, int w_dty
           g.pdl = true;
           count_launch(s, skinny_launch<EPI_PLAIN>(g, (void *)scratch, base, p.err, s->device, s->stream, terms, nullptr, &parts));
           launch_kernel(vec_up ? pool_up_kernel<DT, true, true> : pool_up_kernel<DT, false, true>, dim3(up_grid), dim3(256), 0,
-                        s->stream, true, p, (const float *)thin, yb, mb, N, stretches, parts, (const float *)bias);
+                        s->stream, true, p, (const float *)thin, yb, mb, N, stretches, down_grid, parts, (const float *)bias);
         } else {
           linear(s, (uint64_t)xb, K, w, w_dtype, bias, (uint64_t)yb, N, mb, N, K, true);
           launch_kernel(vec_up ? pool_up_kernel<DT, true, false> : pool_up_kernel<DT, false, false>, dim3(up_grid), dim3(256), 0,
-                        s->stream, true, p, (const float *)thin, yb, mb, N, stretches, parts, (const float *)bias);
+                        s->stream, true, p, (const float *)thin, yb, mb, N, stretches, down_grid, parts, (const float *)bias);
         }
         count_launch(s, 2);
       }
