@@ -235,7 +235,8 @@ int stb_op_causal_attention(stb_session *s, uint64_t q, uint64_t k, uint64_t v, 
 /* Norm and rotation of the query and key heads in one pass, for rows at positions of their own: each head h
  * of row r becomes R(p) (h / sqrt(mean(h^2) + eps) * weight), with R the rotation of stb_op_rope at position
  * p = positions[r].  q: heads * width values per row, rows q_row apart; k the same with kv_heads.  q_weight /
- * k_weight: [width], or 0 to rotate without a norm.  Sums, norm, angle and rotation in double, one rounding.
+ * k_weight: [width], or 0 to rotate without a norm.  Sum of squares, norm and angles in double, their products in
+ * Float32.
  * Rows with a negative position are padding: their outputs stay as they were.  In place (q_out == q with the
  * same row stride, likewise k) is allowed; any other overlap is not.  width is even, at most 512. */
 int stb_op_qk_norm_rope(stb_session *s, uint64_t q, int64_t q_row, int heads, uint64_t k, int64_t k_row, int kv_heads,

@@ -3,11 +3,12 @@
 //   u_d = x_d / sqrt(mean(x^2) + eps) * w_d,   y_d = u_d cos a - u_{d+half} sin a,  y_{d+half} = u_{d+half} cos a + u_d sin a
 // with a = p * theta^(-2 d / width), d < half = width / 2.
 //
-// What bounds it: 8 bytes per element, read and written once, as long as enough loads are under way while the angles
-// are worked out.  A block of 256 threads takes a row at a time (several rows of few heads), all of its heads' loads
-// sent before anything else; the sines and cosines of the row, shared by its heads, go to shared memory meanwhile.  All
-// arithmetic is in double, as stb_op_rmsnorm's and stb_op_rope's, with one rounding: 5 operations and 3 conversions
-// per element, a quarter and a half of what the SM's double and conversion pipes take at the copy rate.
+// What bounds it: 8 bytes per element, read and written once, as long as loads stay under way while the angles are worked
+// out.  Every warp runs alone over its units, whole rows' heads or parts of a row's: three steps' copies ahead, the sines
+// and cosines of the unit's row in shared memory of its own.  Angles, their sines and cosines, the sum of squares and its
+// root are in double; what they are multiplied by is in Float32: at most 2 half steps of the result and 4 of each
+// rotated product beside it.  The rotation in double too took 85 us instead of 60 for 8191 rows of 40 heads of 128
+// (the conversions of its results are the scarce thing), in pairs of Float32 75 us.
 #include <algorithm>
 #include <cmath>
 
@@ -62,104 +63,169 @@ __global__ void __launch_bounds__(256) qk_norm_rope_any_kernel(const NormRope p)
   }
 }
 
-constexpr int THREADS = 256, MAX_ROWS = 8;
+constexpr int THREADS = 128, BLOCKS = 8, STAGES = 4;
 
-// Groups of L lanes take a head each, lane i its elements 4 i .. 4 i + 3 and their partners (i < half / 4 <= L); a block takes
-// `at_once` rows at a time (one, where U > 1), its group g the heads g, g + GROUPS, .. of them, U sent for at once.
-template <int L, int U>
-__global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(const __grid_constant__ NormRope p, int at_once) {
-  constexpr int GROUPS = THREADS / L;
-  __shared__ double s_rate[L * 4];                  // angle per position over pi
-  __shared__ __align__(16) float s_weight[2][L * 8];
-  __shared__ double2 s_turn[2][MAX_ROWS][L * 4];    // (cos, sin), this round's and the next one's
-  const int every = p.heads[0] + p.heads[1], half = p.width / 2, lane = threadIdx.x % L, group = threadIdx.x / L;
+// 1 / sqrt(v) of a positive v to 2^-43: the Float32 root and one Newton step where Float32 has v (the others go the long
+// way), a fifth of the double function's operations.
+__device__ __forceinline__ double inverse_root(double v) {
+  if (!(v > 1e-30 && v < 1e30)) return rsqrt(v);
+  const double y = rsqrtf((float)v);
+  return y * fma(-0.5 * v * y, y, 1.5);
+}
+
+// A step is up to 32 / L neighbouring query heads, or key heads, of a row, L lanes each, lane i its elements 4 i .. 4 i + 3
+// and their partners (i < half / 4 <= L).  A row has q_steps and then k_steps of them, in `parts` units of `per` steps.
+__device__ __forceinline__ void copy16_async(void *dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+
+template <int L>
+__global__ void __launch_bounds__(THREADS, BLOCKS) qk_norm_rope_kernel(const __grid_constant__ NormRope p, int q_steps, int k_steps,
+                                                                       int parts, int per, int64_t units) {
+  constexpr int HEADS = 32 / L;
+  __shared__ double s_rate[L * 4];                 // angle per position over pi
+  __shared__ __align__(16) float s_weight[2][L * 8];  // of q, of k
+  __shared__ __align__(16) float2 s_turn[THREADS / 32][L * 4];  // (cos, sin) of each warp's row
+  __shared__ float4 s_ring[THREADS / 32][STAGES][2][32];  // the steps ahead: a lane reads what it sent for itself
+  const int half = p.width / 2, lane = threadIdx.x % L, in_step = threadIdx.x % 32 / L, per_row = q_steps + k_steps;
   const bool live = lane * 4 < half;
-  const int in_block = U == 1 ? group / every : 0, head0 = U == 1 ? group % every : group;
+  const int warps = gridDim.x * (THREADS / 32), warp = blockIdx.x * (THREADS / 32) + threadIdx.x / 32;
+  const int offset = in_step * p.width + lane * 4;  // of this lane in a step's heads
+
+  // A place in a unit: `left` steps of one side's heads, then `rest` steps of the other's.
+  struct Cursor {
+    float *at;  // this lane's elements of the step
+    int64_t unit;
+    int row, side, left, rest, room, pos;  // room: heads of the side from the step's first on
+  };
+  auto enter = [&](Cursor &c, bool out, int step) {  // at the step-th step of c.side in c.row
+    const float *base = out ? (c.side ? p.y[1] + c.row * p.y_row[1] : p.y[0] + c.row * p.y_row[0])
+                            : (c.side ? p.x[1] + c.row * p.x_row[1] : p.x[0] + c.row * p.x_row[0]);
+    c.at = const_cast<float *>(base) + (int64_t)step * HEADS * p.width + offset;
+    c.room = (c.side ? p.heads[1] : p.heads[0]) - step * HEADS;
+  };
+  auto start = [&](Cursor &c, bool out) {  // of unit c.unit
+    if (c.unit >= units) return;
+    c.row = (int)(c.unit / parts);
+    const int step = (int)(c.unit % parts) * per, end = min(per_row, step + per);
+    c.pos = p.positions[c.row];
+    c.side = step >= q_steps;
+    c.left = (c.side ? end : min(end, q_steps)) - step;
+    c.rest = end - step - c.left;
+    enter(c, out, step - (c.side ? q_steps : 0));
+  };
+  auto advance = [&](Cursor &c, bool out) {
+    c.at += HEADS * p.width;
+    c.room -= HEADS;
+    if (--c.left > 0) return;
+    if (c.rest > 0) {
+      c.side = 1;
+      c.left = c.rest;
+      c.rest = 0;
+      enter(c, out, 0);
+    } else {
+      c.unit += warps;
+      start(c, out);
+    }
+  };
+  Cursor from, to;
+  from.unit = to.unit = warp;
+  start(from, false);
+  start(to, true);
+  float4(*const ring)[2][32] = s_ring[threadIdx.x / 32];
+  auto send = [&](int stage) {
+    if (from.unit < units) {
+      if (live && in_step < from.room && from.pos >= 0) {
+        copy16_async(&ring[stage][0][threadIdx.x % 32], from.at);
+        copy16_async(&ring[stage][1][threadIdx.x % 32], from.at + half);
+      }
+      advance(from, false);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll 1
+  for (int i = 0; i < STAGES - 1; i++) send(i);
   for (int d = threadIdx.x; d < half; d += THREADS) s_rate[d] = exp2(p.rate * d) * 0.31830988618379067154;
   for (int i = threadIdx.x; i < 2 * p.width; i += THREADS) {
     const float *w = i < p.width ? p.w[0] : p.w[1];
     s_weight[i < p.width ? 0 : 1][i % p.width] = w ? w[i % p.width] : 1.0f;
   }
-  const bool normed = p.w[0] || p.w[1];
+  const double mean = 1.0 / p.width;
   __syncthreads();
-  int buffer = 0;
+  float2 *const turn = s_turn[threadIdx.x / 32];  // of row `turned`
+  int turned = -1;
+  int stage = 0;
 #pragma unroll 1
-  for (int64_t r0 = (int64_t)blockIdx.x * at_once; r0 < p.rows; r0 += (int64_t)gridDim.x * at_once, buffer ^= 1) {
-    const int64_t row = r0 + in_block;
-    const bool mine = in_block < at_once && row < p.rows && p.positions[row] >= 0 && live;
-    for (int i = threadIdx.x; i < at_once * half; i += THREADS) {
-      const int r = i / half, d = i % half, pos = r0 + r < p.rows ? p.positions[r0 + r] : -1;
-      if (pos < 0) continue;
-      double sn, cs;
-      sincospi((double)pos * s_rate[d], &sn, &cs);
-      s_turn[buffer][r][d] = make_double2(cs, sn);
-    }
-    bool waited = false;
-#pragma unroll 1
-    for (int h0 = head0; h0 - head0 < (U == 1 ? 1 : every); h0 += U * GROUPS) {
-      float4 a[U], b[U];
-#pragma unroll
-      for (int k = 0; k < U; k++) {
-        const int h = h0 + k * GROUPS, side = h >= p.heads[0];
-        if (!mine || h >= every) continue;
-        const float *x = (side ? p.x[1] + row * p.x_row[1] : p.x[0] + row * p.x_row[0]) + (size_t)(h - (side ? p.heads[0] : 0)) * p.width + lane * 4;
-        a[k] = __ldcs((const float4 *)x);
-        b[k] = __ldcs((const float4 *)(x + half));
-      }
-      if (!waited) __syncthreads();
-      waited = true;
-#pragma unroll
-      for (int k = 0; k < U; k++) {
-        const int h = h0 + k * GROUPS, side = h >= p.heads[0];
-        const bool has = mine && h < every;
-        const float u[4] = {a[k].x, a[k].y, a[k].z, a[k].w}, v[4] = {b[k].x, b[k].y, b[k].z, b[k].w};
-        double inv = 1.0;
-        if (normed) {  // every group of the warp takes part in the shuffles
-          double sq = 0.0;
-          if (has) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) sq = fma((double)u[i], (double)u[i], fma((double)v[i], (double)v[i], sq));
-          }
-#pragma unroll
-          for (int off = L / 2; off > 0; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
-          if (side ? p.w[1] != nullptr : p.w[0] != nullptr) inv = rsqrt(sq / p.width + p.eps);
+  while (to.unit < units) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    const float4 f = ring[stage][0][threadIdx.x % 32], g = ring[stage][1][threadIdx.x % 32];
+    send(stage == 0 ? STAGES - 1 : stage - 1);
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+    if (to.pos >= 0) {
+      if (turned != to.row) {
+        turned = to.row;
+        __syncwarp();
+        for (int d = threadIdx.x % 32; d < half; d += 32) {
+          double sn, cs;
+          sincospi((double)to.pos * s_rate[d], &sn, &cs);
+          turn[d] = make_float2((float)cs, (float)sn);
         }
-        if (!has) continue;
-        const float4 wa = *(const float4 *)&s_weight[side][lane * 4], wb = *(const float4 *)&s_weight[side][lane * 4 + half];
+        __syncwarp();
+      }
+      const bool has = live && in_step < to.room;
+      float u[4] = {f.x, f.y, f.z, f.w}, v[4] = {g.x, g.y, g.z, g.w};
+      if (to.side ? p.w[1] != nullptr : p.w[0] != nullptr) {  // the same for the whole warp
+        double sq = 0.0;
+        if (has) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) sq = fma((double)u[i], (double)u[i], fma((double)v[i], (double)v[i], sq));
+        }
+#pragma unroll
+        for (int off = L / 2; off > 0; off >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, off);
+        double root = inverse_root(fma(sq, mean, p.eps));
+        float down = 1.0f;
+        if (root < 1e-36) {  // Float32 would have it with few bits
+          root *= 0x1p64;
+          down = 0x1p-64f;
+        }
+        const float inv = (float)root;
+        const float4 wa = *(const float4 *)&s_weight[to.side][lane * 4], wb = *(const float4 *)&s_weight[to.side][lane * 4 + half];
         const float wf[4] = {wa.x, wa.y, wa.z, wa.w}, wg[4] = {wb.x, wb.y, wb.z, wb.w};
+        if (down != 1.0f) {
+#pragma unroll
+          for (int k = 0; k < 4; k++) u[k] *= down, v[k] *= down;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) u[k] = u[k] * inv * wf[k], v[k] = v[k] * inv * wg[k];
+      }
+      if (has) {
         float r[4], s[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const double2 turn = s_turn[buffer][in_block][lane * 4 + i];
-          const double c = (double)u[i] * (inv * (double)wf[i]), d = (double)v[i] * (inv * (double)wg[i]);
-          r[i] = (float)(c * turn.x - d * turn.y);
-          s[i] = (float)(d * turn.x + c * turn.y);
+        for (int i = 0; i < 4; i += 2) {
+          const float4 t = *(const float4 *)&turn[lane * 4 + i];
+          r[i] = fmaf(u[i], t.x, -(v[i] * t.y));
+          s[i] = fmaf(v[i], t.x, u[i] * t.y);
+          r[i + 1] = fmaf(u[i + 1], t.z, -(v[i + 1] * t.w));
+          s[i + 1] = fmaf(v[i + 1], t.z, u[i + 1] * t.w);
         }
-        float *y = (side ? p.y[1] + row * p.y_row[1] : p.y[0] + row * p.y_row[0]) + (size_t)(h - (side ? p.heads[0] : 0)) * p.width + lane * 4;
-        __stcs((float4 *)y, make_float4(r[0], r[1], r[2], r[3]));
-        __stcs((float4 *)(y + half), make_float4(s[0], s[1], s[2], s[3]));
+        __stcs((float4 *)to.at, make_float4(r[0], r[1], r[2], r[3]));
+        __stcs((float4 *)(to.at + half), make_float4(s[0], s[1], s[2], s[3]));
       }
     }
-    if (!waited) __syncthreads();
+    advance(to, true);
   }
 }
 
 template <int L>
 void launch_rows(stb_session *s, const NormRope &p) {
-  constexpr int GROUPS = THREADS / L;
-  const int every = p.heads[0] + p.heads[1];
-  const int at_once = every <= GROUPS ? std::min(MAX_ROWS, GROUPS / every) : 1;
-  const int64_t rounds = ((int64_t)p.rows + at_once - 1) / at_once;
-  auto go = [&](auto u) {
-    constexpr int U = decltype(u)::value;
-    const int grid = (int)std::min<int64_t>(rounds, (int64_t)tc::sm_count(s->device) * (U <= 2 ? 4 : 3));
-    launch_kernel(qk_norm_rope_kernel<L, U>, dim3(grid), dim3(THREADS), 0, s->stream, false, p, at_once);
-  };
-  const int deep = (every + GROUPS - 1) / GROUPS;
-  if (deep == 1) go(std::integral_constant<int, 1>());
-  else if (deep == 2) go(std::integral_constant<int, 2>());
-  else if (deep == 3 || deep == 6) go(std::integral_constant<int, 3>());
-  else go(std::integral_constant<int, 5>());
+  const int heads = 32 / L, q_steps = (p.heads[0] + heads - 1) / heads, k_steps = (p.heads[1] + heads - 1) / heads;
+  const int per_row = q_steps + k_steps, most = tc::sm_count(s->device) * BLOCKS;
+  // Rows in parts of five steps (59 us for 8191 rows of 40 heads of 128, 64 with parts of ten), of fewer where that leaves warps idle.
+  const int64_t warps = (int64_t)most * (THREADS / 32);
+  const int per = (int)std::max<int64_t>(1, std::min<int64_t>(5, (int64_t)p.rows * per_row / warps));
+  const int parts = (per_row + per - 1) / per;
+  const int64_t units = (int64_t)p.rows * parts, blocks = std::min<int64_t>((units + THREADS / 32 - 1) / (THREADS / 32), most);
+  launch_kernel(qk_norm_rope_kernel<L>, dim3((unsigned)blocks), dim3(THREADS), 0, s->stream, false, p, q_steps, k_steps, parts, per, units);
 }
 
 }  // namespace

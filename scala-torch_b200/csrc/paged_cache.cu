@@ -155,21 +155,28 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedView c, co
     for (int side = 0; side < 2; side++) {
       int e = 0;
       float inverse = 1.0f;
-      bool finite = true;
-      if (DTYPE == STB_E4M3) {  // every group of the warp takes part in the shuffles
-        float top = 0.0f;
+      bool infinite = false;
+      if (DTYPE == STB_E4M3) {  // every group of the warp takes part in the reductions
+        auto widest = [&](bool finite_only) {
+          float top = 0.0f;
 #pragma unroll
-        for (int v = 0; v < V; v++) {
-          const float f[4] = {x[side][k][v].x, x[side][k][v].y, x[side][k][v].z, x[side][k][v].w};
+          for (int v = 0; v < V; v++) {
+            const float f[4] = {x[side][k][v].x, x[side][k][v].y, x[side][k][v].z, x[side][k][v].w};
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const float a = fabsf(f[i]);
-            if (a <= 3.402823466e38f) top = fmaxf(top, a);
-            else finite = false;
+            for (int i = 0; i < 4; i++)
+              if (!finite_only || fabsf(f[i]) < INFINITY) top = fmaxf(top, fabsf(f[i]));  // drops NaNs
           }
-        }
+          if constexpr (L == 32) {
+            return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+          } else {
 #pragma unroll
-        for (int off = L / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            for (int off = L / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            return top;
+          }
+        };
+        float top = widest(false);
+        infinite = top == INFINITY;
+        if (__any_sync(0xffffffffu, infinite)) top = widest(true);
         e = e4m3_exponent(top);
         inverse = scale_of((uint8_t)(127 - e));
       }
@@ -192,11 +199,11 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedView c, co
         } else {
           uint32_t u = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f.x * inverse, f.y * inverse), __NV_SATFINITE, __NV_E4M3) |
                        (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f.z * inverse, f.w * inverse), __NV_SATFINITE, __NV_E4M3) << 16;
-          if (!finite) {  // the conversion would saturate an infinity
+          if (infinite) {  // the conversion would saturate it
             const float g[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
             for (int b = 0; b < 4; b++)
-              if (!isfinite(g[b])) u = (u & ~(0xffu << (8 * b))) | 0x7fu << (8 * b);
+              if (isinf(g[b])) u = (u & ~(0xffu << (8 * b))) | 0x7fu << (8 * b);
           }
           *(uint32_t *)((uint8_t *)base + i) = u;
         }

@@ -2,9 +2,10 @@
 stb_linear_pool) against their definitions in float64 (tests/serving_oracle.py).
 
 Tolerances, from the arithmetic:
-* norm and rotation: double with one rounding, so half a step of Float32 (2^-24 |y|), plus the double operations'
-  own error: angles up to 2^31 carry 2^31 * 2^-52 ~ 5e-7 at worst; positions here stay below 2^20, 1e-9 of the
-  pair's magnitude.
+* norm and rotation, y = fma(a, c, -(b s)) with a = x inv w, b = x' inv w': in half steps h of Float32 (2^-24), inv, the two
+  products of a and c are rounded once each (4 h |a c|), likewise those of b s and b s itself (5 h |b s|), and the sum
+  once (h |y|).  |a c| + |b s| <= sqrt(2) pair, so 5 sqrt(2) < 7.1 h of the pair's magnitude and h |y|; the norm's factor
+  before its rounding (2^-43) and the angle (two double roundings at positions below 2^20: 5e-10) add 1e-9 of the pair.
 * cache write and read: equal bits.
 * attention in Float32: a score's rounding error is at most (width + 8) 2^-24 of its sum |q k| / sqrt(width) (one
   rounding per product and addition, of any order), a weight moves by e^(2 |error|) - 1 of itself against the sum,
@@ -72,7 +73,7 @@ def check_norm_rope(got, x, w, pos, eps, theta):
     want = norm_rope(x, w, pos, eps, theta)
     half = want.shape[-1] // 2
     pair = np.hypot(want[..., :half], want[..., half:])
-    tol = HALF * np.abs(want) + 1e-9 * np.concatenate((pair, pair), -1) + 1e-37
+    tol = HALF * np.abs(want) + (7.1 * HALF + 1e-9) * np.concatenate((pair, pair), -1) + 1e-37
     np.testing.assert_array_less(np.abs(got.astype(np.float64) - want), tol)
 
 
