@@ -10,7 +10,8 @@
 // is the lanes', the same in both operands.
 //   1. down: thin[s][m][j] = x[m] . A_t[j] over the s-th stretch of K; beside it the shared product's own prologue, the
 //      three BF16 terms of x, where the product takes the skinny tensor-core form;
-//   2. the shared product, launched as a dependent (its weights stream in while the first kernel drains);
+//   2. the shared product, launched as a dependent (its weights stream in while the first kernel drains); where it takes
+//      the vector form, it comes first and the first kernel runs beside it;
 //   3. up: adds the stretches in order, multiplies by B_t; it also adds up the skinny form's pieces of the shared
 //      product (or reads y), and the bias.  Its factors are read before it waits.
 // Rows go through in blocks of 64, the skinny form's.
@@ -221,7 +222,7 @@ __device__ __forceinline__ void copy16_async(void *dst, const void *src, bool li
 // rows of whole 16-byte pieces (plain loads otherwise).
 template <int DTYPE, bool VEC>
 __global__ void __launch_bounds__(512, 1) pool_down_kernel(const Pool p, const float *x, float *thin, int M, int K, int stretches,
-                                                           uint16_t *x3, int terms_rows) {
+                                                           uint16_t *x3, int terms_rows, bool behind) {
   using D = Down<DTYPE>;
   constexpr int NT = DOWN_RANKS / 8, ESZ = D::ESZ;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -344,6 +345,7 @@ __global__ void __launch_bounds__(512, 1) pool_down_kernel(const Pool p, const f
     if (warp < count && lane < rank) thin[((size_t)part * M + s_plan.rows[e][warp]) * p.max_rank + j0 + lane] = v;
     __syncthreads();
   }
+  if (behind) pdl_wait();  // the third kernel waits for this one alone: the shared product has to be done by then
 }
 
 // y[m][n] = base + scale_t thin[m] . B_t[n] + bias[n]: units (group of rows, 256 columns) in turn over the blocks;
@@ -484,7 +486,7 @@ __global__ void __launch_bounds__(256, DTYPE == STB_F32 ? 1 : 2) pool_up_kernel(
 
 template <int DTYPE, bool VEC>
 void launch_down(stb_session *s, int grid, const Pool &p, const float *x, float *thin, int M, int K, int stretches,
-                 uint16_t *x3, int terms_rows) {
+                 uint16_t *x3, int terms_rows, bool behind) {
   constexpr int SMEM = Down<DTYPE>::SMEM;
   {
     static std::mutex mu;
@@ -495,8 +497,8 @@ void launch_down(stb_session *s, int grid, const Pool &p, const float *x, float 
       if (s->device >= 0 && s->device < 64) configured[s->device] = true;
     }
   }
-  launch_kernel(pool_down_kernel<DTYPE, VEC>, dim3(grid), dim3(512), (size_t)SMEM, s->stream, false, p, x, thin, M, K, stretches,
-                x3, terms_rows);
+  launch_kernel(pool_down_kernel<DTYPE, VEC>, dim3(grid), dim3(512), (size_t)SMEM, s->stream, behind, p, x, thin, M, K, stretches,
+                x3, terms_rows, behind);
 }
 
 }  // namespace
@@ -553,8 +555,9 @@ extern "C" int stb_linear_pool(stb_session *s, uint64_t x, uint64_t w, int w_dty
         p.rows = (const int *)rows + m0;
         const int down_grid = skinny ? sms : (int)std::min<int64_t>(sms, (int64_t)mb * stretches * chunks);
         const int up_grid = (int)std::min<int64_t>(resident, (int64_t)mb * columns);
-        if (vec_down) launch_down<DT, true>(s, down_grid, p, xb, thin, mb, K, stretches, terms, terms_rows);
-        else launch_down<DT, false>(s, down_grid, p, xb, thin, mb, K, stretches, terms, terms_rows);
+        if (!skinny) linear(s, (uint64_t)xb, K, w, w_dtype, bias, (uint64_t)yb, N, mb, N, K, true);
+        if (vec_down) launch_down<DT, true>(s, down_grid, p, xb, thin, mb, K, stretches, terms, terms_rows, !skinny);
+        else launch_down<DT, false>(s, down_grid, p, xb, thin, mb, K, stretches, terms, terms_rows, !skinny);
         SkinnyParts parts;
         if (skinny) {
           GemvParams g;
@@ -571,7 +574,6 @@ extern "C" int stb_linear_pool(stb_session *s, uint64_t x, uint64_t w, int w_dty
           launch_kernel(vec_up ? pool_up_kernel<DT, true, true> : pool_up_kernel<DT, false, true>, dim3(up_grid), dim3(256), 0,
                         s->stream, true, p, (const float *)thin, yb, mb, N, stretches, down_grid, parts, (const float *)bias);
         } else {
-          linear(s, (uint64_t)xb, K, w, w_dtype, bias, (uint64_t)yb, N, mb, N, K, true);
           launch_kernel(vec_up ? pool_up_kernel<DT, true, false> : pool_up_kernel<DT, false, false>, dim3(up_grid), dim3(256), 0,
                         s->stream, true, p, (const float *)thin, yb, mb, N, stretches, down_grid, parts, (const float *)bias);
         }

@@ -56,7 +56,7 @@ static void launch_one(const GemvParams &p, cudaStream_t stream) {
   // block's reduction with the next block's loads (a resident-capped grid-stride loop measured
   // slower on the 1 GB lm_head: 229 vs 211 us).
   const long blocks = items;
-  launch_kernel(gemv_kernel<MT, ROWS, TPR, WT, EPI>, dim3((unsigned)blocks), dim3(256), 0, stream, p.pdl, p, mtiles,
+  launch_kernel(gemv_kernel<MT, ROWS, TPR, WT, EPI>, dim3((unsigned)blocks), dim3(256), 0, stream, p.pdl && !p.leads, p, mtiles,
                 (int)items);
 }
 
@@ -146,7 +146,7 @@ __global__ void fill_bias_kernel(float *y, int ldy, const float *bias, int M, in
 }
 
 void linear(stb_session *s, uint64_t x, int ldx, uint64_t w, int w_dtype, uint64_t bias, uint64_t y, int ldy,
-            int M, int N, int K, bool pdl) {
+            int M, int N, int K, bool leads) {
   STB_REQUIRE(M >= 0 && N >= 0 && K >= 0, "Linear dimensions must be nonnegative");
   STB_REQUIRE(w_dtype == STB_F32 || w_dtype == STB_BF16 || w_dtype == STB_F16, "unsupported weight dtype");
   if (M == 0 || N == 0) return;
@@ -189,7 +189,6 @@ void linear(stb_session *s, uint64_t x, int ldx, uint64_t w, int w_dtype, uint64
   p.y = (float *)y;
   p.ldy = ldy;
   p.bias = (const float *)bias;
-  p.pdl = pdl;
   if (skinny_eligible(M, N, K, w_dtype, (const void *)w)) {
     // 2+ token rows: tensor cores with the activations split into three BF16 terms, 64-row blocks
     const uint64_t bytes = skinny_scratch_bytes(M, N, K, s->device);
@@ -197,6 +196,7 @@ void linear(stb_session *s, uint64_t x, int ldx, uint64_t w, int w_dtype, uint64
     count_launch(s, skinny_launch<EPI_PLAIN>(p, scratch, bytes, session_error_word(s), s->device, s->stream));
     return;
   }
+  p.pdl = p.leads = leads;
   launch_gemv<EPI_PLAIN>(p, w_dtype, choose_gemv(M, N, K, false), s->stream);
   count_launch(s);
 }

@@ -52,6 +52,7 @@ struct GemvParams {
   int row_offset = 0;                  // global index of row 0 (vocab shard offset)
   const int *stop = nullptr;  // device flag; nonzero makes the kernel a no-op
   bool pdl = false;           // launched as a programmatic dependent of the previous kernel
+  bool leads = false;         // with pdl: launched plainly, and lets the next kernel start early all the same
   PeerArgs peer{};            // EPI_PEER: receive slots of every rank (slot row stride = ldy)
 };
 
@@ -487,8 +488,8 @@ int skinny_nt(int M);
 // Whether a residual projection of N outputs can do the next projection's RMSNorm prologue (SkinnyNext).
 bool skinny_norm_fusable(int N);
 
-// stb_linear (gemv.cu).  pdl: the first kernel is launched as a programmatic dependent of the one before it.
+// stb_linear (gemv.cu).  leads: a vector kernel lets a programmatic dependent launched behind it start early.
 void linear(stb_session *s, uint64_t x, int ldx, uint64_t w, int w_dtype, uint64_t bias, uint64_t y, int ldy,
-            int M, int N, int K, bool pdl = false);
+            int M, int N, int K, bool leads = false);
 
 }  // namespace stb

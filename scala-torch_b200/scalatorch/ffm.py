@@ -17,6 +17,7 @@ There is no fallback: if libstb200.so is missing or fails to load, every entry p
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import os
 from dataclasses import dataclass, field
@@ -120,9 +121,14 @@ def _declare(L):
         fn.argtypes = args
 
 
+_functions: dict = {}  # bound entry points by name
+
+
 def call(name: str, *args) -> None:
     """CudaDriver.call idiom: nonzero status -> exception with the library's message."""
-    fn = getattr(library(), name)
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(library(), name)
     code = fn(*args)
     if code != 0:
         msg = library().stb_last_error().decode(errors="replace")
@@ -134,6 +140,17 @@ def call(name: str, *args) -> None:
 def require(cond: bool, message: str) -> None:
     if not cond:
         raise IllegalArgumentException(message)
+
+
+def _of_tensors(method):
+    """An operand that is no tensor at all is rejected like any other that the operator does not take."""
+    @functools.wraps(method)
+    def checked(*args, **kw):
+        try:
+            return method(*args, **kw)
+        except AttributeError as e:
+            raise IllegalArgumentException(f"operands must be tensors of the session: {e}") from e
+    return checked
 
 
 @dataclass(eq=False)
@@ -613,20 +630,19 @@ class B200Session:
         return B200AttentionCache(self, batch_size, heads, capacity, key_width, value_width, max_bytes)
 
     # -- several requests in one batch
-    def _rows_of(self, t: DeviceTensor, dtype: int = STB_F32) -> int:
-        """Checks a tensor whose rows may lie apart; elements between its rows."""
-        if t.__class__ is not DeviceTensor or t.session is not self:
-            raise IllegalArgumentException("tensor belongs to another session")
-        if not t._alive[0]:
-            raise IllegalStateException("validate", 6, "tensor was released")
-        if t.dtype != dtype or t.transposed_weight:
-            raise IllegalArgumentException("operation takes Float32 rows and int32 indices")
-        if t.row_stride:
-            return t.row_stride
-        n = 1
-        for d in t.shape[1:]:
-            n *= d
-        return n
+    # These calls are a few microseconds on the GPU: their checks are one expression per tensor on the way through, and
+    # _refuse names what was wrong with it.
+    def _refuse(self, *tensors) -> None:
+        """tensors: (tensor, dtype, shape or None), of which one at least is not what the operator takes."""
+        self._check()
+        for t, dtype, shape in tensors:
+            require(isinstance(t, DeviceTensor) and t.session is self, "tensor belongs to another session")
+            if not t._alive[0]:
+                raise IllegalStateException("validate", 6, "tensor was released")
+            require(t.dtype == dtype and not t.transposed_weight, "operation takes Float32 rows and int32 indices")
+            require(shape is None or t.shape == shape, f"shape mismatch: {t.shape} where {shape} is needed")
+            require(dtype == STB_F32 or t.row_stride == 0, "operation takes packed indices, not a view of columns")
+        raise IllegalArgumentException("operands do not fit together")
 
     def _outs(self, *shapes):
         """Float32 outputs of an operator that has several; none is left behind where one does not fit."""
@@ -640,13 +656,7 @@ class B200Session:
             raise
         return tuple(made)
 
-    def _indices(self, t: DeviceTensor, shape) -> int:
-        """Checks a packed int32 index tensor; its address."""
-        self._rows_of(t, STB_I32)
-        if t.shape != shape or t.row_stride:
-            raise IllegalArgumentException("index shape mismatch")
-        return t.address
-
+    @_of_tensors
     def qk_norm_rope(self, query: DeviceTensor, key: DeviceTensor, query_weight: DeviceTensor | None,
                      key_weight: DeviceTensor | None, positions: DeviceTensor, epsilon: float = 1e-6,
                      theta: float = 10000.0, out=None):
@@ -654,29 +664,32 @@ class B200Session:
         own position, in one pass: query (rows, heads, width), key (rows, kv_heads, width), positions int32 (rows,).
         query and key may be columns of a fused projection.  Returns (query, key); out = (query, key) tensors to
         write, which may be the inputs themselves.  A row with a negative position is padding and left as it is."""
-        self._check()
-        q_row, k_row = self._rows_of(query), self._rows_of(key)
-        if len(query.shape) != 3 or len(key.shape) != 3 or query.shape[0] != key.shape[0] or query.shape[2] != key.shape[2]:
+        qs, ks = getattr(query, "shape", ()), getattr(key, "shape", ())
+        if len(qs) != 3 or len(ks) != 3 or qs[0] != ks[0] or qs[2] != ks[2]:
             raise IllegalArgumentException("query and key heads must have shapes (rows, heads, width)")
-        rows, heads, width = query.shape
-        for w in (query_weight, key_weight):
-            if w is not None:
-                self._rows_of(w)
-                if w.shape != (width,):
-                    raise IllegalArgumentException("invalid RMSNorm shapes")
-        at = self._indices(positions, (rows,))
+        rows, heads, width = qs
         made = out is None
         if made:
-            out = self._outs(query.shape, key.shape)
+            self._check()
+            out = self._outs(qs, ks)
         yq, yk = out
-        yq_row, yk_row = self._rows_of(yq), self._rows_of(yk)
-        if yq.shape != query.shape or yk.shape != key.shape:
-            raise IllegalArgumentException("output shape mismatch")
+        qw, kw = query_weight, key_weight
         try:
-            call("stb_op_qk_norm_rope", self.handle, query.address, q_row, heads, key.address, k_row, key.shape[1], width,
-                 rows, query_weight.address if query_weight is not None else 0,
-                 key_weight.address if key_weight is not None else 0, at, epsilon, theta, yq.address, yq_row, yk.address,
-                 yk_row)
+            if not (not self._closed and query.session is self and query._alive[0] and query.dtype == STB_F32 and not query.transposed_weight
+                    and key.session is self and key._alive[0] and key.dtype == STB_F32 and not key.transposed_weight
+                    and positions.session is self and positions._alive[0] and positions.dtype == STB_I32
+                    and positions.shape == (rows,) and positions.row_stride == 0
+                    and yq.session is self and yq._alive[0] and yq.dtype == STB_F32 and yq.shape == qs and not yq.transposed_weight
+                    and yk.session is self and yk._alive[0] and yk.dtype == STB_F32 and yk.shape == ks and not yk.transposed_weight
+                    and (qw is None or qw.session is self and qw._alive[0] and qw.dtype == STB_F32 and qw.shape == (width,))
+                    and (kw is None or kw.session is self and kw._alive[0] and kw.dtype == STB_F32 and kw.shape == (width,))):
+                self._refuse((query, STB_F32, None), (key, STB_F32, None), (positions, STB_I32, (rows,)), (yq, STB_F32, qs), (yk, STB_F32, ks),
+                             *[(w, STB_F32, (width,)) for w in (qw, kw) if w is not None])
+            kv_heads = ks[1]
+            call("stb_op_qk_norm_rope", self.handle, query.address, query.row_stride or heads * width, heads, key.address,
+                 key.row_stride or kv_heads * width, kv_heads, width, rows, 0 if qw is None else qw.address,
+                 0 if kw is None else kw.address, positions.address, epsilon, theta, yq.address, yq.row_stride or heads * width,
+                 yk.address, yk.row_stride or kv_heads * width)
         except Exception:
             if made:
                 self.release(yq)
@@ -695,29 +708,31 @@ class B200Session:
         b (slots, out, max_rank), ranks int32 (slots,), scales Float32 (slots,)."""
         return AdapterPool(self, a, b, ranks, scales)
 
+    @_of_tensors
     def linear_adapted(self, x: DeviceTensor, weight: DeviceTensor, pool: "AdapterPool", rows: DeviceTensor,
                        bias: DeviceTensor | None = None, out: DeviceTensor | None = None) -> DeviceTensor:
         """x.W^T + scale (x.A^T).B^T + bias with row m's adapter rows[m] of the pool (int32; negative: none)."""
-        self._validate(x)
-        self._validate(weight)
-        require(weight.transposed_weight, "weight must be a resident (out,in) weight")
-        require(x.dtype == STB_F32 and not x.transposed_weight, "activations must be Float32")
-        require(len(x.shape) == 2 and weight.shape[0] == x.shape[1], "Linear shape mismatch")
-        M, K = x.shape
-        N = weight.shape[1]
-        require(pool.session is self and pool.inner == K and pool.out == N, "Linear adapter shape mismatch")
+        require(isinstance(pool, AdapterPool) and pool.session is self, "adapter pool belongs to another session")
+        M, K, N = x.shape[0] if len(x.shape) == 2 else -1, pool.inner, pool.out
+        if not (not self._closed and x.session is self and x._alive[0] and x.dtype == STB_F32 and x.shape == (M, K) and not x.transposed_weight
+                and x.row_stride == 0 and weight.session is self and weight._alive[0] and weight.transposed_weight
+                and weight.shape == (K, N) and rows.session is self and rows._alive[0] and rows.dtype == STB_I32
+                and rows.shape == (M,) and rows.row_stride == 0
+                and (bias is None or bias.session is self and bias._alive[0] and bias.dtype == STB_F32 and bias.shape == (N,))):
+            self._validate(x)
+            self._validate(weight)
+            require(weight.transposed_weight, "weight must be a resident (out,in) weight")
+            require(x.dtype == STB_F32 and not x.transposed_weight, "activations must be Float32")
+            require(weight.shape == (K, N), "Linear adapter shape mismatch")
+            self._refuse((x, STB_F32, (M, K)), (rows, STB_I32, (M,)), *([(bias, STB_F32, (N,))] if bias is not None else []))
         pool.check()
-        if bias is not None:
-            self._validate(bias)
-            require(bias.shape == (N,) and bias.dtype == STB_F32, "Linear bias shape mismatch")
-        at = self._indices(rows, (M,))
         y = self._out((M, N)) if out is None else out
-        if out is not None:
+        if not (y.session is self and y._alive[0] and y.dtype == STB_F32 and y.shape == (M, N) and not y.transposed_weight and y.row_stride == 0):
             self._validate(y)
-            require(y.shape == (M, N) and y.dtype == STB_F32 and not y.transposed_weight, "output shape mismatch")
+            self._refuse((y, STB_F32, (M, N)))
         try:
-            call("stb_linear_pool", self.handle, x.address, weight.address, weight.dtype,
-                 bias.address if bias is not None else 0, pool.ref, at, y.address, M, N, K)
+            call("stb_linear_pool", self.handle, x.address, weight.address, weight.dtype, 0 if bias is None else bias.address,
+                 pool.ref, rows.address, y.address, M, N, K)
         except Exception:
             if out is None:
                 self.release(y)
@@ -857,56 +872,73 @@ class B200PagedCache:
                                      self.pages, self.page_size, self.kv_heads, self.width)
         self.ref = ctypes.byref(self._struct)
 
-    def _tables(self, tables: DeviceTensor):
-        s = self.session
-        s._check()
+    def _check(self) -> None:
+        self.session._check()
         for t in self.tensors:
             if not t._alive[0]:
                 raise IllegalStateException("paged cache", 6, "tensor was released")
-        s._rows_of(tables, STB_I32)
-        if len(tables.shape) != 2 or tables.row_stride:
-            raise IllegalArgumentException("page tables must have shape (batch, blocks)")
-        return tables.shape
 
-    def _rows(self, t: DeviceTensor, rows: int, heads_first: bool = False):
-        """(row, head) strides of a (rows, kv_heads, width) or (kv_heads, rows, width) tensor."""
-        stride = self.session._rows_of(t)
-        if t.shape != ((self.kv_heads, rows, self.width) if heads_first else (rows, self.kv_heads, self.width)):
-            raise IllegalArgumentException("paged rows must have shape (rows, kv_heads, width)")
-        return (self.width, stride) if heads_first else (stride, self.width)
+    def _open(self, tables, *indices) -> None:
+        """Checks the cache, the page tables and row indices of one length."""
+        s = self.session
+        alive = not s._closed
+        for t in self.tensors:
+            alive = alive and t._alive[0]
+        if not (alive and tables.session is s and tables._alive[0] and tables.dtype == STB_I32 and len(tables.shape) == 2
+                and tables.row_stride == 0):
+            self._check()
+            require(len(getattr(tables, "shape", ())) == 2, "page tables must have shape (batch, blocks)")
+            s._refuse((tables, STB_I32, None))
+        shape = indices[0].shape
+        for t in indices:
+            if not (t.session is s and t._alive[0] and t.dtype == STB_I32 and t.shape == shape and len(shape) == 1 and t.row_stride == 0):
+                require(len(shape) == 1, "row indices must have shape (rows,)")
+                s._refuse((t, STB_I32, shape))
 
+    def _rows(self, t: DeviceTensor, shape) -> int:
+        """Checks a Float32 tensor of this shape; elements between its rows."""
+        s = self.session
+        if not (t.session is s and t._alive[0] and t.dtype == STB_F32 and t.shape == shape and not t.transposed_weight):
+            s._refuse((t, STB_F32, shape))
+        return t.row_stride or shape[1] * shape[2]
+
+    @_of_tensors
     def append(self, key: DeviceTensor, value: DeviceTensor, tables: DeviceTensor, sequences: DeviceTensor,
                positions: DeviceTensor) -> None:
         """Writes key and value rows (rows, kv_heads, width) at positions[r] of request sequences[r], rounded or quantised
         to the cache's type.  Rows with a negative sequence or position are padding; no two rows may name one token."""
-        batch, blocks = self._tables(tables)
-        s = self.session
-        rows = sequences.shape[0] if len(sequences.shape) == 1 else -1
-        seq, pos = s._indices(sequences, (rows,)), s._indices(positions, (rows,))
-        (kr, kh), (vr, vh) = self._rows(key, rows), self._rows(value, rows)
-        call("stb_op_paged_append", s.handle, self.ref, key.address, kr, kh, value.address, vr, vh, tables.address, batch,
-             blocks, seq, pos, rows)
+        self._open(tables, sequences, positions)
+        rows, w = sequences.shape[0], self.width
+        shape = (rows, self.kv_heads, w)
+        key_row, value_row = self._rows(key, shape), self._rows(value, shape)
+        batch, blocks = tables.shape
+        call("stb_op_paged_append", self.session.handle, self.ref, key.address, key_row, w, value.address, value_row, w, tables.address,
+             batch, blocks, sequences.address, positions.address, rows)
 
+    @_of_tensors
     def read(self, tables: DeviceTensor, sequences: DeviceTensor, positions: DeviceTensor, out=None,
              heads_first: bool = False):
         """(key, value) of the named tokens in Float32, (rows, kv_heads, width), or (kv_heads, rows, width) with
         heads_first -- causal_attention's layout for one request.  With `out` the two tensors are written, padding
         rows left as they are; without it padding rows come back as zeros."""
-        batch, blocks = self._tables(tables)
-        s = self.session
-        rows = sequences.shape[0] if len(sequences.shape) == 1 else -1
-        seq, pos = s._indices(sequences, (rows,)), s._indices(positions, (rows,))
+        self._open(tables, sequences, positions)
+        s, rows, w = self.session, sequences.shape[0], self.width
+        batch, blocks = tables.shape
+        shape = (self.kv_heads, rows, w) if heads_first else (rows, self.kv_heads, w)
         made = out is None
         if made:
-            shape = (self.kv_heads, rows, self.width) if heads_first else (rows, self.kv_heads, self.width)
             out = s._outs(shape, shape)
         try:
             if made and out[0].numel:  # padding rows of a fresh output
                 for t in out:
                     call("stb_fill_value", s.handle, t.address, STB_F32, t.numel, 0.0)
-            (kr, kh), (vr, vh) = (self._rows(t, rows, heads_first) for t in out)
-            call("stb_op_paged_read", s.handle, self.ref, tables.address, batch, blocks, seq, pos, rows, out[0].address, kr,
-                 kh, out[1].address, vr, vh)
+            k, v = out
+            kr, vr = self._rows(k, shape), self._rows(v, shape)
+            kh = vh = w
+            if heads_first:
+                kr, kh, vr, vh = w, kr, w, vr
+            call("stb_op_paged_read", s.handle, self.ref, tables.address, batch, blocks, sequences.address, positions.address, rows,
+                 k.address, kr, kh, v.address, vr, vh)
         except Exception:
             if made:
                 s.release(out[0])
@@ -914,24 +946,21 @@ class B200PagedCache:
             raise
         return out
 
+    @_of_tensors
     def attend(self, query: DeviceTensor, tables: DeviceTensor, lengths: DeviceTensor,
                out: DeviceTensor | None = None) -> DeviceTensor:
         """Attention of one new token per request: query (batch, heads, width) against the first lengths[b] tokens of
         tables[b] (the new token's own key among them: append first).  A length of zero gives a row of zeros."""
-        batch, blocks = self._tables(tables)
-        s = self.session
-        q_row = s._rows_of(query)
-        shape = query.shape
-        if len(shape) != 3 or shape[0] != batch or shape[2] != self.width or shape[1] % self.kv_heads or not shape[1]:
-            raise IllegalArgumentException("paged attention query must have shape (batch, heads, width)")
-        at = s._indices(lengths, (batch,))
+        self._open(tables, lengths)
+        s, shape = self.session, query.shape
+        batch, blocks = tables.shape
+        require(len(shape) == 3 and shape[0] == batch == lengths.shape[0] and shape[2] == self.width and shape[1] > 0
+                and shape[1] % self.kv_heads == 0, "paged attention query must have shape (batch, heads, width)")
+        q_row = self._rows(query, shape)
         y = s._out(shape) if out is None else out
-        y_row = s._rows_of(y)
-        if y.shape != shape:
-            raise IllegalArgumentException("output shape mismatch")
         try:
             call("stb_op_paged_attention", s.handle, self.ref, query.address, q_row, shape[1], tables.address, batch, blocks,
-                 at, y.address, y_row)
+                 lengths.address, y.address, self._rows(y, shape))
         except Exception:
             if out is None:
                 s.release(y)

@@ -97,6 +97,16 @@ def test_adapter_pool_refusals(s):
         s.linear_adapted(x, w, pool, rows, out=y)
 
 
+def test_operands_that_are_no_tensors(s):
+    a, i = np.zeros((3, 2, 64), np.float32), np.zeros(3, np.int32)
+    kv = t(s, (5, 2, 16, 64))
+    c, pool = s.paged_cache(kv, kv), s.adapter_pool(t(s, (3, 8, 32)), t(s, (3, 48, 8)), t(s, (3,), STB_I32), t(s, (3,)))
+    for bad in (lambda: s.qk_norm_rope(a, a, None, None, i, out=(a, a)), lambda: c.append(a, a, i[None], i, i), lambda: c.read(i[None], i, i, out=(a, a)),
+                lambda: c.attend(a, i[None], i, out=a), lambda: s.linear_adapted(a, a, pool, i), lambda: s.linear_adapted(a, a, None, i)):
+        with pytest.raises(ffm.IllegalArgumentException):
+            bad()
+
+
 def test_the_checkers_known_answers():
     assert E4M3[0x7E] == 448.0 and E4M3[1] == 2.0 ** -9 and E4M3[0x38] == 1.0 and np.isnan(E4M3[0x7F])
     q, e = quantise(np.array([[448.0, 1.0, 0.0, -17.0], [449.0, 1.0, 0.0, -17.0], [0.0, 0.0, 0.0, 0.0], [np.inf, 2.0, np.nan, -2.0]]))
