@@ -112,6 +112,7 @@ __global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedVie
 
 constexpr int MAX_GRID = 160;
 constexpr int DIRECT_TILES = 64;     // most tiles of an item that one block takes alone
+constexpr int WHOLE_TILES = 4;       // most tiles of an item that one warp takes alone
 constexpr int BLOCK_PIECES = 20800;  // floats of a block's pieces, at most: (2 + warps) of 8 heads x (width + 4)
 constexpr int MAX_BATCH = 1024;      // requests of one launch (their prefix sums lie in shared memory)
 constexpr float LAZY = 8.0f;         // a maximum moves only when a score passes it by 2^8
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
   uint8_t *s_meta = smem + S::RING;
   int *s_start = (int *)(s_meta + S::WARPS * S::STAGES * S::META);  // tiles before request b, of one item each
   int *s_len = s_start + MAX_BATCH + 1;
-  __shared__ int s_scan[S::WARPS];
+  __shared__ int s_scan[S::WARPS], s_most[S::WARPS];
   __shared__ int s_part[2 * S::WARPS][4];  // a warp's first and last part: request (or -1), item, whether it starts / ends it
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -261,20 +262,40 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
   if (c.width != WP)  // chunks behind the row are read as zeros and never written
     for (int i = threadIdx.x; i < S::RING / 16; i += S::THREADS) ((uint4 *)smem)[i] = make_uint4(0, 0, 0, 0);
 
-  // Few short items: one block each, no line, nothing to join between blocks (`direct`).
-  bool direct = false;
-  if (a.batch * items <= (int)gridDim.x) {
-    bool deep = false;
-    for (int b = threadIdx.x; b < a.batch; b += S::THREADS) deep |= a.lengths[a.first + b] > DIRECT_TILES * TK;
-    direct = !__syncthreads_or(deep);
+  // The requests' lengths, the longest of them, and the sum of their tiles so far.
+  const int per = (a.batch + S::THREADS - 1) / S::THREADS, b0 = threadIdx.x * per, b1 = min(a.batch, b0 + per);
+  int own = 0, longest = 0;
+  for (int b = b0; b < b1; b++) {
+    const int n = attend_length(c, a, a.first + b);
+    s_len[b] = n;
+    own += (n + TK - 1) / TK;
+    longest = max(longest, n);
   }
+  int before = own;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, before, off);
+    if (lane >= off) before += v;
+  }
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (lane == 31) {
+    s_scan[warp] = before;
+    s_most[warp] = longest;
+  }
+  __syncthreads();
+  for (int w = 0; w < S::WARPS; w++) {
+    longest = max(longest, s_most[w]);
+    if (w < warp) before += s_scan[w];
+  }
+  // Few short items: one block each, no line, nothing to join between blocks.
+  const bool direct = a.batch * items <= (int)gridDim.x && longest <= DIRECT_TILES * TK;
   Cursor load, use;
   int total = 0, grid = 0, block0 = 0, t0, todo;
   if (direct) {
     if ((int)blockIdx.x >= a.batch * items) return;
     load.b = blockIdx.x / items;
     load.item = blockIdx.x % items;
-    load.n = attend_length(c, a, a.first + load.b);
+    load.n = s_len[load.b];
     load.tiles = (load.n + TK - 1) / TK;
     if (load.n == 0) {
       for (int h = load.item % chunks_of * 8; h < min(a.group, (load.item % chunks_of + 1) * 8); h++)
@@ -287,53 +308,55 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     todo = stretch_start(min(warp + 1, warps), load.tiles, warps) - t0;
     load.tile = t0;
   } else {
-    // Prefix sums of the requests' tiles, and zeros for the empty ones.
-    const int per = (a.batch + S::THREADS - 1) / S::THREADS, b0 = threadIdx.x * per, b1 = min(a.batch, b0 + per);
-    int own = 0;
-    for (int b = b0; b < b1; b++) {
-      const int n = attend_length(c, a, a.first + b);
-      s_len[b] = n;
-      own += (n + TK - 1) / TK;
-    }
-    int before = own;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, before, off);
-      if (lane >= off) before += v;
-    }
-    if (lane == 31) s_scan[warp] = before;
-    __syncthreads();
     before -= own;
-    for (int w = 0; w < warp; w++) before += s_scan[w];
     for (int b = b0; b < b1; b++) {
       s_start[b] = before;
       before += (s_len[b] + TK - 1) / TK;
       if (b == a.batch - 1) s_start[a.batch] = before;
     }
     __syncthreads();
-    for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
+    for (int b = blockIdx.x; b < a.batch; b += gridDim.x)  // zeros for the empty ones
       if (s_len[b] == 0)
         for (int i = threadIdx.x; i < a.heads * c.width; i += S::THREADS) a.y[(a.first + b) * a.y_row + i] = 0.0f;
 
     total = s_start[a.batch] * items;
-    grid = min((int)gridDim.x, (total + 2 * S::WARPS - 1) / (2 * S::WARPS));
+    const bool whole = longest <= WHOLE_TILES * TK;  // short items, many of them: no item is cut
+    grid = min((int)gridDim.x, whole ? (total + S::WARPS - 1) / S::WARPS : (total + 2 * S::WARPS - 1) / (2 * S::WARPS));
     if ((int)blockIdx.x >= grid) return;
     block0 = stretch_start(blockIdx.x, total, grid);
     const int mine = stretch_start(blockIdx.x + 1, total, grid) - block0;
     t0 = block0 + stretch_start(warp, mine, S::WARPS);
     todo = block0 + stretch_start(warp + 1, mine, S::WARPS) - t0;
-    int lo = 0, hi = a.batch - 1;  // the last request that starts at or before t0 (the empty ones before it share its start)
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (s_start[mid] * items <= t0) lo = mid;
-      else hi = mid - 1;
+    // The place of tile t: the last request that starts at or before it (the empty ones before that share its start).
+    auto locate = [&](int t) {
+      Cursor k;
+      int lo = 0, hi = a.batch - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_start[mid] * items <= t) lo = mid;
+        else hi = mid - 1;
+      }
+      k.b = lo;
+      k.tiles = s_start[lo + 1] - s_start[lo];
+      k.n = s_len[lo];
+      const int in = t - s_start[lo] * items;
+      k.item = k.tiles ? in / k.tiles : 0;
+      k.tile = k.tiles ? in - k.item * k.tiles : 0;
+      return k;
+    };
+    load = locate(t0);
+    if (whole) {  // both ends move to the next item's start
+      int end = t0 + todo;
+      if (end < total) {
+        const Cursor k = locate(end);
+        if (k.tile) end += k.tiles - k.tile;
+      }
+      if (load.tile) {
+        t0 += load.tiles - load.tile;
+        if (t0 < total) load = locate(t0);
+      }
+      todo = max(0, end - t0);
     }
-    load.b = lo;
-    load.tiles = s_start[lo + 1] - s_start[lo];
-    load.n = s_len[lo];
-    const int in = t0 - s_start[lo] * items;
-    load.item = load.tiles ? in / load.tiles : 0;
-    load.tile = load.tiles ? in % load.tiles : 0;
   }
   use = load;
 
@@ -778,10 +801,9 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     v.z = fmaf(x.z, f, v.z);
     v.w = fmaf(x.w, f, v.w);
   };
-  auto most = [](float x) {
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-    return x;
+  auto most = [](float x) {  // over the warp, by the order of the bits
+    const int i = __float_as_int(x), key = i ^ (i >> 31 & 0x7fffffff), top = __reduce_max_sync(0xffffffffu, key);
+    return __int_as_float(top ^ (top >> 31 & 0x7fffffff));
   };
   auto total_of = [](float x) {
 #pragma unroll
@@ -808,17 +830,29 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       const int row = h * (WP + 4);
       const bool has = which >> lane & 1;
       float4 part = has ? *(const float4 *)(mine_at + row) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      float n1 = most(part.z != 0.0f ? part.x : -INFINITY), n2 = most(part.z != 0.0f ? part.y : -INFINITY);
+      float n1 = most(part.z != 0.0f ? part.x : -INFINITY), n2 = SCALED ? most(part.z != 0.0f ? part.y : -INFINITY) : n1;
       float all = total_of(part.z != 0.0f ? part.z * exp2f(part.x - n1) : 0.0f);
       const float factor = part.z != 0.0f ? exp2f(part.y - n2) : 0.0f;
       float4 v[WIDE] = {};
-      for (uint32_t m = which; m; m &= m - 1) {
-        const int i = __ffs(m) - 1;
-        const float f = __shfl_sync(0xffffffffu, factor, i);
-        const float *at = i & 1 ? (const float *)(smem + (i >> 1) * S::STAGES * S::TILE) : block_pieces + (2 + (i >> 1)) * S::PART;
+      for (uint32_t m = which; m;) {  // four parts on their way at a time
+        float4 x[4][WIDE];
+        float f[4];
 #pragma unroll
-        for (int k = 0; k < WIDE; k++)
-          if (k * 128 + lane * 4 < WP) add(v[k], *(const float4 *)(at + row + 4 + k * 128 + lane * 4), f);
+        for (int j = 0; j < 4; j++) {
+          const int i = __ffs(m) - 1;
+          m &= m - 1;
+          f[j] = __shfl_sync(0xffffffffu, factor, i & 31);
+          if (i < 0) f[j] = 0.0f;
+          const float *at = i & 1 ? (const float *)(smem + (i >> 1) * S::STAGES * S::TILE) : block_pieces + (2 + (i >> 1)) * S::PART;
+#pragma unroll
+          for (int k = 0; k < WIDE; k++)
+            if (i >= 0 && k * 128 + lane * 4 < WP) x[j][k] = *(const float4 *)(at + row + 4 + k * 128 + lane * 4);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int k = 0; k < WIDE; k++)
+            if (k * 128 + lane * 4 < WP) add(v[k], x[j][k], f[j]);
       }
       if (whole) {
 #pragma unroll
@@ -830,15 +864,16 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
 #pragma unroll
       for (int k = 0; k < WIDE; k++)
         if (k * 128 + lane * 4 < WP) *(float4 *)(piece + row + 4 + k * 128 + lane * 4) = v[k];
-      __threadfence();
       __syncwarp();
       int last = 0;
       if (lane == 0) {  // the head's counter of the item's first block; the last block to arrive joins, and clears it
+        __threadfence();
         last = atomicAdd(a.arrived + c0 * 8 + h, 1) == c1 - c0;
         if (last) a.arrived[c0 * 8 + h] = 0;
+        __threadfence();
       }
       if (!__shfl_sync(0xffffffffu, last, 0)) continue;
-      __threadfence();
+      __syncwarp();
       const int count = c1 - c0 + 1;
       auto piece_of = [&](int k) {
         return a.pieces + (size_t)(c0 + k) * BLOCK_PIECES + (stretch_start(c0 + k, total, grid) >= first ? 0 : 1) * S::PART + row;
@@ -857,7 +892,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
           n2 = fmaxf(n2, far[k].y);
         }
       n1 = most(n1);
-      n2 = most(n2);
+      n2 = SCALED ? most(n2) : n1;
       all = 0.0f;
 #pragma unroll
       for (int k = 0; k < FAR; k++) {
@@ -869,7 +904,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       for (int k = 0; k < WIDE; k++) v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int r = 0; r < FAR; r++)
-#pragma unroll 8
+#pragma unroll 16
         for (int i = 0; i < min(32, count - r * 32); i++) {
           const float f = __shfl_sync(0xffffffffu, far[r].w, i);
           const float *at = piece_of(r * 32 + i) + 4;
