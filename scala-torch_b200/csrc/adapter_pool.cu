@@ -407,14 +407,21 @@ __global__ void __launch_bounds__(256, DTYPE == STB_F32 ? 1 : 2) pool_up_kernel(
       if (g + 8 * h >= count) continue;
       const int r = s_plan.rows[e][g + 8 * h];
       if (PIECES) {
-#pragma unroll 4
-        for (int i = 0; i < pieces; i++)
+        for (int i = 0; i < pieces; i += 4) {  // four on their way at a time
+          float2 v[4][NT];
 #pragma unroll
-          for (int n = 0; n < NT; n++) {
-            const float2 v = __ldcg((const float2 *)(at_piece + ((size_t)i * parts.M + r) * 128 + n * 8));
-            base[h][n].x += v.x;
-            base[h][n].y += v.y;
-          }
+          for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+              v[k][n] = i + k < pieces ? __ldcg((const float2 *)(at_piece + ((size_t)(i + k) * parts.M + r) * 128 + n * 8)) : make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+              base[h][n].x += v[k][n].x;
+              base[h][n].y += v[k][n].y;
+            }
+        }
       } else {
 #pragma unroll
         for (int n = 0; n < NT; n++) {

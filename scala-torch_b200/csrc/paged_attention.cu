@@ -121,13 +121,15 @@ constexpr float P_SHIFT = 7.0f, P_SCALE = 128.0f;  // F16 weights times 2^7: at 
 template <int DTYPE, int WP>
 struct Shape {
   static constexpr int ESZ = DTYPE == STB_F32 ? 4 : (DTYPE == STB_E4M3 ? 1 : 2);
-  static constexpr int ROW = WP * ESZ;            // bytes of a key's row in shared memory
+  static constexpr int ROW = (WP == 96 ? 128 : WP) * ESZ;  // bytes of a key's row in shared memory
   static constexpr int CHUNKS = ROW / 16;
+  static constexpr int PAIRS = WP * ESZ / 32;     // pairs of them that the products take
   static constexpr int TK = ROW >= 256 ? 16 : 32; // keys of a tile: 8 KB where the width allows
   static constexpr int TILE = 2 * TK * ROW;       // keys and values of a tile
   // Warps and stages that fill about 192 KB: at least two stages in flight per warp, 128 KB per SM.
-  // E4M3 has the most arithmetic per byte: twelve warps of two stages (three warps per scheduler to fill).
-  static constexpr int WARPS = TILE <= 8192 ? (DTYPE == STB_E4M3 && WP == 128 ? 12 : 8) : (TILE <= 16384 ? 4 : 2);
+  // E4M3 has the most arithmetic per byte: twelve warps of two stages (three warps per scheduler to fill); the 16 KB tiles
+  // of wide rows leave six.
+  static constexpr int WARPS = TILE <= 8192 ? (DTYPE == STB_E4M3 && ROW == 128 ? 12 : 8) : (TILE <= 16384 ? 6 : 3);
   static constexpr int STAGES = 196608 / (WARPS * TILE) < 6 ? 196608 / (WARPS * TILE) : 6;
   static constexpr int META = 16 + (DTYPE == STB_E4M3 ? TK * 8 : 0);  // per stage: valid mask, scales of keys and values
   static constexpr int THREADS = WARPS * 32;
@@ -259,8 +261,13 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
   const int row_chunks = c.width * S::ESZ / 16, row_bytes = row_chunks * 16;
 
   for (int i = threadIdx.x; i < 2 * S::WARPS; i += S::THREADS) s_part[i][0] = -1;
-  if (c.width != WP)  // chunks behind the row are read as zeros and never written
-    for (int i = threadIdx.x; i < S::RING / 16; i += S::THREADS) ((uint4 *)smem)[i] = make_uint4(0, 0, 0, 0);
+  if (row_chunks < 2 * S::PAIRS) {  // chunks behind a key's row meet zeros of q: they must not hold NaNs (a value's go nowhere)
+    const int behind = 2 * S::PAIRS - row_chunks;
+    for (int i = threadIdx.x; i < S::WARPS * S::STAGES * TK * behind; i += S::THREADS) {
+      const int row = i / behind;
+      *(uint4 *)(smem + row / TK * S::TILE + chunk_at<S::ROW>(0, row % TK, row_chunks + i % behind)) = make_uint4(0, 0, 0, 0);
+    }
+  }
 
   // The requests' lengths, the longest of them, and the sum of their tiles so far.
   const int per = (a.batch + S::THREADS - 1) / S::THREADS, b0 = threadIdx.x * per, b1 = min(a.batch, b0 + per);
@@ -593,7 +600,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     {
       const int row = (lane & 7) + ((lane >> 3) & 1) * 8, odd = lane >> 4;
 #pragma unroll
-      for (int s = 0; s < S::CHUNKS / 2; s++)
+      for (int s = 0; s < S::PAIRS; s++)
 #pragma unroll
         for (int b = 0; b < MB; b++) {
           uint32_t r[4];
@@ -739,7 +746,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
         }
       const int row = (lane & 7) + (lane >> 4) * 8, odd = (lane >> 3) & 1;
 #pragma unroll
-      for (int s = 0; s < S::CHUNKS / 2; s++) {
+      for (int s = 0; s < S::PAIRS; s++) {
         constexpr int PAIR = SCALED ? 2 : 1;  // 16-dimension results of two chunks
         float r[PAIR][4] = {};
 #pragma unroll
@@ -814,26 +821,32 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
   const int mine_b = lane < 2 * S::WARPS ? s_part[lane][0] : -1, mine_item = lane < 2 * S::WARPS ? s_part[lane][1] : -1;
   // the part of entry `lane`
   const float *const mine_at = lane & 1 ? (const float *)(smem + (lane >> 1) * S::STAGES * S::TILE) : block_pieces + (2 + (lane >> 1)) * S::PART;
-  uint32_t left = __ballot_sync(0xffffffffu, mine_b >= 0);
+  const uint32_t entries = __ballot_sync(0xffffffffu, mine_b >= 0);
+  const int share = total / max(grid, 1), more = total % max(grid, 1);  // block k's stretch starts at k share + min(k, more)
 #pragma unroll 1
-  while (left) {
-    const int i0 = __ffs(left) - 1;
-    const int b = __shfl_sync(0xffffffffu, mine_b, i0), item = __shfl_sync(0xffffffffu, mine_item, i0);
-    const uint32_t which = __ballot_sync(0xffffffffu, mine_b == b && mine_item == item);
-    left &= ~which;
-    const bool whole = s_part[i0][2] && s_part[31 - __clz(which)][3];
-    const int tiles = whole ? 0 : s_start[b + 1] - s_start[b], first = whole ? 0 : s_start[b] * items + item * tiles;
-    float *piece = block_pieces + (block0 >= first ? 0 : 1) * S::PART;
-    const int c0 = whole ? 0 : stretch_of(first, total, grid), c1 = whole ? 0 : stretch_of(first + tiles - 1, total, grid);
+  for (int h = warp; h < 8; h += S::WARPS) {
+    const int row = h * (WP + 4);
+    float4 v[WIDE];
+    float n1, n2, all;
+    // First every item's parts of this block: to y, or to a piece of the block's (an item at either end of its stretch).
+    struct Split {
+      int b, item, first, c0, c1;
+    } splits[2];
+    int cut = 0;
 #pragma unroll 1
-    for (int h = warp; h < 8; h += S::WARPS) {
-      const int row = h * (WP + 4);
+    for (uint32_t left = entries; left;) {
+      const int i0 = __ffs(left) - 1;
+      const int b = __shfl_sync(0xffffffffu, mine_b, i0), item = __shfl_sync(0xffffffffu, mine_item, i0);
+      const uint32_t which = __ballot_sync(0xffffffffu, mine_b == b && mine_item == item);
+      left &= ~which;
       const bool has = which >> lane & 1;
-      float4 part = has ? *(const float4 *)(mine_at + row) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      float n1 = most(part.z != 0.0f ? part.x : -INFINITY), n2 = SCALED ? most(part.z != 0.0f ? part.y : -INFINITY) : n1;
-      float all = total_of(part.z != 0.0f ? part.z * exp2f(part.x - n1) : 0.0f);
+      const float4 part = has ? *(const float4 *)(mine_at + row) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      n1 = most(part.z != 0.0f ? part.x : -INFINITY);
+      n2 = SCALED ? most(part.z != 0.0f ? part.y : -INFINITY) : n1;
+      all = total_of(part.z != 0.0f ? part.z * exp2f(part.x - n1) : 0.0f);
       const float factor = part.z != 0.0f ? exp2f(part.y - n2) : 0.0f;
-      float4 v[WIDE] = {};
+#pragma unroll
+      for (int k = 0; k < WIDE; k++) v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       for (uint32_t m = which; m;) {  // four parts on their way at a time
         float4 x[4][WIDE];
         float f[4];
@@ -854,29 +867,48 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
           for (int k = 0; k < WIDE; k++)
             if (k * 128 + lane * 4 < WP) add(v[k], x[j][k], f[j]);
       }
-      if (whole) {
+      if (s_part[i0][2] && s_part[31 - __clz(which)][3]) {  // from its start to its end
 #pragma unroll
         for (int k = 0; k < WIDE; k++)
           if (k * 128 + lane * 4 < WP) write(b, item, h, k * 128 + lane * 4, v[k], n1, n2, all);
         continue;
       }
+      const int tiles = s_start[b + 1] - s_start[b], first = s_start[b] * items + item * tiles;
+      float *piece = block_pieces + (block0 >= first ? 0 : 1) * S::PART;
       if (lane == 0) *(float4 *)(piece + row) = make_float4(n1, n2, all, 0.0f);
 #pragma unroll
       for (int k = 0; k < WIDE; k++)
         if (k * 128 + lane * 4 < WP) *(float4 *)(piece + row + 4 + k * 128 + lane * 4) = v[k];
-      __syncwarp();
-      int last = 0;
-      if (lane == 0) {  // the head's counter of the item's first block; the last block to arrive joins, and clears it
-        __threadfence();
-        last = atomicAdd(a.arrived + c0 * 8 + h, 1) == c1 - c0;
-        if (last) a.arrived[c0 * 8 + h] = 0;
-        __threadfence();
-      }
-      if (!__shfl_sync(0xffffffffu, last, 0)) continue;
-      __syncwarp();
-      const int count = c1 - c0 + 1;
+      Split &to = splits[cut ? 1 : 0];
+      to.b = b;
+      to.item = item;
+      to.first = first;
+      to.c0 = stretch_of(first, total, grid);
+      to.c1 = stretch_of(first + tiles - 1, total, grid);
+      cut++;
+    }
+    if (!cut) continue;
+    // Then both pieces are announced, on the counter of the head and of the item's first block; the last block to arrive
+    // joins them, in the blocks' order, and clears the counter.
+    int last = 0;
+    __syncwarp();
+    if (lane == 0) __threadfence();
+    __syncwarp();
+    if (lane < cut) {
+      const Split &of = lane ? splits[1] : splits[0];
+      last = atomicAdd(a.arrived + of.c0 * 8 + h, 1) == of.c1 - of.c0;
+      if (last) a.arrived[of.c0 * 8 + h] = 0;
+      __threadfence();
+    }
+    const uint32_t to_join = __ballot_sync(0xffffffffu, last);
+#pragma unroll 1
+    for (int n = 0; n < 2; n++) {
+      if (!(to_join >> n & 1)) continue;
+      const Split &of = n ? splits[1] : splits[0];
+      const int count = of.c1 - of.c0 + 1;
       auto piece_of = [&](int k) {
-        return a.pieces + (size_t)(c0 + k) * BLOCK_PIECES + (stretch_start(c0 + k, total, grid) >= first ? 0 : 1) * S::PART + row;
+        const int start = (of.c0 + k) * share + min(of.c0 + k, more);
+        return a.pieces + (size_t)(of.c0 + k) * BLOCK_PIECES + (start >= of.first ? 0 : 1) * S::PART + row;
       };
       float4 far[FAR];
       n1 = n2 = -INFINITY;
@@ -904,17 +936,27 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       for (int k = 0; k < WIDE; k++) v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int r = 0; r < FAR; r++)
-#pragma unroll 16
-        for (int i = 0; i < min(32, count - r * 32); i++) {
-          const float f = __shfl_sync(0xffffffffu, far[r].w, i);
-          const float *at = piece_of(r * 32 + i) + 4;
+#pragma unroll 1
+        for (int i0 = r * 32; i0 < min(r * 32 + 32, count); i0 += 8) {  // eight pieces on their way at a time
+          float4 x[8][WIDE];
 #pragma unroll
-          for (int k = 0; k < WIDE; k++)
-            if (k * 128 + lane * 4 < WP) add(v[k], __ldcg((const float4 *)(at + k * 128 + lane * 4)), f);
+          for (int j = 0; j < 8; j++) {
+            const float *at = piece_of(min(i0 + j, count - 1)) + 4;
+#pragma unroll
+            for (int k = 0; k < WIDE; k++)
+              if (k * 128 + lane * 4 < WP) x[j][k] = __ldcg((const float4 *)(at + k * 128 + lane * 4));
+          }
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            const float f = __shfl_sync(0xffffffffu, far[r].w, (i0 + j) & 31);
+#pragma unroll
+            for (int k = 0; k < WIDE; k++)
+              if (k * 128 + lane * 4 < WP) add(v[k], x[j][k], i0 + j < count ? f : 0.0f);
+          }
         }
 #pragma unroll
       for (int k = 0; k < WIDE; k++)
-        if (k * 128 + lane * 4 < WP) write(b, item, h, k * 128 + lane * 4, v[k], n1, n2, all);
+        if (k * 128 + lane * 4 < WP) write(of.b, of.item, h, k * 128 + lane * 4, v[k], n1, n2, all);
     }
   }
 }
@@ -995,6 +1037,7 @@ extern "C" int stb_op_paged_attention(stb_session *s, const stb_paged_cache *cac
     dispatch_paged(cache->dtype, [&](auto t) {
       constexpr int DT = decltype(t)::value;
       if (c.width <= 64) launch_attention<DT, 64>(s, c, a, batch, at_once);
+      else if (c.width <= 96) launch_attention<DT, 96>(s, c, a, batch, at_once);
       else if (c.width <= 128) launch_attention<DT, 128>(s, c, a, batch, at_once);
       else launch_attention<DT, 256>(s, c, a, batch, at_once);
     });
