@@ -235,6 +235,12 @@ __device__ __forceinline__ int stretch_of(int i, int total, int parts) {
   const int q = total / parts, r = total % parts;
   return i < r * (q + 1) ? i / (q + 1) : r + (i - r * (q + 1)) / q;
 }
+// The blocks' stretches: the whole line's tiles, or each item's, cut among `blocks` of them.
+struct Line {
+  int tiles, blocks;
+  __device__ __forceinline__ int start(int k) const { return k / blocks * tiles + stretch_start(k % blocks, tiles, blocks); }
+  __device__ __forceinline__ int of(int i) const { return i / tiles * blocks + stretch_of(i % tiles, tiles, blocks); }
+};
 
 // A place on the line of tiles.
 struct Cursor {
@@ -298,6 +304,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
   const bool direct = a.batch * items <= (int)gridDim.x && longest <= DIRECT_TILES * TK;
   Cursor load, use;
   int total = 0, grid = 0, block0 = 0, t0, todo;
+  Line line = {1, 1};
   if (direct) {
     if ((int)blockIdx.x >= a.batch * items) return;
     load.b = blockIdx.x / items;
@@ -329,9 +336,15 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     total = s_start[a.batch] * items;
     const bool whole = longest <= WHOLE_TILES * TK;  // short items, many of them: no item is cut
     grid = min((int)gridDim.x, whole ? (total + S::WARPS - 1) / S::WARPS : (total + 2 * S::WARPS - 1) / (2 * S::WARPS));
+    line = {total, grid};
+    // One request: the same number of blocks for each of its items, if that idles few (no block then joins twice).
+    if (a.batch == 1 && grid % items <= grid / 16) {
+      grid -= grid % items;
+      line = {total / items, grid / items};
+    }
     if ((int)blockIdx.x >= grid) return;
-    block0 = stretch_start(blockIdx.x, total, grid);
-    const int mine = stretch_start(blockIdx.x + 1, total, grid) - block0;
+    block0 = line.start(blockIdx.x);
+    const int mine = line.start(blockIdx.x + 1) - block0;
     t0 = block0 + stretch_start(warp, mine, S::WARPS);
     todo = block0 + stretch_start(warp + 1, mine, S::WARPS) - t0;
     // The place of tile t: the last request that starts at or before it (the empty ones before that share its start).
@@ -535,29 +548,27 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     for (int j = 0; j < 2; j++)
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], off);
+    const bool whole = starts && ends;
     float *part = ends ? block_pieces + (2 + warp) * S::PART : my_ring;
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       const int in_chunk = 2 * t + j, head = (use.item % chunks_of) * 8 + in_chunk;
-      if (starts && ends) {
-        if (head >= a.group) continue;
-        float *y = a.y + (a.first + use.b) * a.y_row + (size_t)(use.item / chunks_of * a.group + head) * c.width;
-        const float f = (HALF ? 1.0f / P_SCALE : 1.0f) * (SCALED ? exp2f(m2[j] - m1[j]) : 1.0f) / sum[j];
-#pragma unroll
-        for (int i = 0; i < NT; i++)
-#pragma unroll
-          for (int k = 0; k < 2; k++)
-            if (dim_of(i, k) < c.width) y[dim_of(i, k)] = sum[j] != 0.0f ? o[i][j + 2 * k] * f : 0.0f;
-        continue;
+      float *to = part + in_chunk * (WP + 4) + 4, f = 1.0f;
+      int most = WP;
+      if (whole) {
+        to = a.y + (a.first + use.b) * a.y_row + (size_t)(use.item / chunks_of * a.group + head) * c.width;
+        f = (HALF ? 1.0f / P_SCALE : 1.0f) * (SCALED ? exp2f(m2[j] - m1[j]) : 1.0f) / sum[j];
+        most = head < a.group ? c.width : 0;
+      } else if (g == 0) {
+        *(float4 *)(to - 4) = make_float4(m1[j], m2[j], sum[j], 0.0f);
       }
-      float *p = part + in_chunk * (WP + 4);
-      if (g == 0) *(float4 *)p = make_float4(m1[j], m2[j], sum[j], 0.0f);
 #pragma unroll
       for (int i = 0; i < NT; i++)
 #pragma unroll
-        for (int k = 0; k < 2; k++) p[4 + dim_of(i, k)] = o[i][j + 2 * k];
+        for (int k = 0; k < 2; k++)
+          if (dim_of(i, k) < most) to[dim_of(i, k)] = sum[j] != 0.0f ? o[i][j + 2 * k] * f : 0.0f;
     }
-    if (starts && ends) return;
+    if (whole) return;
     if (lane == 0) {
       int *p = s_part[2 * warp + (ends ? 0 : 1)];
       p[0] = use.b;
@@ -822,17 +833,18 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
   // the part of entry `lane`
   const float *const mine_at = lane & 1 ? (const float *)(smem + (lane >> 1) * S::STAGES * S::TILE) : block_pieces + (2 + (lane >> 1)) * S::PART;
   const uint32_t entries = __ballot_sync(0xffffffffu, mine_b >= 0);
-  const int share = total / max(grid, 1), more = total % max(grid, 1);  // block k's stretch starts at k share + min(k, more)
+  // First, head by head, every item's parts of this block: to y, or to a piece of the block's (an item at either end of its
+  // stretch).
+  struct Split {
+    int b, item, first, c0, c1;
+  } splits[2];
+  int cut = 0;
+  float4 v[WIDE];
 #pragma unroll 1
   for (int h = warp; h < 8; h += S::WARPS) {
     const int row = h * (WP + 4);
-    float4 v[WIDE];
     float n1, n2, all;
-    // First every item's parts of this block: to y, or to a piece of the block's (an item at either end of its stretch).
-    struct Split {
-      int b, item, first, c0, c1;
-    } splits[2];
-    int cut = 0;
+    cut = 0;
 #pragma unroll 1
     for (uint32_t left = entries; left;) {
       const int i0 = __ffs(left) - 1;
@@ -883,81 +895,86 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       to.b = b;
       to.item = item;
       to.first = first;
-      to.c0 = stretch_of(first, total, grid);
-      to.c1 = stretch_of(first + tiles - 1, total, grid);
+      to.c0 = line.of(first);
+      to.c1 = line.of(first + tiles - 1);
       cut++;
     }
-    if (!cut) continue;
-    // Then both pieces are announced, on the counter of the head and of the item's first block; the last block to arrive
-    // joins them, in the blocks' order, and clears the counter.
-    int last = 0;
-    __syncwarp();
-    if (lane == 0) __threadfence();
-    __syncwarp();
-    if (lane < cut) {
-      const Split &of = lane ? splits[1] : splits[0];
-      last = atomicAdd(a.arrived + of.c0 * 8 + h, 1) == of.c1 - of.c0;
-      if (last) a.arrived[of.c0 * 8 + h] = 0;
-      __threadfence();
-    }
-    const uint32_t to_join = __ballot_sync(0xffffffffu, last);
+  }
+  if (!cut) return;
+  // Then the warp's pieces are announced, each on the counter of its head and of its item's first block; the last block to
+  // arrive joins them, in the blocks' order, and clears the counter.
+  __syncwarp();
+  __threadfence();
+  int last = 0;
+  if ((lane & 1) < cut && warp + (lane >> 1) * S::WARPS < 8) {
+    const Split &of = lane & 1 ? splits[1] : splits[0];
+    int *const counter = a.arrived + of.c0 * 8 + warp + (lane >> 1) * S::WARPS;
+    last = atomicAdd(counter, 1) == of.c1 - of.c0;
+    if (last) *counter = 0;
+  }
+  __syncwarp();
+  __threadfence();
 #pragma unroll 1
-    for (int n = 0; n < 2; n++) {
-      if (!(to_join >> n & 1)) continue;
-      const Split &of = n ? splits[1] : splits[0];
-      const int count = of.c1 - of.c0 + 1;
-      auto piece_of = [&](int k) {
-        const int start = (of.c0 + k) * share + min(of.c0 + k, more);
-        return a.pieces + (size_t)(of.c0 + k) * BLOCK_PIECES + (start >= of.first ? 0 : 1) * S::PART + row;
-      };
-      float4 far[FAR];
-      n1 = n2 = -INFINITY;
+  for (uint32_t to_join = __ballot_sync(0xffffffffu, last); to_join; to_join &= to_join - 1) {
+    const int n = __ffs(to_join) - 1, h = warp + (n >> 1) * S::WARPS, row = h * (WP + 4);
+    const Split &of = n & 1 ? splits[1] : splits[0];
+    const int count = of.c1 - of.c0 + 1;
+    // A lane per piece: where it lies, its maxima and sum.  This code runs once and cold: what counts is that it is short.
+    float4 far[FAR];
+    int at[FAR];
+    float n1 = -INFINITY, n2 = -INFINITY, all = 0.0f;
 #pragma unroll
-      for (int k = 0; k < FAR; k++) {
-        far[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (k * 32 + lane < count) far[k] = __ldcg((const float4 *)piece_of(k * 32 + lane));
+    for (int r = 0; r < FAR; r++) {
+      const int k = of.c0 + min(r * 32 + lane, count - 1);
+      at[r] = (k * (BLOCK_PIECES / 4) + (line.start(k) >= of.first ? 0 : S::PART / 4)) + row / 4;
+      far[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (r * 32 < count) {
+        if (r * 32 + lane < count) far[r] = __ldcg((const float4 *)a.pieces + at[r]);
+        if (far[r].z != 0.0f) {
+          n1 = fmaxf(n1, far[r].x);
+          n2 = fmaxf(n2, far[r].y);
+        }
+      }
+    }
+    n1 = most(n1);
+    n2 = SCALED ? most(n2) : n1;
+#pragma unroll
+    for (int r = 0; r < FAR; r++)
+      if (r * 32 < count) {
+        if (far[r].z != 0.0f) all += far[r].z * exp2f(far[r].x - n1);
+        far[r].w = far[r].z != 0.0f ? exp2f(far[r].y - n2) : 0.0f;
+      }
+    all = total_of(all);
+#pragma unroll
+    for (int k = 0; k < WIDE; k++) v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    int place = at[0];
+    float factor = far[0].w;
+#pragma unroll 1
+    for (int i0 = 0; i0 < count; i0 += 8) {  // eight pieces on their way at a time
+      if (i0 > 0 && (i0 & 31) == 0) {
+#pragma unroll
+        for (int r = 1; r < FAR; r++)
+          if (i0 == r * 32) place = at[r], factor = far[r].w;
+      }
+      float4 x[8][WIDE];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {  // the last piece again behind the last
+        const float4 *from = (const float4 *)a.pieces + __shfl_sync(0xffffffffu, place, (i0 + j) & 31) + 1 + lane;
+#pragma unroll
+        for (int k = 0; k < WIDE; k++)
+          if (k * 128 + lane * 4 < WP) x[j][k] = __ldcg(from + k * 32);
       }
 #pragma unroll
-      for (int k = 0; k < FAR; k++)
-        if (far[k].z != 0.0f) {
-          n1 = fmaxf(n1, far[k].x);
-          n2 = fmaxf(n2, far[k].y);
-        }
-      n1 = most(n1);
-      n2 = SCALED ? most(n2) : n1;
-      all = 0.0f;
+      for (int j = 0; j < 8; j++) {
+        const float f = __shfl_sync(0xffffffffu, factor, (i0 + j) & 31);
 #pragma unroll
-      for (int k = 0; k < FAR; k++) {
-        if (far[k].z != 0.0f) all += far[k].z * exp2f(far[k].x - n1);
-        far[k].w = far[k].z != 0.0f ? exp2f(far[k].y - n2) : 0.0f;
+        for (int k = 0; k < WIDE; k++)
+          if (k * 128 + lane * 4 < WP) add(v[k], x[j][k], f);
       }
-      all = total_of(all);
-#pragma unroll
-      for (int k = 0; k < WIDE; k++) v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (int r = 0; r < FAR; r++)
-#pragma unroll 1
-        for (int i0 = r * 32; i0 < min(r * 32 + 32, count); i0 += 8) {  // eight pieces on their way at a time
-          float4 x[8][WIDE];
-#pragma unroll
-          for (int j = 0; j < 8; j++) {
-            const float *at = piece_of(min(i0 + j, count - 1)) + 4;
-#pragma unroll
-            for (int k = 0; k < WIDE; k++)
-              if (k * 128 + lane * 4 < WP) x[j][k] = __ldcg((const float4 *)(at + k * 128 + lane * 4));
-          }
-#pragma unroll
-          for (int j = 0; j < 8; j++) {
-            const float f = __shfl_sync(0xffffffffu, far[r].w, (i0 + j) & 31);
-#pragma unroll
-            for (int k = 0; k < WIDE; k++)
-              if (k * 128 + lane * 4 < WP) add(v[k], x[j][k], i0 + j < count ? f : 0.0f);
-          }
-        }
-#pragma unroll
-      for (int k = 0; k < WIDE; k++)
-        if (k * 128 + lane * 4 < WP) write(of.b, of.item, h, k * 128 + lane * 4, v[k], n1, n2, all);
     }
+#pragma unroll
+    for (int k = 0; k < WIDE; k++)
+      if (k * 128 + lane * 4 < WP) write(of.b, of.item, h, k * 128 + lane * 4, v[k], n1, n2, all);
   }
 }
 
