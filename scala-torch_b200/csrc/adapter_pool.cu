@@ -42,79 +42,95 @@ constexpr int WINDOW = 64;         // rows of one launch
 
 // The launch's rows by slot: groups of up to 16 rows that name the same slot (or none).
 struct Plan {
-  int slots[WINDOW];   // per row: -1 without a slot, -2 behind the last row
-  short ranks[WINDOW * 2];  // of a small pool's slots, clamped
-  uint32_t starts[2];  // rows that start a group
-  int groups;
-  int slot[WINDOW];                     // per group
+  int groups, widest;  // of them; most rows of one with a slot
+  int slot[WINDOW];    // per group: -1 without a slot
   short rank[WINDOW], count[WINDOW], first[WINDOW];
   signed char rows[WINDOW][16];
   // (group, chunk of 32 ranks) pairs, and into how many parts each one's columns are split: as many as give every block
   // of the first kernel one (both kernels plan alike).
-  int chunks[2], pairs, parts, per;  // per: stretches of 512 columns in a part
+  int pairs, parts, per;  // per: stretches of 512 columns in a part
   signed char group_of[WINDOW * (MAX_RANK / DOWN_RANKS)];
 };
 
-// A thread per row compares its slot with the others'.  Ends with a barrier.
+// By the first warp alone, lane i for rows i and i + 32, in registers; short code that runs cold.  Ends with a barrier.
 __device__ __forceinline__ void make_plan(const Pool &p, int M, int stretches, int blocks, Plan &s) {
-  const int i = threadIdx.x;
-  const bool small = p.slots <= WINDOW * 2;  // all ranks at once, beside the rows rather than behind them
-  if (small && i < p.slots) s.ranks[i] = (short)max(0, min(p.ranks[i], p.max_rank));
-  if (i < WINDOW) {
-    int t = -2;
-    if (i < M) {
-      t = p.rows[i];
-      if (t >= p.slots) *p.err = DEV_BAD_INDEX + 2;
-      if (t < 0 || t >= p.slots) t = -1;
-    }
-    s.slots[i] = t;
-  }
-  __syncthreads();
-  uint64_t same = 0;
-  int t = -2, at = 0, rank = 0;
-  if (i < WINDOW) {
-    t = s.slots[i];
-    if (t >= 0) rank = small ? s.ranks[t] : max(0, min(p.ranks[t], p.max_rank));
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    const uint32_t below = (1u << lane) - 1;
+    int known[4];  // a small pool's ranks, on their way beside the rows' slots rather than behind them
+    const bool small = p.slots <= 128;
 #pragma unroll
-    for (int k = 0; k < WINDOW; k++) same |= (uint64_t)(s.slots[k] == t) << k;
-    at = __popcll(same & ((1ull << i) - 1));  // its place in the slot's rows
-    const uint32_t starts = __ballot_sync(0xffffffffu, t != -2 && at % 16 == 0);
-    if ((i & 31) == 0) s.starts[i >> 5] = starts;
-  }
-  __syncthreads();
-  if (i < WINDOW && t != -2) {
-    const uint64_t starts = (uint64_t)s.starts[1] << 32 | s.starts[0];
-    uint64_t mine = same & starts;  // its group starts at the (at / 16)-th of these
-    for (int k = 0; k < at / 16; k++) mine &= mine - 1;
-    const int group = __popcll(starts & ((1ull << (__ffsll((long long)mine) - 1)) - 1));
-    s.rows[group][at % 16] = (signed char)i;
-    if (at % 16 == 0) {
-      s.slot[group] = t;
-      s.rank[group] = (short)rank;
-      s.count[group] = (short)min(16, __popcll(same) - at);
-    }
-    if (i == 0) s.groups = __popcll(starts);
-  }
-  __syncthreads();
-  int chunks = 0, before = 0;
-  if (i < WINDOW) {
-    if (i < s.groups && s.slot[i] >= 0) chunks = (s.rank[i] + DOWN_RANKS - 1) / DOWN_RANKS;
-    before = chunks;
+    for (int k = 0; k < 4; k++) known[k] = small && k * 32 + lane < p.slots ? p.ranks[k * 32 + lane] : 0;
+    int t[2];
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, before, off);
-      if ((i & 31) >= off) before += v;
+    for (int h = 0; h < 2; h++) {
+      t[h] = -2;  // behind the last row
+      if (h * 32 + lane < M) {
+        t[h] = p.rows[h * 32 + lane];
+        if (t[h] >= p.slots) *p.err = DEV_BAD_INDEX + 2;
+        if (t[h] < 0 || t[h] >= p.slots) t[h] = -1;
+      }
     }
-    if ((i & 31) == 31) s.chunks[i >> 5] = before;
-  }
-  __syncthreads();
-  if (i < WINDOW) {
-    before += (i >= 32 ? s.chunks[0] : 0) - chunks;
-    s.first[i] = (short)before;
-    for (int k = 0; k < chunks; k++) s.group_of[before + k] = (signed char)i;
-    if (i == 0) {
-      s.pairs = s.chunks[0] + s.chunks[1];
-      const int parts = max(1, min(stretches, blocks / max(1, s.pairs)));
+    uint64_t same[2] = {__match_any_sync(0xffffffffu, t[0]), (uint64_t)__match_any_sync(0xffffffffu, t[1]) << 32};
+    if (M > 32) {
+#pragma unroll 1
+      for (int k = 0; k < 32; k++) {
+        same[0] |= (uint64_t)(__shfl_sync(0xffffffffu, t[1], k) == t[0]) << (32 + k);
+        same[1] |= (uint64_t)(__shfl_sync(0xffffffffu, t[0], k) == t[1]) << k;
+      }
+    }
+    const int at[2] = {__popc((uint32_t)same[0] & below), __popcll(same[1] & ((1ull << (32 + lane)) - 1))};  // place among the slot's rows
+    const uint64_t starts = __ballot_sync(0xffffffffu, t[0] != -2 && at[0] % 16 == 0) |
+                            (uint64_t)__ballot_sync(0xffffffffu, t[1] != -2 && at[1] % 16 == 0) << 32;
+    int chunks[2] = {0, 0}, group[2], widest = 0;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      uint64_t mine = same[h] & starts;  // its group starts at the (at / 16)-th of these
+      for (int k = 0; k < at[h] / 16; k++) mine &= mine - 1;
+      const int start = t[h] == -2 ? 0 : __ffsll((long long)mine) - 1;
+      group[h] = __popcll(starts & ((1ull << start) - 1));
+      int rank = 0;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int r = __shfl_sync(0xffffffffu, known[k], t[h] & 31);
+        if (t[h] >= 0 && t[h] / 32 == k) rank = r;
+      }
+      if (!small && t[h] >= 0) rank = p.ranks[t[h]];
+      rank = max(0, min(rank, p.max_rank));
+      if (t[h] != -2) {
+        s.rows[group[h]][at[h] % 16] = (signed char)(h * 32 + lane);
+        if (at[h] % 16 == 0) {
+          const int count = min(16, __popcll(same[h]) - at[h]);
+          s.slot[group[h]] = t[h];
+          s.rank[group[h]] = (short)rank;
+          s.count[group[h]] = (short)count;
+          if (t[h] >= 0) chunks[h] = (rank + DOWN_RANKS - 1) / DOWN_RANKS, widest = max(widest, count);
+        }
+      }
+    }
+    // pairs in the order of the rows that start their groups
+    int before[2] = {chunks[0], chunks[1]};
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int v = __shfl_up_sync(0xffffffffu, before[h], off);
+        if (lane >= off) before[h] += v;
+      }
+    const int half = __shfl_sync(0xffffffffu, before[0], 31), pairs = half + __shfl_sync(0xffffffffu, before[1], 31);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      if (!(starts >> (h * 32 + lane) & 1)) continue;
+      const int from = before[h] - chunks[h] + (h ? half : 0);
+      s.first[group[h]] = (short)from;
+      for (int k = 0; k < chunks[h]; k++) s.group_of[from + k] = (signed char)group[h];
+    }
+    widest = __reduce_max_sync(0xffffffffu, widest);
+    if (lane == 0) {
+      s.groups = __popcll(starts);
+      s.widest = widest;
+      s.pairs = pairs;
+      const int parts = max(1, min(stretches, blocks / max(1, pairs)));
       s.per = (stretches + parts - 1) / parts;
       s.parts = (stretches + s.per - 1) / s.per;
     }
@@ -203,10 +219,8 @@ template <int DTYPE>
 struct Down {
   static constexpr int ESZ = DTYPE == STB_F32 ? 4 : 2;
   static constexpr int A_ROW = DOWN_COLUMNS * ESZ, X_ROW = DOWN_COLUMNS * 4;
-  static constexpr int SLOT = DOWN_RANKS * A_ROW + 16 * X_ROW;
-  static constexpr int SLOTS = 196608 / SLOT;
-  static constexpr int SMEM = SLOTS * SLOT + 16 * 16 * DOWN_RANKS * 4;  // the ring, then the warps' sums
-  static_assert(SLOTS >= 2 && SMEM + sizeof(Plan) <= 232448, "shared memory");
+  static constexpr int RING = 196608, SMEM = RING + 16 * 16 * DOWN_RANKS * 4;  // the stretches' slots, then the warps' sums
+  static_assert(RING / (DOWN_RANKS * A_ROW + 16 * X_ROW) >= 2 && SMEM + sizeof(Plan) <= 232448, "shared memory");
 };
 
 __device__ __forceinline__ void copy16_async(void *dst, const void *src, bool live) {
@@ -218,7 +232,7 @@ __device__ __forceinline__ void copy16_async(void *dst, const void *src, bool li
 // thin[part][m][j] for all rows: units (pair of a group of rows and a chunk of 32 ranks, part of the columns), one block per
 // SM and, where the plan can, one unit per block; with x3 the blocks also write the terms of x.  The factors come from
 // memory that nothing has touched lately (2 to 3 us away, behind the shared product's weights), so a block sends for all
-// that its shared memory holds (three stretches of 512 columns, 192 KB) before it waits for the first.  VEC: x and A have
+// that its shared memory holds (two to six stretches of 512 columns, by the rows of the widest group) before it waits.  VEC: x and A have
 // rows of whole 16-byte pieces (plain loads otherwise).
 template <int DTYPE, bool VEC>
 __global__ void __launch_bounds__(512, 1) pool_down_kernel(const Pool p, const float *x, float *thin, int M, int K, int stretches,
@@ -227,11 +241,12 @@ __global__ void __launch_bounds__(512, 1) pool_down_kernel(const Pool p, const f
   constexpr int NT = DOWN_RANKS / 8, ESZ = D::ESZ;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Plan s_plan;
-  float(*s_sum)[16][DOWN_RANKS] = (float(*)[16][DOWN_RANKS])(smem + D::SLOTS * D::SLOT);  // row r turned by 8 (r & 3)
+  float(*s_sum)[16][DOWN_RANKS] = (float(*)[16][DOWN_RANKS])(smem + D::RING);  // row r turned by 8 (r & 3)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   pdl_trigger();
   make_plan(p, M, stretches, gridDim.x, s_plan);
   const int units = s_plan.pairs * s_plan.parts, per = s_plan.per;
+  const int slot_bytes = DOWN_RANKS * D::A_ROW + s_plan.widest * D::X_ROW, slots = D::RING / slot_bytes;
 
   // 16-byte chunk c of row r: XORed so that the chunks that eight rows read at once lie in different banks.
   auto a_at = [&](uint8_t *slot, int r, int c) {
@@ -275,11 +290,13 @@ __global__ void __launch_bounds__(512, 1) pool_down_kernel(const Pool p, const f
         }
       }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
+  auto send_all = [&](int n) {  // the next n stretches, into the first slots
 #pragma unroll 1
-  for (int i = 0; i < D::SLOTS; i++) send(smem + i * D::SLOT);
+    for (int i = 0; i < n; i++) send(smem + i * slot_bytes);
+  };
+  if ((int)blockIdx.x < units) send_all(min(slots, min(per, stretches - (int)blockIdx.x % s_plan.parts * per)));
   if (x3) {
     const int quads = K / 4, all = terms_rows * quads, step = gridDim.x * 512;
     for (int i = blockIdx.x * 512 + threadIdx.x; i < all; i += 2 * step) {  // two in flight
@@ -296,43 +313,46 @@ __global__ void __launch_bounds__(512, 1) pool_down_kernel(const Pool p, const f
       }
     }
   }
-  int in = 0;
   for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
     const int pair = unit / s_plan.parts, part = unit % s_plan.parts, e = s_plan.group_of[pair];
     const int j0 = (pair - s_plan.first[e]) * DOWN_RANKS, rank = s_plan.rank[e] - j0, count = s_plan.count[e];
     float acc[NT][4] = {};
     const int end = min(per, stretches - part * per);
 #pragma unroll 1
-    for (int s = 0; s < end; s++) {
-      uint8_t *slot = smem + in * D::SLOT;
-      asm volatile("cp.async.wait_group %0;" ::"n"(D::SLOTS - 1) : "memory");
+    for (int done = 0; done < end; done += slots) {  // what the slots hold, and then the next of it
+      asm volatile("cp.async.wait_all;" ::: "memory");
       __syncthreads();
-      uint32_t hi[4][4], lo[4][4];  // the rows' eight values of this lane, in both terms
+#pragma unroll 1
+      for (int i = 0; i < min(slots, end - done); i++) {
+        uint8_t *slot = smem + i * slot_bytes;
+        uint32_t hi[4][4], lo[4][4];  // the rows' eight values of this lane, in both terms
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int r = g + 8 * h;
-        const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const float4 u = r < count ? *(const float4 *)x_at(slot, r, warp * 8 + t4 * 2) : zero;
-        const float4 v = r < count ? *(const float4 *)x_at(slot, r, warp * 8 + t4 * 2 + 1) : zero;
-        const float f[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+        for (int h = 0; h < 2; h++) {
+          const int r = g + 8 * h;
+          const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          const float4 u = r < count ? *(const float4 *)x_at(slot, r, warp * 8 + t4 * 2) : zero;
+          const float4 v = r < count ? *(const float4 *)x_at(slot, r, warp * 8 + t4 * 2 + 1) : zero;
+          const float f[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int j = 0; j < 4; j++)
+          for (int j = 0; j < 4; j++)
 #pragma unroll
-          for (int i = 0; i < 2; i++) split_tf32(f[2 * j + i], hi[j][2 * i + h], lo[j][2 * i + h]);
+            for (int i = 0; i < 2; i++) split_tf32(f[2 * j + i], hi[j][2 * i + h], lo[j][2 * i + h]);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          Eight<DTYPE, true> f;  // ranks behind the last hold anything, and go nowhere
+#pragma unroll
+          for (int i = 0; i < ESZ / 2; i++) f.raw[i] = *(const uint4 *)a_at(slot, n * 8 + g, (warp * 4 + t4) * (ESZ / 2) + i);
+          float c[4] = {};
+          eight_products<DTYPE>(c, hi, lo, f);
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[n][i] += c[i];
+        }
       }
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-        Eight<DTYPE, true> f;  // ranks behind the last hold anything, and go nowhere
-#pragma unroll
-        for (int i = 0; i < ESZ / 2; i++) f.raw[i] = *(const uint4 *)a_at(slot, n * 8 + g, (warp * 4 + t4) * (ESZ / 2) + i);
-        float c[4] = {};
-        eight_products<DTYPE>(c, hi, lo, f);
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[n][i] += c[i];
-      }
-      __syncthreads();  // the stretch has been read
-      send(slot);
-      in = in + 1 == D::SLOTS ? 0 : in + 1;
+      __syncthreads();  // the slots have been read
+      const int left = end - done - slots;
+      if (left > 0) send_all(min(slots, left));
+      else if (unit + gridDim.x < units) send_all(min(slots, min(per, stretches - (unit + (int)gridDim.x) % s_plan.parts * per)));
     }
 #pragma unroll
     for (int n = 0; n < NT; n++)
@@ -489,6 +509,7 @@ __global__ void __launch_bounds__(256, DTYPE == STB_F32 ? 1 : 2) pool_up_kernel(
     }
     __syncthreads();  // before thin's sums are replaced
   }
+  if (!waited) pdl_wait();  // what waits for this kernel has to find the ones before it done, too
 }
 
 template <int DTYPE, bool VEC>
