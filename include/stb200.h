@@ -158,10 +158,12 @@ typedef struct stb_adapter_pool {
 } stb_adapter_pool;
 
 /* y[m] = x[m].W^T + scales[t] * (x[m].A_t^T).B_t^T + bias with t = rows[m], int32 [M] on the device: the slot
- * of row m, negative for a row without an adapter.  Rows may name slots in any order and repeat them; every
- * slot's factors are read once per call for all its rows (16 rows at a time).  The shared product is stb_linear's; the thin
- * products accumulate in Float32.  A slot >= pool->slots leaves its row without an adapter and fails the next
- * stb_sync / stb_download.  y may not overlap an input. */
+ * of row m, negative for a row without an adapter.  Rows may name slots in any order and repeat them; a
+ * slot's factors are read once for up to 16 of its rows, 64 rows of the call at a time.  The shared product is
+ * stb_linear's; the thin products accumulate in Float32.  A slot >= pool->slots leaves its row without an adapter and
+ * fails the next stb_sync / stb_download.  y may not overlap an input.  The session's scratch holds the thin products
+ * of one call at a time and grows with the largest: make a call of the size before capturing one (STB_ERR_STATE
+ * otherwise), and replay graphs that captured it on one stream at a time. */
 int stb_linear_pool(stb_session *s, uint64_t x, uint64_t w, int w_dtype, uint64_t bias,
                     const stb_adapter_pool *pool, uint64_t rows, uint64_t y, int M, int N, int K);
 /* Host-buffer form used for end-to-end measurement: copies x from host, runs stb_linear against
@@ -228,7 +230,7 @@ int stb_op_causal_attention(stb_session *s, uint64_t q, uint64_t k, uint64_t v, 
  * Operators of a batch whose rows belong to different requests, each at its own position.  No counterpart in
  * the reference, whose caches hold one position for the whole batch.  Row indices, positions, lengths and page
  * tables are int32 device buffers, so a captured step is replayed with new ones; the calls allocate nothing
- * after the first of a session (which a capture must not be).  An index that names nothing (a page outside the
+ * after the first of a session (which a capture must not be: STB_ERR_STATE).  An index that names nothing (a page outside the
  * cache, a position behind the table) is skipped, and the next stb_sync / stb_download fails with STB_ERR_CUDA.
  * All buffers are Float32 unless stated; strides are in elements. */
 
@@ -278,8 +280,10 @@ int stb_op_paged_read(stb_session *s, const stb_paged_cache *cache, uint64_t tab
  * tables[b], scores scaled by 1 / sqrt(width), softmax in Float32 with the running maximum.  lengths: int32
  * [batch] on the device, the new token's own key included (append first).  A length of zero or below gives a
  * row of zeros; one behind the table is cut to it.  The cache is split over its length among all SMs and the
- * parts joined in a fixed order: the same call gives the same bits.  The session's one workspace serves all
- * calls, in stream order: replay graphs that captured this call on one stream at a time. */
+ * parts joined in a fixed order: the same call gives the same bits.  Weights of up to 2^8 times the largest values
+ * are summed before the division, and have to stay finite; an infinite value makes its dimension NaN.  The session's one
+ * workspace (13.3 MB of its budget) serves all calls, in stream order: replay graphs that captured this call on one
+ * stream at a time.  y may not overlap q or the cache. */
 int stb_op_paged_attention(stb_session *s, const stb_paged_cache *cache, uint64_t q, int64_t q_row, int heads,
                            uint64_t tables, int batch, int blocks, uint64_t lengths, uint64_t y, int64_t y_row);
 

@@ -566,7 +566,8 @@ extern "C" int stb_linear_pool(stb_session *s, uint64_t x, uint64_t w, int w_dty
     const int stretches = (K + DOWN_COLUMNS - 1) / DOWN_COLUMNS, columns = (N + UP_COLUMNS - 1) / UP_COLUMNS;
     STB_REQUIRE((int64_t)WINDOW * stretches * chunks <= 0x7fffffff && (int64_t)WINDOW * columns <= 0x7fffffff, "adapted Linear too large");
     const int sms = tc::sm_count(s->device), resident = (pool->dtype == STB_F32 ? 1 : 2) * sms;  // blocks of `up` at once
-    const bool skinny = K % 8 == 0 && x % 16 == 0 && skinny_eligible(M, N, K, w_dtype, (const void *)w);
+    auto tensor_cores = [&](int m) { return m > 0 && skinny_eligible(m, N, K, w_dtype, (const void *)w); };
+    const bool skinny = K % 8 == 0 && x % 16 == 0 && (tensor_cores(M) || tensor_cores(most) || tensor_cores(M % WINDOW));
     // The partial sums lie behind the shared product's own scratch.
     const uint64_t base = ((skinny ? skinny_scratch_bytes(M, N, K, s->device) : 0) + 255) & ~255ull;
     const uint64_t scratch = session_scratch(s, base + (uint64_t)stretches * most * p.max_rank * sizeof(float));

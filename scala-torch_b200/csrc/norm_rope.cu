@@ -73,12 +73,12 @@ __device__ __forceinline__ double inverse_root(double v) {
   return y * fma(-0.5 * v * y, y, 1.5);
 }
 
-// A step is up to 32 / L neighbouring query heads, or key heads, of a row, L lanes each, lane i its elements 4 i .. 4 i + 3
-// and their partners (i < half / 4 <= L).  A row has q_steps and then k_steps of them, in `parts` units of `per` steps.
 __device__ __forceinline__ void copy16_async(void *dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
 }
 
+// A step is up to 32 / L neighbouring query heads, or key heads, of a row, L lanes each, lane i its elements 4 i .. 4 i + 3
+// and their partners (i < half / 4 <= L).  A row has q_steps and then k_steps of them, in `parts` units of `per` steps.
 template <int L>
 __global__ void __launch_bounds__(THREADS, BLOCKS) qk_norm_rope_kernel(const __grid_constant__ NormRope p, int q_steps, int k_steps,
                                                                        int parts, int per, int64_t units) {
@@ -187,6 +187,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) qk_norm_rope_kernel(const __g
         if (root < 1e-36) {  // Float32 would have it with few bits
           root *= 0x1p64;
           down = 0x1p-64f;
+        } else if (root > 1e36) {  // or not at all
+          root = fmin(root * 0x1p-64, 0x1p127);
+          down = 0x1p64f;
         }
         const float inv = (float)root;
         const float4 wa = *(const float4 *)&s_weight[to.side][lane * 4], wb = *(const float4 *)&s_weight[to.side][lane * 4 + half];

@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
   const int page_shift = (c.page_size & (c.page_size - 1)) == 0 ? 31 - __clz(c.page_size) : -1;
   auto page_ahead = [&](bool live) {
     const int key = load.tile * TK + my_key;
-    if (!live || key >= load.n) return -2;
+    if (!live || key >= load.n) return -1;
     return c.tables[(size_t)(a.first + load.b) * c.blocks + (page_shift >= 0 ? key >> page_shift : key / c.page_size)];
   };
   int issued = 0, page = page_ahead(todo > 0);
@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     }
     if (issued < todo) {
       const int key = load.tile * TK + my_key, kvh = chunks_of == 1 ? load.item : load.item / chunks_of;
-      bool live = page != -2;
+      bool live = key < load.n;
       if (live && (unsigned)page >= (unsigned)c.pages) {
         *c.err = DEV_BAD_INDEX;
         live = false;
@@ -539,6 +539,9 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
   // o[i][j + 2 k]: head 2 t + j at this dimension (E4M3 values come in pairs of neighbouring dimensions).
   auto dim_of = [&](int i, int k) { return SCALED ? i * 16 + 2 * g + k : i * 16 + g + 8 * k; };
 
+  // What takes the weights' scale from a result; E4M3's own can pass Float32's range at either end: its root, applied twice.
+  auto back = [](float shift) { return SCALED ? exp2f(0.5f * (shift - P_SHIFT)) : (HALF ? 1.0f / P_SCALE : 1.0f); };
+
   // The result of an item's tiles that this warp has seen: all of them to y; a part to the block's pieces (a first
   // part, while the ring is in use) or over the warp's own ring (a last part).
   float *const block_pieces = a.pieces + (size_t)blockIdx.x * BLOCK_PIECES;
@@ -553,11 +556,12 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       const int in_chunk = 2 * t + j, head = (use.item % chunks_of) * 8 + in_chunk;
-      float *to = part + in_chunk * (WP + 4) + 4, f = 1.0f;
+      float *to = part + in_chunk * (WP + 4) + 4, f = 1.0f, f2 = 1.0f;
       int most = WP;
       if (whole) {
         to = a.y + (a.first + use.b) * a.y_row + (size_t)(use.item / chunks_of * a.group + head) * c.width;
-        f = (HALF ? 1.0f / P_SCALE : 1.0f) * (SCALED ? exp2f(m2[j] - m1[j]) : 1.0f) / sum[j];
+        f2 = back(m2[j] - m1[j]);
+        f = (SCALED ? f2 : 1.0f) / sum[j];
         most = head < a.group ? c.width : 0;
       } else if (g == 0) {
         *(float4 *)(to - 4) = make_float4(m1[j], m2[j], sum[j], 0.0f);
@@ -566,7 +570,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       for (int i = 0; i < NT; i++)
 #pragma unroll
         for (int k = 0; k < 2; k++)
-          if (dim_of(i, k) < most) to[dim_of(i, k)] = sum[j] != 0.0f ? o[i][j + 2 * k] * f : 0.0f;
+          if (dim_of(i, k) < most) to[dim_of(i, k)] = sum[j] != 0.0f ? o[i][j + 2 * k] * f2 * f : 0.0f;
     }
     if (whole) return;
     if (lane == 0) {
@@ -806,11 +810,11 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     const int head = item % chunks_of * 8 + h;
     if (head >= a.group) return;
     float *y = a.y + (a.first + b) * a.y_row + (size_t)(item / chunks_of * a.group + head) * c.width + d;
-    const float f = (HALF ? 1.0f / P_SCALE : 1.0f) * (SCALED ? exp2f(n2 - n1) : 1.0f) / all;
+    const float f2 = back(n2 - n1), f = (SCALED ? f2 : 1.0f) / all;
     const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; i++)
-      if (d + i < c.width) y[i] = all != 0.0f ? x[i] * f : 0.0f;
+      if (d + i < c.width) y[i] = all != 0.0f ? x[i] * f2 * f : 0.0f;
   };
   auto add = [](float4 &v, const float4 &x, float f) {
     if (f == 0.0f) return;  // a part without a key may hold anything

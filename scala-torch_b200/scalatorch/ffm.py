@@ -711,7 +711,8 @@ class B200Session:
     @_of_tensors
     def linear_adapted(self, x: DeviceTensor, weight: DeviceTensor, pool: "AdapterPool", rows: DeviceTensor,
                        bias: DeviceTensor | None = None, out: DeviceTensor | None = None) -> DeviceTensor:
-        """x.W^T + scale (x.A^T).B^T + bias with row m's adapter rows[m] of the pool (int32; negative: none)."""
+        """x.W^T + scale (x.A^T).B^T + bias with row m's adapter rows[m] of the pool (int32; negative: none).  out may not
+        overlap x.  A capture needs a call of this size before it."""
         require(isinstance(pool, AdapterPool) and pool.session is self, "adapter pool belongs to another session")
         M, K, N = x.shape[0] if len(x.shape) == 2 else -1, pool.inner, pool.out
         if not (not self._closed and x.session is self and x._alive[0] and x.dtype == STB_F32 and x.shape == (M, K) and not x.transposed_weight
@@ -950,7 +951,8 @@ class B200PagedCache:
     def attend(self, query: DeviceTensor, tables: DeviceTensor, lengths: DeviceTensor,
                out: DeviceTensor | None = None) -> DeviceTensor:
         """Attention of one new token per request: query (batch, heads, width) against the first lengths[b] tokens of
-        tables[b] (the new token's own key among them: append first).  A length of zero gives a row of zeros."""
+        tables[b] (the new token's own key among them: append first).  A length of zero gives a row of zeros.  out may
+        not overlap the query."""
         self._open(tables, lengths)
         s, shape = self.session, query.shape
         batch, blocks = tables.shape

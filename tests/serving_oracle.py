@@ -1,4 +1,4 @@
-"""The serving operators' definitions in numpy float64, the checkers of tests/test_serving_*.py."""
+"""The serving operators' definitions in numpy float64, the oracle of tests/test_serving_*.py."""
 import numpy as np
 
 E4M3_MAX = 448.0

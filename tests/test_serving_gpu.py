@@ -95,6 +95,29 @@ def test_qk_norm_rope(session, rows, heads, kv, width, normed, theta):
         check_norm_rope(session.download(yk), k, wk if normed else None, pos, 1e-5, theta)
 
 
+@pytest.mark.parametrize("width", [64, 36])
+def test_qk_norm_rope_of_tiny_and_large_heads(session, width):
+    """Heads whose mean square leaves Float32 at either end, and heads of zeros, beside ordinary ones."""
+    rng = np.random.default_rng(8)
+    rows, eps = 5, 1e-100
+    x = rng.standard_normal((rows, 2, width))
+    x[0] *= 1e-40
+    x[1] *= 1e37
+    x[2] = 0.0
+    x[3, 0] *= 1e-30
+    x[3, 1, :-1] = 0.0
+    x[3, 1, -1] = 1e-44
+    x = x.astype(np.float32)
+    w = (1 + 0.2 * rng.standard_normal(width)).astype(np.float32)
+    pos = np.array([0, 7, 3, 1, 50])
+    with Held(session) as h:
+        dw, dp = h.f32(w), h.ints(pos)
+        q, k = session.qk_norm_rope(h.f32(x), h.f32(x[:, :1]), dw, dw, dp, eps, 1e4)
+        h.keep(q), h.keep(k)
+        check_norm_rope(session.download(q), x, w, pos, eps, 1e4)
+        check_norm_rope(session.download(k), x[:, :1], w, pos, eps, 1e4)
+
+
 def test_qk_norm_rope_in_the_rows_of_a_fused_projection_and_in_place(session):
     """q and k as columns of one matrix whose rows have an odd length (no 16-byte alignment), one weight only, padding
     rows left as they were; then in place; extreme rows (zeros, huge, tiny, infinite)."""
@@ -286,6 +309,41 @@ def test_paged_attention_of_many_requests(session):
         check_attend(session, q, o, tables, lengths, h)
 
 
+@pytest.mark.parametrize("dtype", ["BF16", "E4M3"])
+@pytest.mark.parametrize("batch,heads,kv,width,longest", [(1100, 4, 1, 64, 20), (60, 8, 4, 128, 40), (200, 16, 1, 128, 33), (1, 8, 8, 64, 9850),
+                                                          (1, 24, 3, 80, 4000), (2, 2, 2, 64, 60)])
+def test_paged_attention_by_batch(session, dtype, batch, heads, kv, width, longest):
+    """More requests than one launch takes; many that a warp each takes whole; one request whose items take whole blocks."""
+    rng = np.random.default_rng(batch + width)
+    lengths = rng.integers(0, longest + 1, batch)
+    lengths[-1] = longest
+    tables, pages = tables_for(rng, lengths, 16)
+    o = PagedCacheOracle(rng, pages, kv, 16, width, dtype)
+    q = rng.standard_normal((batch, heads, width)).astype(np.float32)
+    with Held(session) as h:
+        check_attend(session, q, o, tables, lengths, h)
+
+
+@pytest.mark.parametrize("dtype", ["F32", "BF16", "E4M3"])
+def test_paged_attention_of_tiny_and_large_values(session, dtype):
+    """Values near the lowest scale that an E4M3 row takes (2^-126) and up to 2^100: results keep their bits.  Tolerance
+    as everywhere, and a step of the smallest Float32."""
+    rng = np.random.default_rng(14)
+    lengths, width = [150, 9, 600, 40], 64
+    tables, pages = tables_for(rng, lengths, 16)
+    o = PagedCacheOracle(rng, pages, 1, 16, width, dtype)
+    q = rng.standard_normal((4, 8, width)).astype(np.float32)
+    for b, by in enumerate((2.0 ** -119, 2.0 ** -118, 2.0 ** -119, 2.0 ** 100)):
+        n = lengths[b]
+        o.append(1, (rng.uniform(1, 2, (n, 1, width)) * by).astype(np.float32), tables, np.full(n, b), np.arange(n))
+    with Held(session) as h:
+        y = session.download(h.keep(h.cache(o).attend(h.f32(q), h.ints(tables), h.ints(lengths)))).astype(np.float64)
+        for b, n in enumerate(lengths):
+            want, mass, score = attend(q[b], o.rows(0, tables, b, n), o.rows(1, tables, b, n))
+            tol = (np.expm1(2 * (width + 8) * HALF * score) + (n + 16) * 2 * HALF) * mass + 2.0 ** -149
+            np.testing.assert_array_less(np.abs(y[b] - want), tol)
+
+
 @pytest.mark.parametrize("dtype", ["F32", "BF16", "F16", "E4M3"])
 def test_paged_attention_of_peaked_and_flat_scores(session, dtype):
     """One key that takes everything, keys far below it, scales that differ by 2^40 between tokens (E4M3), equal keys,
@@ -351,6 +409,22 @@ def test_nan_keys_and_values_inside_a_request_stay_its_own(session):
             assert np.isnan(y[0]).all()
             assert np.isnan(y[1, :, 7]).all() and np.isfinite(np.delete(y[1], 7, axis=1)).all()
             assert np.isfinite(y[2]).all()
+
+
+@pytest.mark.parametrize("page", [-1, -2, -2 ** 31, 4, 2 ** 31 - 1])
+def test_attention_reports_any_page_outside_the_cache(session, page):
+    rng = np.random.default_rng(10)
+    o = PagedCacheOracle(rng, 4, 1, 16, 64, "BF16")
+    q = rng.standard_normal((2, 4, 64)).astype(np.float32)
+    tables = np.array([[0, page], [1, 2]])
+    with Held(session) as h:
+        y = h.keep(h.cache(o).attend(h.f32(q), h.ints(tables), h.ints([20, 20])))
+        with pytest.raises(ffm.IllegalStateException, match="paged cache"):
+            session.sync()
+        got = session.download(y)
+        for b, n in ((0, 16), (1, 20)):  # what the bad page held is skipped
+            want, _, _ = attend(q[b], o.rows(0, tables, b, n), o.rows(1, tables, b, n))
+            np.testing.assert_allclose(got[b], want, rtol=0, atol=1e-5)
 
 
 def test_bad_indices_are_skipped_and_reported(session):
@@ -556,6 +630,75 @@ def test_a_serving_step_of_several_requests(session, captured):
             np.testing.assert_array_less(np.abs(got - want), 2e-5 * (1 + np.abs(want)))
         if captured:
             del graph
+
+
+def test_captures_allocate_nothing(session):
+    """A session's first call inside a capture, and one that would need more scratch, are refused; a graph captured before
+    the scratch grew replays on the buffer that it holds.  (The scratch starts at 64 MiB; 64 rows of 131072 outputs take
+    two Float32 pieces each, and the terms of x beside them.)"""
+    import torch
+    rng = np.random.default_rng(23)
+    own = ffm.B200Session(0, 4 << 30)
+    try:
+        with Held(own) as h:
+            stream = torch.cuda.ExternalStream(own.stream)
+
+            def projection(M, N, K):
+                bits = oracle.round_bf16((rng.standard_normal((N, K)) / np.sqrt(K)).astype(np.float32))
+                x, rows, pool = rng.standard_normal((M, K)).astype(np.float32), rng.integers(-1, 2, M), pool_case(rng, M, N, K, 2, 16, "BF16")
+                dw, dpool = h.keep(own.upload_weight(bits, ffm.STB_BF16)), device_pool(h, *pool, "BF16")
+                dx, drows, y = h.f32(x), h.ints(rows), h.keep(own.allocate((M, N)))
+                return lambda: own.linear_adapted(dx, dw, dpool, drows, out=y), y, adapted(x, oracle.widen(bits, oracle.BF16), None, *pool, rows)
+
+            small, y, want = projection(2, 4096, 4096)
+            large, large_y, large_want = projection(64, 131072, 128)
+            lengths = [20, 3]
+            tables, pages = tables_for(rng, lengths, 16)
+            o = PagedCacheOracle(rng, pages, 1, 16, 64, "BF16")
+            cache, q = h.cache(o), rng.standard_normal((2, 4, 64)).astype(np.float32)
+            dq, dt, dl, dz = h.f32(q), h.ints(tables), h.ints(lengths), h.keep(own.allocate((2, 4, 64)))
+            kv = h.f32(rng.standard_normal((2, 1, 64)))
+
+            def captured(calls):
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.stream(stream):
+                    graph.capture_begin(capture_error_mode="thread_local")
+                    own.qk_norm_rope(dq, kv, None, None, dl, out=(dz, kv))
+                    calls()
+                    graph.capture_end()
+                return graph
+
+            def refused(call):
+                with pytest.raises(ffm.IllegalStateException):
+                    call()
+
+            def first_calls():
+                refused(lambda: cache.attend(dq, dt, dl, out=dz))
+                refused(lambda: cache.append(kv, kv, dt, dl, dl))
+                refused(small)
+
+            del_me = captured(first_calls)
+            del del_me
+            small()
+            own.sync()
+
+            def more_scratch():
+                small()
+                refused(large)
+
+            graph = captured(more_scratch)
+            large()  # grows the scratch
+            other = h.f32(rng.standard_normal((1 << 20,)))  # what was freed may be taken again
+            kept = own.download(other)
+            ffm.call("stb_fill_value", own.handle, y.address, ffm.STB_F32, y.numel, 0.0)
+            with torch.cuda.stream(stream):
+                graph.replay()
+            for got, expected in ((own.download(y), want), (own.download(large_y), large_want)):
+                np.testing.assert_array_less(np.abs(got - expected), 1e-5 * (1 + np.abs(expected)))
+            assert np.array_equal(own.download(other), kept)
+            del graph
+    finally:
+        own.close()
 
 
 def test_chunked_prompt_through_a_quantised_cache(session):

@@ -1,4 +1,4 @@
-"""Refusals of the serving operators' Python binding, before any native call (no GPU), and their checkers' own answers."""
+"""Refusals of the serving operators' Python binding, before any native call (no GPU), and their oracle's own answers."""
 import numpy as np
 import pytest
 
@@ -107,7 +107,7 @@ def test_operands_that_are_no_tensors(s):
             bad()
 
 
-def test_the_checkers_known_answers():
+def test_the_oracles_known_answers():
     assert E4M3[0x7E] == 448.0 and E4M3[1] == 2.0 ** -9 and E4M3[0x38] == 1.0 and np.isnan(E4M3[0x7F])
     q, e = quantise(np.array([[448.0, 1.0, 0.0, -17.0], [449.0, 1.0, 0.0, -17.0], [0.0, 0.0, 0.0, 0.0], [np.inf, 2.0, np.nan, -2.0]]))
     assert list(e) == [127, 128, 127, 127 - 7]
