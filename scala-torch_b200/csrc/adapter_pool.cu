@@ -2,12 +2,18 @@
 //   y[m] = x[m].W^T + scale_t ((x[m].A_t^T).B_t^T) + bias,   t = rows[m] (none where negative),
 // the shared product and bias as stb_linear does them, the thin products by two kernels around it.
 //
-// What bounds them: the factors of every slot in use, read once (the rows of a slot go through them 16 at a time), and the
-// launches.  Every block plans the rows by slot for itself and takes units of the plan in turn.  Both products run on the
-// tensor cores in TF32 terms (the rows of a slot are the product's 16 rows): BF16 and F16 factors are TF32 values
-// already, Float32 factors and the activations are split into two terms, so the result keeps 22 bits; sums of 32 products
-// are joined in Float32.  A lane reads whole 16-byte pieces of a factor's row: the order of the summed index within 32
-// is the lanes', the same in both operands.
+// One or two rows with small factors take one launch (pool_small_kernel): every block works the thin product out for
+// itself.  The others take three.
+//
+// What bounds those: the factors of every slot in use, read once (the rows of a slot go through them 16 at a time), and
+// the launches' own starts and ends.  32 rows of 4096 x 14336 with 12 slots of rank 64 take 43.5 us, 21.6 for their bytes
+// at the copy rate: 12 us down (2.5 for the plan, 2.5 to send, 2.5 until the first factors are there, 4.5 for the
+// products), 20 the shared product, 10 up (6 of them for the pieces and thin out of L2).  The shared product's weights
+// prefetched into L2 meanwhile made it 44 to 47.  Every block plans the rows by slot for itself and takes units of the
+// plan in turn.  Both products run on the tensor cores in TF32 terms (the rows of a slot are the product's 16 rows): BF16
+// and F16 factors are TF32 values already, Float32 factors and the activations are split into two terms, so the result
+// keeps 22 bits; sums of 32 products are joined in Float32.  A lane reads whole 16-byte pieces of a factor's row: the
+// order of the summed index within 32 is the lanes', the same in both operands.
 //   1. down: thin[s][m][j] = x[m] . A_t[j] over the s-th stretch of K; beside it the shared product's own prologue, the
 //      three BF16 terms of x, where the product takes the skinny tensor-core form;
 //   2. the shared product, launched as a dependent (its weights stream in while the first kernel drains); where it takes
@@ -39,6 +45,10 @@ constexpr int DOWN_COLUMNS = 512;  // columns of it: 32 for each of 16 warps
 constexpr int UP_COLUMNS = 256;    // outputs of a unit of the second
 constexpr int MAX_RANK = 256;
 constexpr int WINDOW = 64;         // rows of one launch
+// Multiply-adds of thin that every block may repeat for one row, twice as many as for each of two.  One launch against
+// three: 1 x 1536 x 576 rank 8 4.1 against 10.0 us, rank 64 8.5 against 10.9; 1 x 1024 x 4096 rank 16 (2^16) 9.1 against
+// 12.2, rank 64 23 against 13; 2 x 576 x 576 rank 16 5.7 against 10.0, rank 56 11.9 against 10.9.
+constexpr int SMALL_WORK = 1 << 16;
 
 // The launch's rows by slot: groups of up to 16 rows that name the same slot (or none).
 struct Plan {
@@ -512,6 +522,149 @@ __global__ void __launch_bounds__(256, DTYPE == STB_F32 ? 1 : 2) pool_up_kernel(
   if (!waited) pdl_wait();  // what waits for this kernel has to find the ones before it done, too
 }
 
+// Few rows of a product that a warp per output takes anyway, with factors small enough that every block works out all of
+// thin for itself: one launch.  Float32 FMAs; a lane's eight neighbouring elements at a time, four such pieces on their
+// way together, those of the first output sent for before anything is known of the rows' slots.
+template <typename WT, int DTYPE, int MT>
+__global__ void __launch_bounds__(256) pool_small_kernel(const Pool p, const float *x, const uint16_t *w, const float *bias, float *y,
+                                                         int M, int N, int K, int per) {
+  constexpr int PIECE = DTYPE == STB_F32 ? 2 : 1, BATCH = 4, THIN = 4 / PIECE;  // loads of a factor's piece; a warp's pieces of 256 at a time
+  __shared__ float s_thin[MT][MAX_RANK];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n0 = (blockIdx.x * 8 + warp) * per;
+  auto weights = [&](uint4 (&u)[BATCH], int n, int k0) {
+#pragma unroll
+    for (int i = 0; i < BATCH; i++) {
+      const int k = k0 + i * 256 + lane * 8;
+      u[i] = n < N && k < K ? ld_stream_u4(w + (size_t)n * K + k) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  uint4 first[BATCH];
+  weights(first, n0, 0);
+  int t = -1, rank = 0;  // of row `lane`
+  float scale = 0.0f;
+  if (lane < M) {
+    t = p.rows[lane];
+    if (t >= p.slots) *p.err = DEV_BAD_INDEX + 2;
+    if (t < 0 || t >= p.slots) t = -1;
+    if (t >= 0) {
+      rank = max(0, min(p.ranks[t], p.max_rank));
+      scale = p.scales[t];
+    }
+  }
+  auto b_at = [&](int n, int m, int j) {  // the m-th row's factor of output n, rank j
+    const size_t i = ((size_t)max(0, __shfl_sync(0xffffffffu, t, m)) * N + n) * p.max_rank + j;
+    const bool in = n < N && j < __shfl_sync(0xffffffffu, rank, m);
+    if (DTYPE == STB_F32) return in ? ((const float *)p.b)[i] : 0.0f;
+    const uint16_t u = in ? ((const uint16_t *)p.b)[i] : (uint16_t)0;
+    return DTYPE == STB_BF16 ? widen1<__nv_bfloat16>(u) : widen1<__half>(u);
+  };
+  float b[MT];
+#pragma unroll
+  for (int m = 0; m < MT; m++) b[m] = m < M ? b_at(n0, m, lane) : 0.0f;
+  auto at_x = [&](int m, int k, bool half) { return k < K ? *(const float4 *)(x + (size_t)m * K + k + half * 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f); };
+  // thin: a warp per (row, rank)
+  int turn = warp;
+#pragma unroll 1
+  for (int m = 0; m < M; m++) {
+    const int r = __shfl_sync(0xffffffffu, rank, m), slot = __shfl_sync(0xffffffffu, t, m);
+#pragma unroll 1
+    for (int j = turn; j < r; j += 16) {  // ranks j and j + 8
+      const size_t row = ((size_t)slot * p.max_rank + j) * K;
+      float v[2] = {};
+#pragma unroll 1
+      for (int k0 = 0; k0 < K; k0 += THIN * 256) {
+        uint4 u[2][THIN][PIECE];
+        float4 f[THIN][2];
+#pragma unroll
+        for (int i = 0; i < THIN; i++) {
+          const int k = k0 + i * 256 + lane * 8;
+#pragma unroll
+          for (int q = 0; q < 2; q++)
+#pragma unroll
+            for (int h = 0; h < PIECE; h++)
+              u[q][i][h] = k < K && j + q * 8 < r ? *(const uint4 *)((const uint8_t *)p.a + (row + (size_t)q * 8 * K + k) * (PIECE * 2) + h * 16)
+                                                  : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int h = 0; h < 2; h++) f[i][h] = at_x(m, k, h);
+        }
+#pragma unroll
+        for (int i = 0; i < THIN; i++)
+#pragma unroll
+          for (int q = 0; q < 2; q++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              float2 c, d;
+              if constexpr (DTYPE == STB_F32) {
+                const uint4 e = u[q][i][h];
+                c = make_float2(__uint_as_float(e.x), __uint_as_float(e.y));
+                d = make_float2(__uint_as_float(e.z), __uint_as_float(e.w));
+              } else {
+                using T = std::conditional_t<DTYPE == STB_BF16, __nv_bfloat16, __half>;
+                c = widen2<T>(h ? u[q][i][0].z : u[q][i][0].x);
+                d = widen2<T>(h ? u[q][i][0].w : u[q][i][0].y);
+              }
+              v[q] = fmaf(f[i][h].x, c.x, fmaf(f[i][h].y, c.y, fmaf(f[i][h].z, d.x, fmaf(f[i][h].w, d.y, v[q]))));
+            }
+      }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1)
+#pragma unroll
+        for (int q = 0; q < 2; q++) v[q] += __shfl_xor_sync(0xffffffffu, v[q], off);
+      if (lane < 2 && j + lane * 8 < r) s_thin[m][j + lane * 8] = lane ? v[1] : v[0];
+    }
+    turn = (turn - r) & 7;  // the next row's ranks go on where these end
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int o = 0; o < per; o++) {
+    const int n = n0 + o;
+    if (n >= N) break;
+    float acc[MT] = {};
+#pragma unroll 1
+    for (int k0 = 0; k0 < K; k0 += BATCH * 256) {
+      uint4 u[BATCH];
+      if (o == 0 && k0 == 0) {
+#pragma unroll
+        for (int i = 0; i < BATCH; i++) u[i] = first[i];
+      } else {
+        weights(u, n, k0);
+      }
+#pragma unroll
+      for (int m = 0; m < MT; m++) {
+        if (m >= M) continue;
+#pragma unroll
+        for (int i = 0; i < BATCH; i++) {
+          const int k = k0 + i * 256 + lane * 8;
+          const float4 e = at_x(m, k, false), f = at_x(m, k, true);
+          const float2 c0 = widen2<WT>(u[i].x), c1 = widen2<WT>(u[i].y), c2 = widen2<WT>(u[i].z), c3 = widen2<WT>(u[i].w);
+          acc[m] = fmaf(e.x, c0.x, fmaf(e.y, c0.y, fmaf(e.z, c1.x, fmaf(e.w, c1.y, acc[m]))));
+          acc[m] = fmaf(f.x, c2.x, fmaf(f.y, c2.y, fmaf(f.z, c3.x, fmaf(f.w, c3.y, acc[m]))));
+        }
+      }
+    }
+    float out = 0.0f;
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+      if (m >= M) continue;
+      const int r = __shfl_sync(0xffffffffu, rank, m);
+      float v = 0.0f;
+      if (lane < r) v = s_thin[m][lane] * b[m];
+      for (int j0 = 32; j0 < r; j0 += 32) {
+        const float more = b_at(n, m, j0 + lane);
+        if (j0 + lane < r) v = fmaf(s_thin[m][j0 + lane], more, v);
+      }
+      const float by = __shfl_sync(0xffffffffu, scale, m);
+      v = r ? fmaf(by, v, acc[m]) : acc[m];
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+      if (lane == m) out = v;
+      if (o + 1 < per) b[m] = b_at(n + 1, m, lane);
+    }
+    if (lane < M) y[(size_t)lane * N + n] = out + (bias ? bias[n] : 0.0f);
+  }
+}
+
 template <int DTYPE, bool VEC>
 void launch_down(stb_session *s, int grid, const Pool &p, const float *x, float *thin, int M, int K, int stretches,
                  uint16_t *x3, int terms_rows, bool behind) {
@@ -527,6 +680,13 @@ void launch_down(stb_session *s, int grid, const Pool &p, const float *x, float 
   }
   launch_kernel(pool_down_kernel<DTYPE, VEC>, dim3(grid), dim3(512), (size_t)SMEM, s->stream, behind, p, x, thin, M, K, stretches,
                 x3, terms_rows, behind);
+}
+
+template <typename F>
+void dispatch_pool(int dtype, F &&f) {
+  if (dtype == STB_F32) f(std::integral_constant<int, STB_F32>());
+  else if (dtype == STB_BF16) f(std::integral_constant<int, STB_BF16>());
+  else f(std::integral_constant<int, STB_F16>());
 }
 
 }  // namespace
@@ -568,11 +728,28 @@ extern "C" int stb_linear_pool(stb_session *s, uint64_t x, uint64_t w, int w_dty
     const int sms = tc::sm_count(s->device), resident = (pool->dtype == STB_F32 ? 1 : 2) * sms;  // blocks of `up` at once
     auto tensor_cores = [&](int m) { return m > 0 && skinny_eligible(m, N, K, w_dtype, (const void *)w); };
     const bool skinny = K % 8 == 0 && x % 16 == 0 && (tensor_cores(M) || tensor_cores(most) || tensor_cores(M % WINDOW));
+    const bool vec_down = K % 8 == 0 && x % 16 == 0 && pool->a % 16 == 0;
+    if (!skinny && vec_down && w % 16 == 0 && w_dtype != STB_F32 && M <= 2 && (int64_t)M * M * p.max_rank * K <= SMALL_WORK) {
+      p.rows = (const int *)rows;
+      const int per = (N + sms * 16 - 1) / (sms * 16);
+      auto small = [&](auto wt, auto type) {
+        using WT = decltype(wt);
+        constexpr int DT = decltype(type)::value;
+        launch_kernel(M == 1 ? pool_small_kernel<WT, DT, 1> : pool_small_kernel<WT, DT, 2>,
+                      dim3((N + per * 8 - 1) / (per * 8)), dim3(256), 0, s->stream, false, p, (const float *)x, (const uint16_t *)w,
+                      (const float *)bias, (float *)y, M, N, K, per);
+      };
+      dispatch_pool(pool->dtype, [&](auto type) {
+        if (w_dtype == STB_BF16) small(__nv_bfloat16(), type);
+        else small(__half(), type);
+      });
+      count_launch(s);
+      return;
+    }
     // The partial sums lie behind the shared product's own scratch.
     const uint64_t base = ((skinny ? skinny_scratch_bytes(M, N, K, s->device) : 0) + 255) & ~255ull;
     const uint64_t scratch = session_scratch(s, base + (uint64_t)stretches * most * p.max_rank * sizeof(float));
     float *thin = (float *)(scratch + base);
-    const bool vec_down = K % 8 == 0 && x % 16 == 0 && pool->a % 16 == 0;
     const bool vec_up = p.max_rank % 8 == 0 && pool->b % 16 == 0;
     auto go = [&](auto type) {
       constexpr int DT = decltype(type)::value;
@@ -609,8 +786,6 @@ extern "C" int stb_linear_pool(stb_session *s, uint64_t x, uint64_t w, int w_dty
         count_launch(s, 2);
       }
     };
-    if (pool->dtype == STB_F32) go(std::integral_constant<int, STB_F32>());
-    else if (pool->dtype == STB_BF16) go(std::integral_constant<int, STB_BF16>());
-    else go(std::integral_constant<int, STB_F16>());
+    dispatch_pool(pool->dtype, go);
   });
 }

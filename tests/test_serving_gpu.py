@@ -527,6 +527,36 @@ def test_linear_of_a_pool(session, dtype, M, N, K, slots, rank, weight):
                 np.testing.assert_array_less(np.abs(got - want), 1e-5 * (1 + np.abs(want)))
 
 
+@pytest.mark.parametrize("dtype", ["F32", "BF16", "F16"])
+@pytest.mark.parametrize("M,N,K,rank", [(1, 1, 8, 1), (1, 577, 1032, 33), (2, 40, 264, 16), (2, 20000, 64, 9), (1, 100, 80, 256), (1, 24, 4096, 16),
+                                        (2, 300, 1096, 7), (3, 1536, 576, 8), (2, 1000, 1016, 32)])
+def test_linear_of_a_pool_for_one_or_two_rows(session, dtype, M, N, K, rank):
+    """Both sides of the rule that gives them one launch; F16 weights; a rank below the pool's; no adapter; no bias."""
+    rng = np.random.default_rng(N + K)
+    x = rng.standard_normal((M, K)).astype(np.float32)
+    bits = oracle.round_f16((rng.standard_normal((N, K)) / np.sqrt(K)).astype(np.float32))
+    w = oracle.widen(bits, oracle.F16)
+    a, b, ranks, scales = pool_case(rng, M, N, K, 3, rank, dtype)
+    ranks[1], ranks[2] = max(1, rank // 2), 0
+    a[1, ranks[1]:], b[1, :, ranks[1]:] = np.nan, np.nan
+    a[2], b[2], scales[2] = np.nan, np.nan, np.inf
+    bias = rng.standard_normal(N).astype(np.float32)
+    with Held(session) as h:
+        dw, dx, db = h.keep(session.upload_weight(bits, ffm.STB_F16)), h.f32(x), h.f32(bias)
+        pool = device_pool(h, a, b, ranks, scales, dtype)
+        for rows in ([0, 1, -7], [1, 1, 0], [-1, 0, 1], [2, 1, 2]):
+            rows = np.array(rows[:M])
+            for use in (db, None):
+                y = h.keep(session.linear_adapted(dx, dw, pool, h.ints(rows), use))
+                plain = np.where(rows == 2, -1, rows)  # a slot of rank zero adds nothing
+                want = adapted(x, w, bias if use is not None else None, np.nan_to_num(a), np.nan_to_num(b), ranks, scales, plain)
+                np.testing.assert_array_less(np.abs(session.download(y) - want), 1e-5 * (1 + np.abs(want)))
+        y = h.keep(session.linear_adapted(dx, dw, pool, h.ints(np.full(M, 3))))
+        with pytest.raises(ffm.IllegalStateException, match="adapter"):
+            session.sync()
+        np.testing.assert_array_less(np.abs(session.download(y) - x.astype(np.float64) @ w.T.astype(np.float64)), 2e-5)
+
+
 def test_linear_of_a_pool_edges(session):
     """Ranks of zero, negative and behind the pool's; NaN factors behind a slot's rank and in slots that no row names; a
     slot behind the pool; scales of zero and below; empty dimensions."""
