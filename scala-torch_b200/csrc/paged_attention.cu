@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedVie
 
 constexpr int MAX_GRID = 160;
 constexpr int DIRECT_TILES = 64;     // most tiles of an item that one block takes alone
-constexpr int WHOLE_TILES = 4;       // most tiles of an item that one warp takes alone
+constexpr int WHOLE_TILES = 8;       // most tiles of an item that one warp takes alone
 constexpr int BLOCK_PIECES = 20800;  // floats of a block's pieces, at most: (2 + warps) of 8 heads x (width + 4)
 constexpr int MAX_BATCH = 1024;      // requests of one launch (their prefix sums lie in shared memory)
 constexpr float LAZY = 8.0f;         // a maximum moves only when a score passes it by 2^8
