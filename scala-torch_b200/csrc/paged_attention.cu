@@ -126,17 +126,19 @@ struct Shape {
   static constexpr int PAIRS = WP * ESZ / 32;     // pairs of them that the products take
   static constexpr int TK = ROW >= 256 ? 16 : 32; // keys of a tile: 8 KB where the width allows
   static constexpr int TILE = 2 * TK * ROW;       // keys and values of a tile
-  // Warps and stages that fill about 192 KB: at least two stages in flight per warp, 128 KB per SM.
-  // E4M3 has the most arithmetic per byte: twelve warps of two stages (three warps per scheduler to fill); the 16 KB tiles
-  // of wide rows leave six.
-  static constexpr int WARPS = TILE <= 8192 ? (DTYPE == STB_E4M3 && ROW == 128 ? 12 : 8) : (TILE <= 16384 ? 6 : 3);
+  // Warps and stages that fill about 192 KB.  With enough arithmetic per byte more warps are worth more than a second stage
+  // for each: what one waits for, the others compute over.  0.5 GiB of cache, 82 us at the copy rate: E4M3 of width 64
+  // eight warps 165 us, twelve 136; F32 of width 128 six warps of two stages 119, twelve of one 102; F32 of width 256 three
+  // of two 268, six of one 178.  BF16 and F16 of width 64 and 128 take 93 to 97 with eight.
+  static constexpr int WARPS = TILE <= 8192 ? (DTYPE == STB_E4M3 && ROW <= 128 ? 12 : 8) : (DTYPE == STB_F32 && ROW == 512 ? 12 : 6);
   static constexpr int STAGES = 196608 / (WARPS * TILE) < 6 ? 196608 / (WARPS * TILE) : 6;
   static constexpr int META = 16 + (DTYPE == STB_E4M3 ? TK * 8 : 0);  // per stage: valid mask, scales of keys and values
+  static constexpr bool META_SCALES = DTYPE == STB_E4M3;
   static constexpr int THREADS = WARPS * 32;
   static constexpr int RING = WARPS * STAGES * TILE;
   static constexpr int PART = 8 * (WP + 4);       // floats of a partial result: per head max, weight max, sum, -, values
   static constexpr int SMEM = RING + WARPS * STAGES * META + (2 * MAX_BATCH + 4) * 4;
-  static_assert(STAGES >= 2 && SMEM + 1024 <= 232448, "shared memory per block");
+  static_assert(STAGES >= 1 && (STAGES > 1 || !META_SCALES) && SMEM + 1024 <= 232448, "shared memory per block");
   static_assert(STAGES * TILE >= PART * 4, "a warp's last part reuses its ring");
   static_assert((2 + WARPS) * PART <= BLOCK_PIECES, "workspace");
 };
@@ -594,12 +596,16 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       want = 1;
     }
     if (i >= 0) {
-      copy_wait<S::STAGES - 2>();
+      copy_wait<(S::STAGES > 1 ? S::STAGES - 2 : 0)>();
       __syncwarp();  // every lane's copies of this tile are there, and the tile before it has been read
     }
     issue(next);
     next = next + 1 == S::STAGES ? 0 : next + 1;
     if (i < 0) continue;
+    if (S::STAGES == 1) {
+      copy_wait<0>();
+      __syncwarp();
+    }
     if (SCALED && S::STAGES == 2) __syncwarp();  // the tile's scales, stored just now
     if (want == 1) {
       start_item();
