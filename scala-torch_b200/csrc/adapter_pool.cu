@@ -253,7 +253,8 @@ __global__ void __launch_bounds__(512, 1) pool_down_kernel(const Pool p, const f
   __shared__ Plan s_plan;
   float(*s_sum)[16][DOWN_RANKS] = (float(*)[16][DOWN_RANKS])(smem + D::RING);  // row r turned by 8 (r & 3)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  pdl_trigger();
+  if (!behind) pdl_wait();
+  pdl_trigger();  // after the wait: what starts early may read weights and factors at once
   make_plan(p, M, stretches, gridDim.x, s_plan);
   const int units = s_plan.pairs * s_plan.parts, per = s_plan.per;
   const int slot_bytes = DOWN_RANKS * D::A_ROW + s_plan.widest * D::X_ROW, slots = D::RING / slot_bytes;
@@ -539,6 +540,8 @@ __global__ void __launch_bounds__(256) pool_small_kernel(const Pool p, const flo
       u[i] = n < N && k < K ? ld_stream_u4(w + (size_t)n * K + k) : make_uint4(0, 0, 0, 0);
     }
   };
+  pdl_wait();
+  pdl_trigger();
   uint4 first[BATCH];
   weights(first, n0, 0);
   int t = -1, rank = 0;  // of row `lane`
@@ -678,7 +681,7 @@ void launch_down(stb_session *s, int grid, const Pool &p, const float *x, float 
       if (s->device >= 0 && s->device < 64) configured[s->device] = true;
     }
   }
-  launch_kernel(pool_down_kernel<DTYPE, VEC>, dim3(grid), dim3(512), (size_t)SMEM, s->stream, behind, p, x, thin, M, K, stretches,
+  launch_kernel(pool_down_kernel<DTYPE, VEC>, dim3(grid), dim3(512), (size_t)SMEM, s->stream, true, p, x, thin, M, K, stretches,
                 x3, terms_rows, behind);
 }
 
@@ -736,7 +739,7 @@ extern "C" int stb_linear_pool(stb_session *s, uint64_t x, uint64_t w, int w_dty
         using WT = decltype(wt);
         constexpr int DT = decltype(type)::value;
         launch_kernel(M == 1 ? pool_small_kernel<WT, DT, 1> : pool_small_kernel<WT, DT, 2>,
-                      dim3((N + per * 8 - 1) / (per * 8)), dim3(256), 0, s->stream, false, p, (const float *)x, (const uint16_t *)w,
+                      dim3((N + per * 8 - 1) / (per * 8)), dim3(256), 0, s->stream, true, p, (const float *)x, (const uint16_t *)w,
                       (const float *)bias, (float *)y, M, N, K, per);
       };
       dispatch_pool(pool->dtype, [&](auto type) {

@@ -7,8 +7,8 @@
 // out.  Every warp runs alone over its units, whole rows' heads or parts of a row's: three steps' copies ahead, the sines
 // and cosines of the unit's row in shared memory of its own.  Angles, their sines and cosines, the sum of squares and its
 // root are in double; what they are multiplied by is in Float32: at most 2 half steps of the result and 4 of each
-// rotated product beside it.  The rotation in double too took 85 us instead of 60 for 8191 rows of 40 heads of 128
-// (the conversions of its results are the scarce thing), in pairs of Float32 75 us.
+// rotated product beside it.  8191 rows of 40 heads of 128 take 60 us = 5.6 TB/s, 0.85 of the copy rate.  The rotation in
+// double too took 85 us (the conversions of its results are the scarce thing), in pairs of Float32 75.
 #include <algorithm>
 #include <cmath>
 
@@ -33,6 +33,8 @@ struct NormRope {
 __global__ void __launch_bounds__(256) qk_norm_rope_any_kernel(const NormRope p) {
   const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31, every = p.heads[0] + p.heads[1], half = p.width / 2;
+  pdl_wait();
+  pdl_trigger();
   if (unit >= (int64_t)p.rows * every) return;
   const int row = (int)(unit / every);
   int head = (int)(unit % every);
@@ -128,6 +130,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) qk_norm_rope_kernel(const __g
       start(c, out);
     }
   };
+  for (int d = threadIdx.x; d < half; d += THREADS) s_rate[d] = exp2(p.rate * d) * 0.31830988618379067154;
+  pdl_wait();
+  pdl_trigger();
   Cursor from, to;
   from.unit = to.unit = warp;
   start(from, false);
@@ -145,7 +150,6 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) qk_norm_rope_kernel(const __g
   };
 #pragma unroll 1
   for (int i = 0; i < STAGES - 1; i++) send(i);
-  for (int d = threadIdx.x; d < half; d += THREADS) s_rate[d] = exp2(p.rate * d) * 0.31830988618379067154;
   for (int i = threadIdx.x; i < 2 * p.width; i += THREADS) {
     const float *w = i < p.width ? p.w[0] : p.w[1];
     s_weight[i < p.width ? 0 : 1][i % p.width] = w ? w[i % p.width] : 1.0f;
@@ -223,12 +227,12 @@ template <int L>
 void launch_rows(stb_session *s, const NormRope &p) {
   const int heads = 32 / L, q_steps = (p.heads[0] + heads - 1) / heads, k_steps = (p.heads[1] + heads - 1) / heads;
   const int per_row = q_steps + k_steps, most = tc::sm_count(s->device) * BLOCKS;
-  // Rows in parts of five steps (59 us for 8191 rows of 40 heads of 128, 64 with parts of ten), of fewer where that leaves warps idle.
+  // Rows in parts of five steps (60 us for 8191 rows of 40 heads of 128, 64 with parts of ten), of fewer where that leaves warps idle.
   const int64_t warps = (int64_t)most * (THREADS / 32);
   const int per = (int)std::max<int64_t>(1, std::min<int64_t>(5, (int64_t)p.rows * per_row / warps));
   const int parts = (per_row + per - 1) / per;
   const int64_t units = (int64_t)p.rows * parts, blocks = std::min<int64_t>((units + THREADS / 32 - 1) / (THREADS / 32), most);
-  launch_kernel(qk_norm_rope_kernel<L>, dim3((unsigned)blocks), dim3(THREADS), 0, s->stream, false, p, q_steps, k_steps, parts, per, units);
+  launch_kernel(qk_norm_rope_kernel<L>, dim3((unsigned)blocks), dim3(THREADS), 0, s->stream, true, p, q_steps, k_steps, parts, per, units);
 }
 
 }  // namespace
@@ -283,7 +287,7 @@ extern "C" int stb_op_qk_norm_rope(stb_session *s, uint64_t q, int64_t q_row, in
     } else {
       const int64_t blocks = ((int64_t)rows * (heads + kv_heads) + 7) / 8;
       STB_REQUIRE(blocks <= 0x7fffffff, "too many rows");
-      launch_kernel(qk_norm_rope_any_kernel, dim3((unsigned)blocks), dim3(256), 0, s->stream, false, p);
+      launch_kernel(qk_norm_rope_any_kernel, dim3((unsigned)blocks), dim3(256), 0, s->stream, true, p);
     }
     count_launch(s);
   });

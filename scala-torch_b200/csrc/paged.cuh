@@ -7,6 +7,11 @@
 
 namespace stb {
 
+// The kernels of a batch of several requests start while the one before drains: each waits for it before it reads anything,
+// weights too, and lets the next one start only then, so whoever starts early finds all that came before its own
+// predecessor done.  One after another in a stream, norm and rotation of one token 3.0 -> 2.7 us, a cache write 2.2 -> 1.7,
+// attention over 33 tokens 5.9 -> 5.1; from Python 8.2 -> 5.3 us per call of the last.
+
 // A cache of the caller's (stb_paged_cache), with the page table of the call.
 struct PagedView {
   void *kv[2];        // keys, values: (pages, kv_heads, page_size, width)

@@ -18,8 +18,14 @@
 // the device only: a captured step is replayed with new ones).  A warp runs alone over its stretch, across items,
 // with a ring of cp.async stages of its own: no block barrier until its end.  The cache is the 16-row operand of
 // both products (keys, then dimensions, as rows), the 8 heads are the columns, a product per term: no row of the
-// tensor core's tile is padding.  Maxima move only when a score passes them by 2^8, which one vote per tile sees.  Items that a block covers only in part are joined
-// first among its warps in shared memory, then by the last block to arrive, always in the order of the keys.
+// tensor core's tile is padding.  Maxima move only when a score passes them by 2^8, which one vote per tile sees.
+// Items that a block covers only in part are joined first among its warps in shared memory, then by the last block to
+// arrive, always in the order of the keys.  Short items go to one block each (no join between blocks) or, many of them, to
+// one warp each (no join at all).
+//
+// Measured: 24 requests of up to 16384 BF16 tokens (8 kv heads of 128, 64 heads) 157 us = 6.1 TB/s, 0.93 of the copy rate;
+// one request of 60001 E4M3 tokens 36 us = 3.4 TB/s (its stream runs at 6.4; the rest is the start and two joins); 8 requests of up
+// to 544 E4M3 tokens 12 us; one of 33 tokens 5.8 us.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -59,6 +65,8 @@ __global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedVie
   __shared__ float s_max[W], s_sum[W], s_acc[W][512];
   const int b = a.first + blockIdx.y, h = blockIdx.x, kvh = h / a.group;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_trigger();
   const int n = attend_length(c, a, b);
   float q[D], acc[D];
 #pragma unroll
@@ -277,6 +285,8 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     }
   }
 
+  pdl_wait();
+  pdl_trigger();
   // The requests' lengths, the longest of them, and the sum of their tiles so far.
   const int per = (a.batch + S::THREADS - 1) / S::THREADS, b0 = threadIdx.x * per, b1 = min(a.batch, b0 + per);
   int own = 0, longest = 0;
@@ -1003,7 +1013,7 @@ void launch_attention(stb_session *s, const PagedView &c, AttendArgs a, int batc
   const int grid = std::min(tc::sm_count(s->device), MAX_GRID);
   for (a.first = 0; a.first < batch; a.first += at_once) {
     a.batch = std::min(at_once, batch - a.first);
-    launch_kernel(paged_attention_kernel<DTYPE, WP>, dim3(grid), dim3(S::THREADS), (size_t)S::SMEM, s->stream, false, c, a);
+    launch_kernel(paged_attention_kernel<DTYPE, WP>, dim3(grid), dim3(S::THREADS), (size_t)S::SMEM, s->stream, true, c, a);
     count_launch(s);
   }
 }
@@ -1048,7 +1058,7 @@ extern "C" int stb_op_paged_attention(stb_session *s, const stb_paged_cache *cac
                          (int64_t)c.pages * c.kv_heads * c.page_size <= 0x7fffffff && at_once > 0;
     if (!chunked) {
       dispatch_paged(cache->dtype, [&](auto t) {
-        launch_kernel(paged_attention_any_kernel<decltype(t)::value>, dim3(heads, batch), dim3(256), 0, s->stream, false, c, a);
+        launch_kernel(paged_attention_any_kernel<decltype(t)::value>, dim3(heads, batch), dim3(256), 0, s->stream, true, c, a);
       });
       count_launch(s);
       return;

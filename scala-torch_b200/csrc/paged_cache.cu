@@ -9,7 +9,9 @@
 // What bounds both: the bytes, 4 per Float32 element and 1 to 4 per stored one, each moved once.  A group of 16 or 32 lanes
 // takes the keys and values of a head for R tokens in a row, a float4 per lane each, all sent for at once (append) or
 // as soon as the tokens' pages are known (read); the lanes look the R pages up side by side.  R = 4 keeps 64 to 128 KB
-// under way per SM; calls too small to fill the SMs that way take R = 1.
+// under way per SM; calls too small to fill the SMs that way take R = 1.  E4M3, 8 heads of 128: append of 14273 tokens 29 us =
+// 5.1 TB/s, read of 20005 39 us = 5.3 TB/s, 3 us of each the launch and the ramp (26 and 35 us on the same buffers again, partly out
+// of L2).
 #include <cmath>
 
 #include "paged.cuh"
@@ -60,6 +62,8 @@ template <int DTYPE>
 __global__ void __launch_bounds__(256) paged_append_any_kernel(const PagedView c, const Rows r) {
   const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_trigger();
   if (unit >= (int64_t)r.rows * c.kv_heads) return;
   const int row = (int)(unit / c.kv_heads), head = (int)(unit % c.kv_heads);
   const int seq = r.sequences[row], pos = r.positions[row];
@@ -99,6 +103,8 @@ template <int DTYPE>
 __global__ void __launch_bounds__(256) paged_read_any_kernel(const PagedView c, const Rows r) {
   const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_trigger();
   if (unit >= (int64_t)r.rows * c.kv_heads) return;
   const int row = (int)(unit / c.kv_heads), head = (int)(unit % c.kv_heads);
   const int seq = r.sequences[row], pos = r.positions[row];
@@ -137,6 +143,8 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedView c, co
   const int lane = threadIdx.x % L, head = (int)(unit % c.kv_heads);
   const int64_t r0 = unit / c.kv_heads * R;
   float4 x[2][R][V];
+  pdl_wait();
+  pdl_trigger();
 #pragma unroll
   for (int side = 0; side < 2; side++)
 #pragma unroll
@@ -217,6 +225,8 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const PagedView c, cons
   const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / L;
   const int lane = threadIdx.x % L, head = (int)(unit % c.kv_heads);
   const int64_t r0 = unit / c.kv_heads * R;
+  pdl_wait();
+  pdl_trigger();
   const int64_t mine = token_row<R>(c, r, r0, head, lane);
   uint4 raw[2][R][V];  // as stored: 4 elements
   uint8_t e[2][R];
@@ -342,12 +352,12 @@ int stb_op_paged_append(stb_session *s, const stb_paged_cache *cache, uint64_t k
     dispatch_paged(cache->dtype, [&](auto t) {
       constexpr int DT = decltype(t)::value;
       if (!in_quads(c, r, DT)) {
-        launch_kernel(paged_append_any_kernel<DT>, dim3(grid_of(c, rows, 32, 1)), dim3(256), 0, s->stream, false, c, r);
+        launch_kernel(paged_append_any_kernel<DT>, dim3(grid_of(c, rows, 32, 1)), dim3(256), 0, s->stream, true, c, r);
         return;
       }
       by_shape(s, c, rows, [&](auto l, auto v, auto k) {
         constexpr int L = decltype(l)::value, V = decltype(v)::value, R = decltype(k)::value;
-        launch_kernel(paged_append_kernel<DT, L, V, R>, dim3(grid_of(c, rows, L, R)), dim3(256), 0, s->stream, false, c, r);
+        launch_kernel(paged_append_kernel<DT, L, V, R>, dim3(grid_of(c, rows, L, R)), dim3(256), 0, s->stream, true, c, r);
       });
     });
     count_launch(s);
@@ -366,12 +376,12 @@ int stb_op_paged_read(stb_session *s, const stb_paged_cache *cache, uint64_t tab
     dispatch_paged(cache->dtype, [&](auto t) {
       constexpr int DT = decltype(t)::value;
       if (!in_quads(c, r, DT)) {
-        launch_kernel(paged_read_any_kernel<DT>, dim3(grid_of(c, rows, 32, 1)), dim3(256), 0, s->stream, false, c, r);
+        launch_kernel(paged_read_any_kernel<DT>, dim3(grid_of(c, rows, 32, 1)), dim3(256), 0, s->stream, true, c, r);
         return;
       }
       by_shape(s, c, rows, [&](auto l, auto v, auto k) {
         constexpr int L = decltype(l)::value, V = decltype(v)::value, R = decltype(k)::value;
-        launch_kernel(paged_read_kernel<DT, L, V, R>, dim3(grid_of(c, rows, L, R)), dim3(256), 0, s->stream, false, c, r);
+        launch_kernel(paged_read_kernel<DT, L, V, R>, dim3(grid_of(c, rows, L, R)), dim3(256), 0, s->stream, true, c, r);
       });
     });
     count_launch(s);

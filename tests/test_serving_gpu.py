@@ -662,6 +662,58 @@ def test_a_serving_step_of_several_requests(session, captured):
             del graph
 
 
+@pytest.mark.parametrize("rows,N,K,rank", [(6, 1024, 320, 8), (24, 4096, 512, 33), (2, 768, 256, 4)])
+def test_steps_behind_one_another_see_what_was_written_before(session, rows, N, K, rank):
+    """Calls that start while the one before still runs: 25 steps in a row, the inputs, weights, adapters and tables of each
+    written by kernels right before it, give the same bits with a synchronisation after every call and with none."""
+    import torch
+    heads, kv, width, page, steps = 4, 2, 64, 4, 25
+    assert N >= (heads + 2 * kv) * width
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    f32 = lambda *shape: torch.randn(*shape, device="cuda", generator=gen)
+    ints = lambda high, *shape: torch.randint(0, high, shape, device="cuda", generator=gen, dtype=torch.int32)
+    blocks = -(-(steps + 30) // page)
+    start = ints(30, rows)
+    new = [dict(x=f32(rows, K), w=(f32(N, K) / K ** 0.5).bfloat16(), a=(f32(3, rank, K) / K ** 0.5).bfloat16(), b=f32(3, N, rank).bfloat16(),
+                ranks=ints(rank + 1, 3), slots=ints(4, rows) - 1, bias=f32(N), qw=f32(width), pos=start + t, len=start + t + 1) for t in range(steps)]
+    codes = dict(w=ffm.STB_BF16, a=ffm.STB_BF16, b=ffm.STB_BF16, ranks=ffm.STB_I32, slots=ffm.STB_I32, pos=ffm.STB_I32, len=ffm.STB_I32)
+    tables = torch.randperm(rows * blocks, device="cuda", generator=gen).int().reshape(rows, blocks)
+    seq = torch.arange(rows, device="cuda").int()
+    scales, stream = torch.ones(3, device="cuda"), torch.cuda.ExternalStream(session.stream)
+    wrap = lambda t, code=ffm.STB_F32: session.wrap(t.data_ptr(), t.shape, code)
+
+    def run(sync):
+        now = {k: torch.zeros_like(v) for k, v in new[0].items()}
+        pages = [torch.zeros(rows * blocks, kv, page, width, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+        fused, y = torch.zeros(rows, N, device="cuda"), torch.zeros(rows, heads, width, device="cuda")
+        kept = torch.zeros(steps, *y.shape, device="cuda")
+        torch.cuda.synchronize()
+        d = {k: wrap(v, codes.get(k, ffm.STB_F32)) for k, v in now.items()}
+        cache = session.paged_cache(*[wrap(t, ffm.STB_BF16) for t in pages])
+        pool, weight = session.adapter_pool(d["a"], d["b"], d["ranks"], wrap(scales)), session.as_weight(d["w"])
+        df, dy, dt, ds = wrap(fused), wrap(y), wrap(tables, ffm.STB_I32), wrap(seq, ffm.STB_I32)
+        q, k, v = (session.columns(df, at * width, (n, width)) for at, n in ((0, heads), (heads, kv), (heads + kv, kv)))
+        for t in range(steps):
+            with torch.cuda.stream(stream):
+                for name, value in new[t].items():
+                    now[name].copy_(value)
+            for call in (lambda: session.linear_adapted(d["x"], weight, pool, d["slots"], d["bias"], out=df),
+                         lambda: session.qk_norm_rope(q, k, d["qw"], d["qw"], d["pos"], out=(q, k)),
+                         lambda: cache.append(k, v, dt, ds, d["pos"]), lambda: cache.attend(q, dt, d["len"], out=dy)):
+                if sync:
+                    session.sync()
+                call()
+            with torch.cuda.stream(stream):
+                kept[t].copy_(y)
+        session.sync()
+        return kept.cpu(), [t.cpu() for t in pages]
+
+    slow, fast = run(True), run(False)
+    assert torch.isfinite(slow[0]).all() and (slow[0] != 0).any()
+    assert torch.equal(slow[0].view(torch.int32), fast[0].view(torch.int32))
+    assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(slow[1], fast[1]))
+
+
 def test_captures_allocate_nothing(session):
     """A session's first call inside a capture, and one that would need more scratch, are refused; a graph captured before
     the scratch grew replays on the buffer that it holds.  (The scratch starts at 64 MiB; 64 rows of 131072 outputs take
