@@ -10,7 +10,7 @@
 // takes the keys and values of a head for R tokens in a row, a float4 per lane each, all sent for at once (append) or
 // as soon as the tokens' pages are known (read); the lanes look the R pages up side by side.  R = 4 keeps 64 to 128 KB
 // under way per SM; calls too small to fill the SMs that way take R = 1.  E4M3, 8 heads of 128: append of 14273 tokens 29 us =
-// 5.1 TB/s, read of 20005 39 us = 5.3 TB/s, 3 us of each the launch and the ramp (26 and 35 us on the same buffers again, partly out
+// 5.1 TB/s, read of 20005 38 us = 5.4 TB/s, 3 us of each the launch and the ramp (26 and 35 us on the same buffers again, partly out
 // of L2).
 #include <cmath>
 
