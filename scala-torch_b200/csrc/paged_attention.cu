@@ -20,8 +20,8 @@
 // both products (keys, then dimensions, as rows), the 8 heads are the columns, a product per term: no row of the
 // tensor core's tile is padding.  Maxima move only when a score passes them by 2^8, which one vote per tile sees.
 // Items that a block covers only in part are joined first among its warps in shared memory, then by the last block to
-// arrive, always in the order of the keys.  Short items go to one block each (no join between blocks) or, many of them, to
-// one warp each (no join at all).
+// arrive, always in the order of the keys.  Few short items go to one block each, many to one warp each (no join at all),
+// many of medium length to one block each as the line has them (none between blocks).
 //
 // Measured: 24 requests of up to 16384 BF16 tokens (8 kv heads of 128, 64 heads) 157 us = 6.1 TB/s, 0.93 of the copy rate;
 // one request of 60001 E4M3 tokens 36 us = 3.4 TB/s (its stream runs at 6.4; the rest is the start and two joins); 8 requests of up
@@ -121,6 +121,11 @@ __global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedVie
 constexpr int MAX_GRID = 160;
 constexpr int DIRECT_TILES = 64;     // most tiles of an item that one block takes alone
 constexpr int WHOLE_TILES = 8;       // most tiles of an item that one warp takes alone
+// Most tiles of an item that one block takes alone where there are more items than blocks, and twice as many where there
+// are half as many again: the blocks' stretches differ by up to an item, and none is joined between blocks.  256 items of
+// up to 300 BF16 tokens 21.7 -> 15.6 us, 400 of up to 500 22.3 -> 17.5; 160 of 500 21.6 -> 19.6, of 1000 (63 tiles) 29.6
+// against 32.8; 400 of 1000 51 -> 47.
+constexpr int ROUND_TILES = 32;
 constexpr int BLOCK_PIECES = 20800;  // floats of a block's pieces, at most: (2 + warps) of 8 heads x (width + 4)
 constexpr int MAX_BATCH = 1024;      // requests of one launch (their prefix sums lie in shared memory)
 constexpr float LAZY = 8.0f;         // a maximum moves only when a score passes it by 2^8
@@ -346,7 +351,8 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
         for (int i = threadIdx.x; i < a.heads * c.width; i += S::THREADS) a.y[(a.first + b) * a.y_row + i] = 0.0f;
 
     total = s_start[a.batch] * items;
-    const bool whole = longest <= WHOLE_TILES * TK;  // short items, many of them: no item is cut
+    const bool whole = longest <= WHOLE_TILES * TK;  // short items, many of them: none is cut
+    const bool rounded = !whole && longest <= (a.batch * items >= (int)gridDim.x * 3 / 2 ? 2 : 1) * ROUND_TILES * TK;  // none is cut between blocks
     grid = min((int)gridDim.x, whole ? (total + S::WARPS - 1) / S::WARPS : (total + 2 * S::WARPS - 1) / (2 * S::WARPS));
     line = {total, grid};
     // One request: the same number of blocks for each of its items, if that idles few (no block then joins twice).
@@ -355,10 +361,6 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       line = {total / items, grid / items};
     }
     if ((int)blockIdx.x >= grid) return;
-    block0 = line.start(blockIdx.x);
-    const int mine = line.start(blockIdx.x + 1) - block0;
-    t0 = block0 + stretch_start(warp, mine, S::WARPS);
-    todo = block0 + stretch_start(warp + 1, mine, S::WARPS) - t0;
     // The place of tile t: the last request that starts at or before it (the empty ones before that share its start).
     auto locate = [&](int t) {
       Cursor k;
@@ -376,19 +378,29 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       k.tile = k.tiles ? in - k.item * k.tiles : 0;
       return k;
     };
-    load = locate(t0);
-    if (whole) {  // both ends move to the next item's start
-      int end = t0 + todo;
-      if (end < total) {
-        const Cursor k = locate(end);
-        if (k.tile) end += k.tiles - k.tile;
+    auto next_item = [&](int t) {  // the first tile from t on that starts an item
+      if (t >= total) return t;
+      const Cursor k = locate(t);
+      return k.tile ? t + k.tiles - k.tile : t;
+    };
+    int from = line.start(blockIdx.x), to = line.start(blockIdx.x + 1);
+#pragma unroll 1
+    for (int level = 0; level < 2; level++) {  // the block's stretch, then the warp's
+      if (level) {
+        const int mine = to - from;
+        block0 = from;
+        from = block0 + stretch_start(warp, mine, S::WARPS);
+        to = block0 + stretch_start(warp + 1, mine, S::WARPS);
       }
-      if (load.tile) {
-        t0 += load.tiles - load.tile;
-        if (t0 < total) load = locate(t0);
+      if (level ? whole : rounded) {
+        from = next_item(from);
+        to = next_item(to);
+        if (!level && from == to) return;
       }
-      todo = max(0, end - t0);
     }
+    t0 = from;
+    todo = to - from;
+    load = locate(t0);
   }
   use = load;
 

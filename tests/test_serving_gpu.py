@@ -311,9 +311,10 @@ def test_paged_attention_of_many_requests(session):
 
 @pytest.mark.parametrize("dtype", ["BF16", "E4M3"])
 @pytest.mark.parametrize("batch,heads,kv,width,longest", [(1100, 4, 1, 64, 20), (60, 8, 4, 128, 40), (200, 16, 1, 128, 33), (1, 8, 8, 64, 9850),
-                                                          (1, 24, 3, 80, 4000), (2, 2, 2, 64, 60)])
+                                                          (1, 24, 3, 80, 4000), (2, 2, 2, 64, 60), (32, 32, 8, 128, 300), (21, 16, 8, 64, 900), (100, 40, 2, 96, 800)])
 def test_paged_attention_by_batch(session, dtype, batch, heads, kv, width, longest):
-    """More requests than one launch takes; many that a warp each takes whole; one request whose items take whole blocks."""
+    """More requests than one launch takes; many that a warp, and longer ones that a block each takes whole; one request whose
+    items take whole blocks."""
     rng = np.random.default_rng(batch + width)
     lengths = rng.integers(0, longest + 1, batch)
     lengths[-1] = longest
