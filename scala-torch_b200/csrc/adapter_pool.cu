@@ -48,7 +48,9 @@ constexpr int WINDOW = 64;         // rows of one launch
 // Multiply-adds of thin that every block may repeat for one row, twice as many as for each of two.  One launch against
 // three: 1 x 1536 x 576 rank 8 4.1 against 10.0 us, rank 64 8.5 against 10.9; 1 x 1024 x 4096 rank 16 (2^16) 9.1 against
 // 12.2, rank 64 23 against 13; 2 x 576 x 576 rank 16 5.7 against 10.0, rank 56 11.9 against 10.9.
-constexpr int SMALL_WORK = 1 << 16;
+// A warp takes an output's whole row, so wide rows and many outputs lose: 1 x 64 x 16384 rank 4 23 against 16, 1 x 32000 x
+// 512 rank 8 21 against 14.
+constexpr int SMALL_WORK = 1 << 16, SMALL_INNER = 4096, SMALL_OUTPUTS = 2;  // outputs of a warp
 
 // The launch's rows by slot: groups of up to 16 rows that name the same slot (or none).
 struct Plan {
@@ -732,7 +734,8 @@ extern "C" int stb_linear_pool(stb_session *s, uint64_t x, uint64_t w, int w_dty
     auto tensor_cores = [&](int m) { return m > 0 && skinny_eligible(m, N, K, w_dtype, (const void *)w); };
     const bool skinny = K % 8 == 0 && x % 16 == 0 && (tensor_cores(M) || tensor_cores(most) || tensor_cores(M % WINDOW));
     const bool vec_down = K % 8 == 0 && x % 16 == 0 && pool->a % 16 == 0;
-    if (!skinny && vec_down && w % 16 == 0 && w_dtype != STB_F32 && M <= 2 && (int64_t)M * M * p.max_rank * K <= SMALL_WORK) {
+    if (!skinny && vec_down && w % 16 == 0 && w_dtype != STB_F32 && M <= 2 && K <= SMALL_INNER &&
+        N <= sms * 16 * SMALL_OUTPUTS && (int64_t)M * M * p.max_rank * K <= SMALL_WORK) {
       p.rows = (const int *)rows;
       const int per = (N + sms * 16 - 1) / (sms * 16);
       auto small = [&](auto wt, auto type) {
