@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     total = s_start[a.batch] * items;
     const bool whole = longest <= WHOLE_TILES * TK;  // short items, many of them: none is cut
     const bool rounded = !whole && longest <= (a.batch * items >= (int)gridDim.x * 3 / 2 ? 2 : 1) * ROUND_TILES * TK;  // none is cut between blocks
-    grid = min((int)gridDim.x, whole ? (total + S::WARPS - 1) / S::WARPS : (total + 2 * S::WARPS - 1) / (2 * S::WARPS));
+    grid = min((int)gridDim.x, whole ? total : (total + 2 * S::WARPS - 1) / (2 * S::WARPS));
     line = {total, grid};
     // One request: the same number of blocks for each of its items, if that idles few (no block then joins twice).
     if (a.batch == 1 && grid % items <= grid / 16) {
