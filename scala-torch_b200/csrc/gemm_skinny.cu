@@ -40,14 +40,15 @@ namespace {
 
 using namespace tc;
 
-constexpr int SK_BM = 128, SK_ACC_MAX = 4;
+constexpr int SK_ACC_MAX = 4;
+static_assert(BK == SK_BK, "K block of the plan");
 
 template <int NT>
 struct SkinnyShape {
   // Two CTAs per SM for 16- and 32-row term tiles (their MMA and epilogue latencies overlap: the 70B
   // gate/up shard at M = 8 took 169 us with one 9-stage CTA per SM and 155 us with two 5-stage CTAs),
   // one for 64-row tiles, whose stages are too large to fit two rings.
-  static constexpr int CTAS_PER_SM = NT == 64 ? 1 : 2;
+  static constexpr int CTAS_PER_SM = skinny_ctas_per_sm(NT);
   static constexpr int STAGES = NT == 16 ? 5 : (NT == 32 ? 3 : 5);
   static constexpr int A_BYTES = SK_BM * BK * 2;
   static constexpr int B_BYTES = 3 * NT * BK * 2;  // multiple of 1024: the tile stays swizzle-aligned
@@ -590,27 +591,7 @@ uint32_t skinny_idesc(int nt) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)((3 * nt) >> 3) << 17) | ((uint32_t)(SK_BM >> 4) << 24);
 }
 
-struct SkinnyPlan {
-  int nt, tiles, kbs, grid, pmax;
-  long long iters;
-  uint64_t x3_bytes, part_bytes;
-};
-
-SkinnyPlan skinny_plan(int M, int N, int K, int device) {
-  SkinnyPlan q;
-  q.nt = skinny_nt(M);
-  q.tiles = (N + SK_BM - 1) / SK_BM;
-  q.kbs = (K + BK - 1) / BK;
-  q.iters = (long long)q.tiles * q.kbs;
-  const int per_sm = q.nt == 16 ? SkinnyShape<16>::CTAS_PER_SM
-                                : (q.nt == 32 ? SkinnyShape<32>::CTAS_PER_SM : SkinnyShape<64>::CTAS_PER_SM);
-  q.grid = (int)std::min<long long>((long long)per_sm * sm_count(device), q.iters);
-  const long long per = q.iters / q.grid;  // every range holds per or per + 1 iterations
-  q.pmax = (int)std::min<long long>(q.grid, (q.kbs + per - 1) / per + 1);
-  q.x3_bytes = ((uint64_t)3 * q.nt * K * 2 + 255) & ~255ull;
-  q.part_bytes = (uint64_t)q.tiles * q.pmax * M * SK_BM * 4;
-  return q;
-}
+SkinnyPlan skinny_plan(int M, int N, int K, int device) { return skinny_plan_of(M, N, K, sm_count(device)); }
 
 template <int NT>
 void configure(int device) {
@@ -655,12 +636,11 @@ void skinny_prepare(int device) {
   configure<64>(device);
 }
 
-uint64_t skinny_scratch_bytes(int M, int N, int K, int device) {
-  const SkinnyPlan q = skinny_plan(std::min(M, 64), N, K, device);  // one 64-row block at a time
-  return q.x3_bytes + q.part_bytes;
-}
+uint64_t skinny_scratch_bytes(int M, int N, int K, int device) { return skinny_bytes_of(M, N, K, sm_count(device)); }
 
-int skinny_nt(int M) { return M <= 16 ? 16 : (M <= 32 ? 32 : 64); }
+uint64_t skinny_scratch_bytes_up_to(int rows, int N, int K, int device) {
+  return skinny_bytes_up_to(rows, N, K, sm_count(device));
+}
 
 bool skinny_norm_fusable(int N) { return N % 4 == 0 && N <= SK_NORM_CTAS * SK_NORM_THREADS * 4; }
 

@@ -21,6 +21,7 @@
 
 #include "common.cuh"
 #include "peer.cuh"
+#include "skinny_plan.cuh"
 
 namespace stb {
 
@@ -438,9 +439,11 @@ int gemv_grid_blocks(int M, int N, GemvConfig cfg, int epi);
 // activations split into three BF16 terms (FP32-accurate), with the same prologue (RMSNorm) and
 // epilogues as the vector kernel.  p.stop must be null.  skinny_eligible() says whether a
 // problem takes it (STB_SKINNY=0 keeps the vector kernel; STB_SKINNY_MIN_ROWS / _MAX_ROWS bound
-// M, default 1 .. unbounded); skinny_scratch_bytes() is the scratch one call of (M, N, K) needs.
+// M, default 1 .. unbounded); skinny_scratch_bytes() is the scratch one call of (M, N, K) needs,
+// skinny_scratch_bytes_up_to() what any call of up to `rows` rows (and of more where rows >= 64) needs.
 bool skinny_eligible(int M, int N, int K, int w_dtype, const void *w);
 uint64_t skinny_scratch_bytes(int M, int N, int K, int device);
+uint64_t skinny_scratch_bytes_up_to(int rows, int N, int K, int device);
 // Sets the kernels' shared-memory limits on `device` (before a graph capture that launches them).
 void skinny_prepare(int device);
 // The next projection's prologue done by this projection's fixup (one 64-row block): its activation
@@ -483,8 +486,6 @@ template <int EPI>
 int skinny_launch(const GemvParams &p, void *scratch, uint64_t scratch_bytes, int *err, int device,
                   cudaStream_t stream, const uint16_t *x3_ready = nullptr, const SkinnyNext *next = nullptr,
                   SkinnyParts *deferred = nullptr);
-// Token rows of the activation-term tile for a block of M <= 64 rows: 16, 32 or 64.
-int skinny_nt(int M);
 // Whether a residual projection of N outputs can do the next projection's RMSNorm prologue (SkinnyNext).
 bool skinny_norm_fusable(int N);
 

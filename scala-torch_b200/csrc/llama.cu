@@ -1577,7 +1577,7 @@ void ensure_rows(stb_llama_cache *c, int rows) {
   c->att_count = alloc_owned(s, c->owned, (uint64_t)c->batch * m->KV * sizeof(int));
   STB_CUDA(cudaMemsetAsync((void *)c->att_count, 0, (size_t)c->batch * m->KV * sizeof(int), s->stream));
   c->skin = c->skin_bytes = c->skin_next = 0;
-  {  // the largest scratch any projection of a chunk of up to min(rows, 64) rows takes
+  {  // the largest scratch any projection of a chunk of up to `rows` rows takes
     const int sm = std::min(rows, 64);
     const int wdt = m->c.weight_dtype;
     const int qkv_n = (m->NH + 2 * m->KV) * m->hd;
@@ -1586,7 +1586,7 @@ void ensure_rows(stb_llama_cache *c, int rows) {
     uint64_t need = 0;
     for (const auto &sh : shapes)
       if (skinny_eligible(sh[0], sh[1], sh[2], wdt, (const void *)256))
-        need = std::max(need, skinny_scratch_bytes(sh[0], sh[1], sh[2], s->device));
+        need = std::max(need, skinny_scratch_bytes_up_to(sh[0], sh[1], sh[2], s->device));
     if (need) {
       c->skin = alloc_owned(s, c->owned, need);
       c->skin_bytes = need;

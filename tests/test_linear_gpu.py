@@ -336,3 +336,12 @@ def test_fresh_adapter_leaves_the_linear_unchanged(session):
         session.linear(xd, wd, bd, lora=bad)
     with pytest.raises(ffm.IllegalArgumentException):
         ffm.LowRankAdapter(own_d.a, own_d.b, 0.0)
+
+
+@pytest.mark.parametrize("m,n,k", [(96, 2048, 2048), (89, 2048, 2048), (96, 6144, 768), (160, 4096, 1024), (92, 1024, 4096)])
+def test_last_blocks_that_take_more_scratch_than_whole_ones(session, m, n, k):
+    """More than 64 rows whose last block of 64 has 17 to 32: its pieces may take more than a whole block's."""
+    rng = np.random.default_rng(m + n)
+    x = rng.standard_normal((m, k)).astype(np.float32)
+    w = oracle.normal_bf16(n * k, seed=m, stream=3, std=0.02).reshape(n, k)
+    close(run_linear(session, x, w, ffm.STB_BF16), oracle.linear(x, w, oracle.BF16))

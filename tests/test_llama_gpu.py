@@ -395,3 +395,18 @@ def test_skinny_decode_with_fused_prologues(batch, fuse, heads, kvh):
     env = dict(os.environ, STB_SKINNY_MIN_WORK="0", STB_FUSE_NEXT=str(fuse), STB_FUSE_ATT=str(fuse))
     r = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=600)
     assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stdout[-2000:] + r.stderr[-4000:]
+
+
+def test_a_chunk_whose_last_block_takes_more_scratch_than_a_whole_one(session):
+    """92 prompt tokens in one chunk: blocks of 64 and 28 rows, of which the second leaves more pieces of the 2048 x 1024
+    projections; then chunks of 28 and of one, on the same cache."""
+    cfg = LlamaConfig(**dict(TINY, hidden_size=1024, intermediate_size=1024, num_attention_heads=16, num_key_value_heads=4, max_positions=128))
+    ref = oracle_model(cfg, seed=41)
+    tokens = np.random.default_rng(41).integers(0, cfg.vocab_size, (1, 121))
+    with BackendLlama.prepare_random(session, cfg, seed=41, tc_prefill_rows=-1) as m:
+        cache, oc = m.new_cache(1, 128), ref.new_cache(1, 128)
+        for a, b in ((0, 92), (92, 120), (120, 121)):
+            got, _ = cache.decode(tokens[:, a:b])
+            close(got, ref.decode(oc, tokens[:, a:b]))
+        ref.free_cache(oc)
+        cache.close()

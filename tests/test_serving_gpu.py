@@ -558,6 +558,23 @@ def test_linear_of_a_pool_for_one_or_two_rows(session, dtype, M, N, K, rank):
         np.testing.assert_array_less(np.abs(session.download(y) - x.astype(np.float64) @ w.T.astype(np.float64)), 2e-5)
 
 
+@pytest.mark.parametrize("M,N,K", [(96, 2048, 2048), (89, 2048, 2048), (96, 6144, 768), (160, 4096, 1024), (92, 1024, 4096)])
+def test_linear_of_a_pool_whose_last_window_takes_more_scratch(session, M, N, K):
+    """More than 64 rows whose last window of 64 has 17 to 32: its pieces of the shared product may take more than a whole
+    window's."""
+    rng = np.random.default_rng(M + N)
+    x = rng.standard_normal((M, K)).astype(np.float32)
+    bits = oracle.round_bf16((rng.standard_normal((N, K)) / np.sqrt(K)).astype(np.float32))
+    w = oracle.widen(bits, oracle.BF16)
+    a, b, ranks, scales = pool_case(rng, M, N, K, 5, 16, "BF16")
+    rows = rng.integers(-1, 5, M)
+    with Held(session) as h:
+        dw, dx = h.keep(session.upload_weight(bits, ffm.STB_BF16)), h.f32(x)
+        y = h.keep(session.linear_adapted(dx, dw, device_pool(h, a, b, ranks, scales, "BF16"), h.ints(rows)))
+        want = adapted(x, w, None, a, b, ranks, scales, rows)
+        np.testing.assert_array_less(np.abs(session.download(y) - want), 1e-5 * (1 + np.abs(want)))
+
+
 def test_linear_of_a_pool_edges(session):
     """Ranks of zero, negative and behind the pool's; NaN factors behind a slot's rank and in slots that no row names; a
     slot behind the pool; scales of zero and below; empty dimensions."""
