@@ -192,6 +192,13 @@ struct Eight {
   }
 };
 
+// The terms of an activation: rounded beside Float32 factors, whose own are cut; beside exact factors nothing is left out.
+template <int DTYPE>
+__device__ __forceinline__ void split_row(float x, uint32_t &hi, uint32_t &lo) {
+  if (DTYPE == STB_F32) split_tf32(x, hi, lo);
+  else cut_tf32(x, hi, lo);
+}
+
 // c += x . f over eight elements of each lane: hi and lo are x's terms (rows g, g + 8 by element), f the factor's.
 template <int DTYPE, typename E>
 __device__ __forceinline__ void eight_products(float (&c)[4], const uint32_t (&hi)[4][4], const uint32_t (&lo)[4][4], const E &f) {
@@ -200,8 +207,8 @@ __device__ __forceinline__ void eight_products(float (&c)[4], const uint32_t (&h
     const float f0 = f.get(2 * j), f1 = f.get(2 * j + 1);
     if constexpr (DTYPE == STB_F32) {
       uint32_t h0, l0, h1, l1;
-      split_tf32(f0, h0, l0);
-      split_tf32(f1, h1, l1);
+      cut_tf32(f0, h0, l0);
+      cut_tf32(f1, h1, l1);
       product_tf32(c, hi[j], l0, l1);
       product_tf32(c, lo[j], h0, h1);
       product_tf32(c, hi[j], h0, h1);
@@ -349,7 +356,7 @@ __global__ void __launch_bounds__(512, 1) pool_down_kernel(const Pool p, const f
 #pragma unroll
           for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int i = 0; i < 2; i++) split_tf32(f[2 * j + i], hi[j][2 * i + h], lo[j][2 * i + h]);
+            for (int i = 0; i < 2; i++) split_row<DTYPE>(f[2 * j + i], hi[j][2 * i + h], lo[j][2 * i + h]);
         }
 #pragma unroll
         for (int n = 0; n < NT; n++) {
@@ -489,8 +496,8 @@ __global__ void __launch_bounds__(256, DTYPE == STB_F32 ? 1 : 2) pool_up_kernel(
 #pragma unroll
         for (int i = 0; i < 2; i++) {
           const int at = kb * 32 + t4 * 8 + 2 * j + i;
-          split_tf32(g < count ? s_thin[g][at] : 0.0f, hi[j][2 * i], lo[j][2 * i]);
-          split_tf32(g + 8 < count ? s_thin[g + 8][at] : 0.0f, hi[j][2 * i + 1], lo[j][2 * i + 1]);
+          split_row<DTYPE>(g < count ? s_thin[g][at] : 0.0f, hi[j][2 * i], lo[j][2 * i]);
+          split_row<DTYPE>(g + 8 < count ? s_thin[g + 8][at] : 0.0f, hi[j][2 * i + 1], lo[j][2 * i + 1]);
         }
       const int live = rank - (kb * 32 + t4 * 8);
 #pragma unroll

@@ -10,7 +10,7 @@
 //   * BF16 cache: q and p in three BF16 terms (24 bits);
 //   * F16 and E4M3 cache (E4M3 widens to F16 exactly): two F16 terms (22 bits), after a power of two that puts the
 //     largest q of a head at 2^12 and p at 2^7 .. 2^15, so that F16's range costs nothing;
-//   * F32 cache: both sides in two TF32 terms.
+//   * F32 cache: both sides in two TF32 terms (q and p 23 bits, keys 22, values 21), without the product of the lower ones.
 // The tensor core truncates its sums, so chains are kept short (at most 8 products) and joined by Float32 additions.
 //
 // Work: items (request, kv head, chunk of 8 query heads) are cut into tiles of 16 or 32 keys, all tiles in one line; each
@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
           } else if constexpr (DTYPE == STB_F32) {
             uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) split_tf32(__uint_as_float(r[i]), hi[i], lo[i]);
+            for (int i = 0; i < 4; i++) cut_tf32(__uint_as_float(r[i]), hi[i], lo[i]);
             product<DTYPE>(acc[b][0][s & 1], hi, q[s][0], q[s][1]);
             product<DTYPE>(acc[b][1][s & 1], hi, q[s][2], q[s][3]);
             product<DTYPE>(acc[b][2][s & 1], lo, q[s][0], q[s][1]);
@@ -767,7 +767,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
             asm volatile("ld.shared.f32 %0, [%1];"
                          : "=f"(v)
                          : "r"(chunk_at<S::ROW>(values, 8 * k + 2 * t + (i >> 1), 4 * n + 2 * (i & 1) + (g >> 2)) + (g & 3) * 4));
-            split_tf32(v, vh[i], vl[i]);
+            cut_both_tf32(v, vh[i], vl[i]);
           }
           product<DTYPE>(r, vl, hi[k][0], hi[k][1]);
           product<DTYPE>(r, vh, lo[k][0], lo[k][1]);
