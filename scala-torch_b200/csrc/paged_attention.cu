@@ -8,8 +8,10 @@
 // cores (mma.sync, fed by each warp's own ring: with 8 columns there is no reuse that larger tiles could find), with
 // Float32 accuracy kept by splitting the Float32 side into terms that the products take exactly:
 //   * BF16 cache: q and p in three BF16 terms (24 bits);
-//   * F16 and E4M3 cache (E4M3 widens to F16 exactly): two F16 terms (22 bits), after a power of two that puts the
-//     largest q of a head at 2^12 and p at 2^7 .. 2^15, so that F16's range costs nothing;
+//   * F16 and E4M3 cache (E4M3 widens to F16 exactly): two F16 terms (22 bits).  q after a power of two that puts the largest
+//     of a head at 2^12 (22 bits of that largest one); weights after one per head that follows the tiles' largest (2^7 ..
+//     2^15), the second term's times 2^12, in a sum of its own.  That keeps 22 bits of every weight down to 2^-21 of its
+//     tile's largest; lower ones beside it are added in Float32, key by key;
 //   * F32 cache: both sides in two TF32 terms (q and p 23 bits, keys 22, values 21), without the product of the lower ones.
 // The tensor core truncates its sums, so chains are kept short (at most 8 products) and joined by Float32 additions.
 //
@@ -129,7 +131,9 @@ constexpr int ROUND_TILES = 32;
 constexpr int BLOCK_PIECES = 20800;  // floats of a block's pieces, at most: (2 + warps) of 8 heads x (width + 4)
 constexpr int MAX_BATCH = 1024;      // requests of one launch (their prefix sums lie in shared memory)
 constexpr float LAZY = 8.0f;         // a maximum moves only when a score passes it by 2^8
-constexpr float P_SHIFT = 7.0f, P_SCALE = 128.0f;  // F16 weights times 2^7: at most 2^15, and 2^-32 apart at their lowest
+// F16 weights: the tile's largest is put at 2^7 (and may grow to 2^15 before that moves), the rest behind the first term's 11
+// bits times 2^12.  From 2^-14 on, F16's smallest with all its bits, both terms together keep 22.
+constexpr float P_SHIFT = 7.0f, P_LOW = -14.0f, P_REST = 4096.0f;  // log2, log2, factor
 
 template <int DTYPE, int WP>
 struct Shape {
@@ -141,9 +145,10 @@ struct Shape {
   static constexpr int TILE = 2 * TK * ROW;       // keys and values of a tile
   // Warps and stages that fill about 192 KB.  With enough arithmetic per byte more warps are worth more than a second stage
   // for each: what one waits for, the others compute over.  0.5 GiB of cache, 82 us at the copy rate: E4M3 of width 64
-  // eight warps 165 us, twelve 136; F32 of width 128 six warps of two stages 119, twelve of one 102; F32 of width 256 three
-  // of two 268, six of one 178.  BF16 and F16 of width 64 and 128 take 93 to 97 with eight.
-  static constexpr int WARPS = TILE <= 8192 ? (DTYPE == STB_E4M3 && ROW <= 128 ? 12 : 8) : (DTYPE == STB_F32 && ROW == 512 ? 12 : 6);
+  // eight warps 165 us, twelve 136 (143 with the weights' range, below); F32 of width 128 six warps of two stages 119, twelve of one 102; F32 of width 256 three
+  // of two 268, six of one 178.  BF16 and F16 of width 64 and 128 take 93 to 97 with eight.  E4M3 of width 128 has too few
+  // registers with twelve: 64 requests of 3000 tokens, 8 kv heads of it, 113 us with twelve, 91 with eleven.
+  static constexpr int WARPS = TILE <= 8192 ? (DTYPE == STB_E4M3 && ROW <= 128 ? (WP == 128 ? 11 : 12) : 8) : (DTYPE == STB_F32 && ROW == 512 ? 12 : 6);
   static constexpr int STAGES = 196608 / (WARPS * TILE) < 6 ? 196608 / (WARPS * TILE) : 6;
   static constexpr int META = 16 + (DTYPE == STB_E4M3 ? TK * 8 : 0);  // per stage: valid mask, scales of keys and values
   static constexpr bool META_SCALES = DTYPE == STB_E4M3;
@@ -219,11 +224,11 @@ __device__ __forceinline__ void split3_pair(float x, float y, uint32_t (&t)[3]) 
     y -= __uint_as_float(t[i] & 0xffff0000u);
   }
 }
-// Two F16 terms.
-__device__ __forceinline__ void split2_pair(float x, float y, uint32_t (&t)[2]) {
+// Two F16 terms, the second times `up`.
+__device__ __forceinline__ void split2_pair(float x, float y, uint32_t (&t)[2], float up = 1.0f) {
   const __half2 h = __floats2half2_rn(x, y);
   const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  const __half2 l = __floats2half2_rn((x - f.x) * up, (y - f.y) * up);
   t[0] = *reinterpret_cast<const uint32_t *>(&h);
   t[1] = *reinterpret_cast<const uint32_t *>(&l);
 }
@@ -492,6 +497,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
 
   uint32_t q[STEPS][2 * TERMS];
   float o[NT][4], m1[2], m2[2], sum[2], unscale[2] = {1.0f, 1.0f};
+  float base[2], down[2];  // F16 weights are 2^(score - base); `down` takes them to the scale of o, 2^P_SHIFT at m2
 
   // q of the item at `use` into registers: dimensions of this lane in step s, two pairs (F32: two single ones).
   constexpr int N = DTYPE == STB_F32 ? 2 : 4;
@@ -558,13 +564,15 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
     for (int i = 0; i < NT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
     m1[0] = m1[1] = m2[0] = m2[1] = -INFINITY;
     sum[0] = sum[1] = 0.0f;
+    base[0] = base[1] = -1e30f;
+    down[0] = down[1] = 1.0f;
   };
 
   // o[i][j + 2 k]: head 2 t + j at this dimension (E4M3 values come in pairs of neighbouring dimensions).
   auto dim_of = [&](int i, int k) { return SCALED ? i * 16 + 2 * g + k : i * 16 + g + 8 * k; };
 
   // What takes the weights' scale from a result; E4M3's own can pass Float32's range at either end: its root, applied twice.
-  auto back = [](float shift) { return SCALED ? exp2f(0.5f * (shift - P_SHIFT)) : (HALF ? 1.0f / P_SCALE : 1.0f); };
+  auto back = [](float shift) { return SCALED ? exp2f(0.5f * (shift - P_SHIFT)) : (HALF ? 0x1p-7f : 1.0f); };
 
   // The result of an item's tiles that this warp has seen: all of them to y; a part to the block's pieces (a first
   // part, while the ring is in use) or over the warp's own ring (a last part).
@@ -670,7 +678,6 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
         }
     }
     float sc[MB][4], sw[SCALED ? MB : 1][4];  // [2 k + j]: key g + 8 k, head 2 t + j
-    bool move = false;
 #pragma unroll
     for (int b = 0; b < MB; b++)
 #pragma unroll
@@ -696,51 +703,116 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
           if (!(mask >> (16 * b + 8 * k + g) & 1))
             sc[b][2 * k] = sc[b][2 * k + 1] = sw[SCALED ? b : 0][2 * k] = sw[SCALED ? b : 0][2 * k + 1] = -INFINITY;
     }
+    // What is rare, by one vote: a score that passed its maximum by far, or (F16 weights) one out of the weights' range.
+    auto weighed = [&](int b, int i) { return SCALED ? sw[b][i] : sc[b][i]; };  // log2 of the weight
+    auto is_rare = [&](bool masked_too) {
+      bool rare = false;
 #pragma unroll
-    for (int b = 0; b < MB; b++)
+      for (int b = 0; b < MB; b++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        move |= sc[b][i] > m1[i & 1] + LAZY;
-        if (SCALED) move |= sw[b][i] > m2[i & 1] + LAZY;
-      }
-    if (__any_sync(0xffffffffu, move)) {  // some score passed its maximum by far: move the heads' maxima
-#pragma unroll
-      for (int j = 0; j < 2; j++) {
-        float n1 = m1[j], n2 = m2[j];
-#pragma unroll
-        for (int b = 0; b < MB; b++) {
-          n1 = fmaxf(n1, fmaxf(sc[b][j], sc[b][2 + j]));
-          if (SCALED) n2 = fmaxf(n2, fmaxf(sw[b][j], sw[b][2 + j]));
+        for (int i = 0; i < 4; i++) {
+          if (SCALED || !HALF) rare |= sc[b][i] > m1[i & 1] + LAZY;
+          if (HALF) {
+            rare |= weighed(b, i) > base[i & 1] + (P_SHIFT + LAZY);
+            if (masked_too) rare |= weighed(b, i) < base[i & 1] + P_LOW;
+            else rare |= (weighed(b, i) < base[i & 1] + P_LOW) & (weighed(b, i) != -INFINITY);
+          }
         }
+      return __any_sync(0xffffffffu, rare);  // the same for the whole warp
+    };
+    if (is_rare(true)) {  // a masked key looks so at first
+      if (!HALF || is_rare(false)) {  // move the heads' maxima, and the weights' base to this tile's
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-          n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, off));
-          if (SCALED) n2 = fmaxf(n2, __shfl_xor_sync(0xffffffffu, n2, off));
-        }
-        if (!SCALED) n2 = n1;
-        const float f1 = n1 == m1[j] ? 1.0f : pow2(m1[j] - n1), f2 = n2 == m2[j] ? 1.0f : pow2(m2[j] - n2);
-        sum[j] *= f1;
+        for (int j = 0; j < 2; j++) {
+          float t1 = -INFINITY, t2 = -INFINITY;  // of this tile
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
-          o[i][j] *= f2;
-          o[i][2 + j] *= f2;
+          for (int b = 0; b < MB; b++) {
+            t1 = fmaxf(t1, fmaxf(sc[b][j], sc[b][2 + j]));
+            if (SCALED) t2 = fmaxf(t2, fmaxf(sw[b][j], sw[b][2 + j]));
+          }
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) {
+            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, off));
+            if (SCALED) t2 = fmaxf(t2, __shfl_xor_sync(0xffffffffu, t2, off));
+          }
+          const float n1 = fmaxf(m1[j], t1), n2 = SCALED ? fmaxf(m2[j], t2) : n1;
+          const float f1 = n1 == m1[j] ? 1.0f : pow2(m1[j] - n1), f2 = n2 == m2[j] ? 1.0f : pow2(m2[j] - n2);
+          sum[j] *= f1;
+#pragma unroll
+          for (int i = 0; i < NT; i++) {
+            o[i][j] *= f2;
+            o[i][2 + j] *= f2;
+          }
+          m1[j] = n1;
+          m2[j] = n2;
+          if (HALF) {
+            if (!SCALED) t2 = t1;
+            if (t2 != -INFINITY) {
+              base[j] = n2 - (P_SHIFT + fminf(100.0f, ceilf(n2 - t2)));
+              down[j] = pow2(base[j] - n2 + P_SHIFT);
+            }
+          }
         }
-        m1[j] = n1;
-        m2[j] = n2;
+        if constexpr (HALF) {  // weights out of the range even so: in Float32, key by key
+          float apart[MB][4];
+          bool some = false;
+#pragma unroll
+          for (int b = 0; b < MB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const bool low = (weighed(b, i) < base[i & 1] + P_LOW) & (weighed(b, i) != -INFINITY);
+              apart[b][i] = low ? pow2(weighed(b, i) - base[i & 1]) : 0.0f;
+              if (!SCALED) sum[i & 1] += low ? pow2(sc[b][i] - m1[i & 1]) : 0.0f;
+              if (SCALED) sw[b][i] = low ? -INFINITY : sw[b][i];
+              else sc[b][i] = low ? -INFINITY : sc[b][i];
+              some |= apart[b][i] > 0.0f;
+            }
+          if (__any_sync(0xffffffffu, some)) {
+#pragma unroll 1
+            for (int key = 0; key < TK; key++) {
+              float x[2];
+#pragma unroll
+              for (int j = 0; j < 2; j++) {
+                x[j] = apart[0][j];
+#pragma unroll
+                for (int i = 1; i < 2 * MB; i++) x[j] = key >> 3 == i ? apart[i >> 1][2 * (i & 1) + j] : x[j];
+                x[j] = __shfl_sync(0xffffffffu, x[j], (key & 7) * 4 + t) * down[j];
+              }
+              if (!__any_sync(0xffffffffu, (x[0] > 0.0f) | (x[1] > 0.0f))) continue;
+#pragma unroll
+              for (int i = 0; i < NT; i++)
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                  float v;
+                  if constexpr (SCALED) {
+                    uint32_t u;
+                    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(u) : "r"(chunk_at<S::ROW>(values, key, i) + 2 * g + k));
+                    v = widen_e4m3x2((uint16_t)u).x;
+                  } else {
+                    uint16_t u;
+                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(chunk_at<S::ROW>(values, key, 2 * i + k) + 2 * g));
+                    v = widen1<__half>(u);
+                  }
+                  o[i][2 * k] = fmaf(x[0], v, o[i][2 * k]);
+                  o[i][2 * k + 1] = fmaf(x[1], v, o[i][2 * k + 1]);
+                }
+            }
+          }
+        }
       }
     }
     // Weights; a maximum of -inf means that no key has counted yet, and none does here (their scores are -inf).
     float w[MB][4];
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-      const float base1 = m1[j] == -INFINITY ? 0.0f : m1[j], base2 = m2[j] == -INFINITY ? 0.0f : m2[j] - P_SHIFT;
+      const float base1 = m1[j] == -INFINITY ? 0.0f : m1[j];
 #pragma unroll
       for (int b = 0; b < MB; b++)
 #pragma unroll
         for (int k = 0; k < 2; k++) {
           const float p = pow2(sc[b][2 * k + j] - base1);
           sum[j] += p;
-          w[b][2 * k + j] = SCALED ? pow2(sw[b][2 * k + j] - base2) : (HALF ? p * P_SCALE : p);
+          w[b][2 * k + j] = HALF ? pow2(weighed(b, 2 * k + j) - base[j]) : p;
         }
     }
 
@@ -783,7 +855,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
 #pragma unroll
         for (int k = 0; k < 2; k++) {
           if constexpr (DTYPE == STB_BF16) split3_pair(w[b][2 * k], w[b][2 * k + 1], p[b][k]);
-          else split2_pair(w[b][2 * k], w[b][2 * k + 1], p[b][k]);
+          else split2_pair(w[b][2 * k], w[b][2 * k + 1], p[b][k], P_REST);
 #pragma unroll
           for (int i = 0; i < TERMS; i++) p[b][k][i] = transpose8(p[b][k][i]);
         }
@@ -791,28 +863,32 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
 #pragma unroll
       for (int s = 0; s < S::PAIRS; s++) {
         constexpr int PAIR = SCALED ? 2 : 1;  // 16-dimension results of two chunks
-        float r[PAIR][4] = {};
+        constexpr int SUMS = HALF ? 2 : 1;    // of the first terms, and of the second ones
+        uint32_t v[MB][4];
 #pragma unroll
-        for (int b = 0; b < MB; b++) {
-          uint32_t v[4];
-          load_matrix4_trans(v, chunk_at<S::ROW>(values, row + 16 * b, 2 * s + odd));
-          if constexpr (SCALED) {
+        for (int b = 0; b < MB; b++) load_matrix4_trans(v[b], chunk_at<S::ROW>(values, row + 16 * b, 2 * s + odd));
 #pragma unroll
-            for (int h = 0; h < 2; h++) {  // bytes (key, dim), (key, dim + 1), (key + 1, dim), (key + 1, dim + 1)
-              const uint32_t x = __byte_perm(v[h], 0, 0x3120), z = __byte_perm(v[2 + h], 0, 0x3120);
+        for (int h = 0; h < PAIR; h++) {
+          float r[SUMS][4] = {};
+#pragma unroll
+          for (int b = 0; b < MB; b++) {
+            if constexpr (SCALED) {  // bytes (key, dim), (key, dim + 1), (key + 1, dim), (key + 1, dim + 1)
+              const uint32_t x = __byte_perm(v[b][h], 0, 0x3120), z = __byte_perm(v[b][2 + h], 0, 0x3120);
               const uint32_t u[4] = {widen_pair(x & 0xffffu), widen_pair(x >> 16), widen_pair(z & 0xffffu), widen_pair(z >> 16)};
 #pragma unroll
-              for (int i = TERMS - 1; i >= 0; i--) product<DTYPE>(r[h], u, p[b][0][i], p[b][1][i]);
-            }
-          } else {
+              for (int i = TERMS - 1; i >= 0; i--) product<DTYPE>(r[i % SUMS], u, p[b][0][i], p[b][1][i]);
+            } else {
 #pragma unroll
-            for (int i = TERMS - 1; i >= 0; i--) product<DTYPE>(r[0], v, p[b][0][i], p[b][1][i]);
+              for (int i = TERMS - 1; i >= 0; i--) product<DTYPE>(r[i % SUMS], v[b], p[b][0][i], p[b][1][i]);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            float &to = o[PAIR * s + h][i];
+            if (HALF) to = fmaf(r[0][i], down[i & 1], fmaf(r[SUMS - 1][i], down[i & 1] / P_REST, to));
+            else to += r[0][i];
           }
         }
-#pragma unroll
-        for (int h = 0; h < PAIR; h++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) o[PAIR * s + h][i] += r[h][i];
       }
     }
 

@@ -186,3 +186,88 @@ def test_float32_factors_at_the_top_of_the_range(session, M, N, K):
             got = session.download(h.keep(session.linear_adapted(dx, dw, device_pool(h, a, b, ranks, scales, "F32"), h.ints(rows))))
             want = adapted(x, w, None, a, b, ranks, scales, rows)
             np.testing.assert_array_less(np.abs(got - want), 1e-5 * (1 + np.abs(want)))
+
+
+# ------------------------------------------------------------------ weights far below the largest
+
+
+@pytest.mark.parametrize("dtype,width", [("F32", 64), ("BF16", 128), ("F16", 64), ("F16", 128), ("F16", 96), ("F16", 256), ("E4M3", 64), ("E4M3", 128),
+                                         ("E4M3", 96), ("E4M3", 256), ("F16", 36)])
+@pytest.mark.parametrize("gap", [0, 11, 16, 20, 23, 30, 45])
+def test_keys_far_below_one_without_a_value_keep_their_bits(session, dtype, width, gap):
+    """A first key `gap` nats above all others whose own value is zero (request 0), or as small as their share of the result
+    (request 1), a key like it in the middle (request 2, whose others score alike).  Weights in Float32 keep the rest of
+    the result.  Beside the 2e-6 of the norm, the scores' own roundings: a weight moves with its score and the largest one's,
+    each within 8 half steps of its sum |q k| / sqrt(width), so 16 half steps of the largest."""
+    rng = np.random.default_rng(gap * 7 + width)
+    page, lengths, heads = 16, [2001, 2001, 700], 8
+    tables, pages = tables_for(rng, lengths, page)
+    o = PagedCacheOracle(rng, pages, 1, page, width, dtype)
+    q = (0.5 * rng.standard_normal((3, heads, width))).astype(np.float32)
+    q[:, :, 0] = np.sqrt(width)
+    for b, n in enumerate(lengths):
+        k, v = (rng.standard_normal((n, 1, width)).astype(np.float32) for _ in range(2))
+        k[:, :, 0] = 0.0
+        if b == 2:
+            k[:] = k[5]
+        first = n // 2 if b == 2 else 0
+        k[first] = 0.0
+        k[first, 0, 0] = gap
+        v[first] *= np.exp(-gap) if b == 1 else 0.0
+        for side, x in ((0, k), (1, v)):
+            o.append(side, x, tables, np.full(n, b), np.arange(n))
+    with Held(session) as h:
+        got = attended(h, o, q, tables, lengths)
+    check_rows(got, o, q, tables, lengths)
+    for b, n in enumerate(lengths):
+        want, _, score = attend(q[b], o.rows(0, tables, b, n), o.rows(1, tables, b, n))
+        off = np.linalg.norm(got[b] - want) / np.linalg.norm(want)
+        assert off <= 2e-6 + 16 * HALF * score.max(), (b, off)
+
+
+@pytest.mark.parametrize("width", [64, 128, 96, 256, 36])
+@pytest.mark.parametrize("by", [-6, -12, -20, -40, -80])
+def test_small_rows_beside_rows_of_zeros_keep_their_bits(session, width, by):
+    """E4M3 rows of zeros carry the scale 2^0, above that of rows of 2^by: every fourth value is zero."""
+    rng = np.random.default_rng(width - by)
+    lengths = [33, 900]
+    tables, pages = tables_for(rng, lengths, 16)
+    o = PagedCacheOracle(rng, pages, 1, 16, width, "E4M3")
+    q = rng.standard_normal((2, 8, width)).astype(np.float32)
+    for b, n in enumerate(lengths):
+        v = (rng.uniform(1, 2, (n, 1, width)) * 2.0 ** by).astype(np.float32)
+        v[::4] = 0.0
+        o.append(1, v, tables, np.full(n, b), np.arange(n))
+    with Held(session) as h:
+        got = attended(h, o, q, tables, lengths)
+    check_rows(got, o, q, tables, lengths)
+    for b, n in enumerate(lengths):
+        want, _, score = attend(q[b], o.rows(0, tables, b, n), o.rows(1, tables, b, n))
+        assert np.linalg.norm(got[b] - want) <= (2e-6 + 16 * HALF * score.max()) * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("dtype", ["F16", "E4M3"])
+def test_weights_of_every_size_in_one_cache(session, dtype):
+    """Scores spread evenly over 80 nats, rising, falling and shuffled: the running maximum moves, and every tile holds weights
+    of many sizes; only the lowest keys have a value in some dimensions."""
+    rng = np.random.default_rng(5)
+    n, width = 1500, 64
+    tables, pages = tables_for(rng, [n] * 3, 16)
+    o = PagedCacheOracle(rng, pages, 1, 16, width, dtype)
+    q = np.zeros((3, 8, width), np.float32)
+    q[:, :, 0] = 8.0
+    for b in range(3):
+        s = np.linspace(-40, 40, n)
+        s = s if b == 0 else (s[::-1] if b == 1 else rng.permutation(s))
+        k, v = np.zeros((n, 1, width), np.float32), rng.uniform(1, 2, (n, 1, width)).astype(np.float32)
+        k[:, 0, 0] = s
+        for d in range(0, 32):
+            v[s > 40 - 2 * d, 0, d] = 0.0
+        for side, x in ((0, k), (1, v)):
+            o.append(side, x, tables, np.full(n, b), np.arange(n))
+    with Held(session) as h:
+        got = attended(h, o, q, tables, [n] * 3)
+    for b in range(3):
+        want, mass, score = attend(q[b], o.rows(0, tables, b, n), o.rows(1, tables, b, n))
+        # each dimension by itself: 40 half steps (22-bit terms, the scores' roundings as above) of its own sum
+        np.testing.assert_array_less(np.abs(got[b] - want), (40 + 16 * score.max()) * HALF * mass + 1e-37)
