@@ -89,7 +89,8 @@ __global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedVie
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
     if (DTYPE == STB_E4M3) dot *= scale_of(c.scale[0][at]);
-    const float now = fmaxf(top, dot), keep = top == now ? 1.0f : exp2f(top - now), p = exp2f(dot - now);
+    const float now = fmaxf(top, dot), keep = top == now ? 1.0f : exp2f(top - now);
+    const float p = dot == -INFINITY ? 0.0f : exp2f(dot - now);  // the maximum itself may be -inf still
     const float pv = DTYPE == STB_E4M3 ? p * scale_of(c.scale[1][at]) : p;
     sum = sum * keep + p;
 #pragma unroll

@@ -271,3 +271,31 @@ def test_weights_of_every_size_in_one_cache(session, dtype):
         want, mass, score = attend(q[b], o.rows(0, tables, b, n), o.rows(1, tables, b, n))
         # each dimension by itself: 40 half steps (22-bit terms, the scores' roundings as above) of its own sum
         np.testing.assert_array_less(np.abs(got[b] - want), (40 + 16 * score.max()) * HALF * mass + 1e-37)
+
+
+# ------------------------------------------------------------------ scores of minus infinity
+
+
+@pytest.mark.parametrize("width", [64, 36, 33, 512])  # whole 16-byte pieces and the others: the answer is the same
+@pytest.mark.parametrize("dtype", ["F32", "BF16"])
+def test_keys_whose_scores_overflow_weigh_nothing(session, dtype, width):
+    """Finite keys whose score leaves Float32 downwards: the first ones, all but one, all (a row of zeros), none."""
+    rng = np.random.default_rng(width)
+    lengths = [60, 60, 20, 60]
+    tables, pages = tables_for(rng, lengths, 16)
+    o = PagedCacheOracle(rng, pages, 1, 16, width, dtype)
+    q = (np.abs(rng.standard_normal((4, 4, width))) + 8).astype(np.float32)
+    low = np.zeros((4, 60), bool)
+    low[0, :23], low[1, :], low[1, 31], low[2] = True, True, False, True
+    for b, n in enumerate(lengths):
+        k = rng.standard_normal((n, 1, width)).astype(np.float32) / 8
+        k[low[b, :n]] = -3e38
+        o.append(0, k, tables, np.full(n, b), np.arange(n))
+    with Held(session) as h:
+        got = attended(h, o, q, tables, lengths)
+    for b, n in enumerate(lengths):
+        seen = ~low[b, :n]
+        k, v = (o.rows(side, tables, b, n)[:, seen] for side in range(2))
+        want, mass, score = attend(q[b], k, v)
+        tol = (np.expm1(2 * (width + 8) * HALF * score) + (n + 16) * 2 * HALF) * mass + 1e-37
+        np.testing.assert_array_less(np.abs(got[b].astype(np.float64) - want), tol, err_msg=f"request {b}")
