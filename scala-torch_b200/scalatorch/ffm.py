@@ -641,7 +641,8 @@ class B200Session:
                 raise IllegalStateException("validate", 6, "tensor was released")
             require(t.dtype == dtype and not t.transposed_weight, "operation takes Float32 rows and int32 indices")
             require(shape is None or t.shape == shape, f"shape mismatch: {t.shape} where {shape} is needed")
-            require(dtype == STB_F32 or t.row_stride == 0, "operation takes packed indices, not a view of columns")
+            require(t.row_stride == 0 or dtype == STB_F32 and len(t.shape) > 1,
+                    "operation takes packed indices, weights and biases, not a view of columns")
         raise IllegalArgumentException("operands do not fit together")
 
     def _outs(self, *shapes):
@@ -681,8 +682,8 @@ class B200Session:
                     and positions.shape == (rows,) and positions.row_stride == 0
                     and yq.session is self and yq._alive[0] and yq.dtype == STB_F32 and yq.shape == qs and not yq.transposed_weight
                     and yk.session is self and yk._alive[0] and yk.dtype == STB_F32 and yk.shape == ks and not yk.transposed_weight
-                    and (qw is None or qw.session is self and qw._alive[0] and qw.dtype == STB_F32 and qw.shape == (width,))
-                    and (kw is None or kw.session is self and kw._alive[0] and kw.dtype == STB_F32 and kw.shape == (width,))):
+                    and (qw is None or qw.session is self and qw._alive[0] and qw.dtype == STB_F32 and qw.shape == (width,) and qw.row_stride == 0)
+                    and (kw is None or kw.session is self and kw._alive[0] and kw.dtype == STB_F32 and kw.shape == (width,) and kw.row_stride == 0)):
                 self._refuse((query, STB_F32, None), (key, STB_F32, None), (positions, STB_I32, (rows,)), (yq, STB_F32, qs), (yk, STB_F32, ks),
                              *[(w, STB_F32, (width,)) for w in (qw, kw) if w is not None])
             kv_heads = ks[1]
@@ -719,7 +720,7 @@ class B200Session:
                 and x.row_stride == 0 and weight.session is self and weight._alive[0] and weight.transposed_weight
                 and weight.shape == (K, N) and rows.session is self and rows._alive[0] and rows.dtype == STB_I32
                 and rows.shape == (M,) and rows.row_stride == 0
-                and (bias is None or bias.session is self and bias._alive[0] and bias.dtype == STB_F32 and bias.shape == (N,))):
+                and (bias is None or bias.session is self and bias._alive[0] and bias.dtype == STB_F32 and bias.shape == (N,) and bias.row_stride == 0)):
             self._validate(x)
             self._validate(weight)
             require(weight.transposed_weight, "weight must be a resident (out,in) weight")

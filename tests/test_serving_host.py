@@ -120,3 +120,18 @@ def test_the_oracles_known_answers():
     y, _, _ = attend(np.array([[2.0, 0.0]]), np.array([[[0.0, 1.0], [0.0, 5.0]]]), np.array([[[1.0, 2.0], [3.0, 4.0]]]))
     np.testing.assert_allclose(y, [[2.0, 3.0]])
     assert np.all(attend(np.ones((1, 2)), np.zeros((1, 0, 2)), np.zeros((1, 0, 2)))[0] == 0)
+
+
+def test_a_column_is_no_packed_vector(s):
+    """One column of a matrix has a weight's or a bias's shape, but its elements lie apart."""
+    q, k, p = t(s, (3, 4, 64)), t(s, (3, 2, 64)), t(s, (3,), STB_I32)
+    w, apart = t(s, (64,)), s.columns(t(s, (64, 5)), 2, ())
+    assert apart.shape == (64,) and apart.row_stride == 5
+    for weights in ((apart, w), (w, apart)):
+        with pytest.raises(ffm.IllegalArgumentException, match="packed"):
+            s.qk_norm_rope(q, k, *weights, p, out=(q, k))
+    pool = s.adapter_pool(t(s, (3, 8, 32)), t(s, (3, 48, 8)), t(s, (3,), STB_I32), t(s, (3,)))
+    x, rows, y = t(s, (5, 32)), t(s, (5,), STB_I32), t(s, (5, 48))
+    bias = s.columns(t(s, (48, 9)), 0, ())
+    with pytest.raises(ffm.IllegalArgumentException, match="packed"):
+        s.linear_adapted(x, s.as_weight(t(s, (48, 32), STB_BF16)), pool, rows, bias, out=y)
