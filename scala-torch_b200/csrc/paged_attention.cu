@@ -9,9 +9,9 @@
 // Float32 accuracy kept by splitting the Float32 side into terms that the products take exactly:
 //   * BF16 cache: q and p in three BF16 terms (24 bits);
 //   * F16 and E4M3 cache (E4M3 widens to F16 exactly): two F16 terms (22 bits).  q after a power of two that puts the largest
-//     of a head at 2^12 (22 bits of that largest one); weights after one per head that follows the tiles' largest (2^7 ..
-//     2^15), the second term's times 2^12, in a sum of its own.  That keeps 22 bits of every weight down to 2^-21 of its
-//     tile's largest; lower ones beside it are added in Float32, key by key;
+//     of a head at 2^12 (22 bits of that largest one); weights after one per head that follows the tiles' largest, the
+//     second term's times 2^12, in a sum of its own.  Weights 2^26 times lower than their tile's largest are added in
+//     Float32, key by key, where the result is not large enough that their last bits cannot count;
 //   * F32 cache: both sides in two TF32 terms (q and p 23 bits, keys 22, values 21), without the product of the lower ones.
 // The tensor core truncates its sums, so chains are kept short (at most 8 products) and joined by Float32 additions.
 //
@@ -132,9 +132,13 @@ constexpr int ROUND_TILES = 32;
 constexpr int BLOCK_PIECES = 20800;  // floats of a block's pieces, at most: (2 + warps) of 8 heads x (width + 4)
 constexpr int MAX_BATCH = 1024;      // requests of one launch (their prefix sums lie in shared memory)
 constexpr float LAZY = 8.0f;         // a maximum moves only when a score passes it by 2^8
-// F16 weights: the tile's largest is put at 2^7 (and may grow to 2^15 before that moves), the rest behind the first term's 11
-// bits times 2^12.  From 2^-14 on, F16's smallest with all its bits, both terms together keep 22.
-constexpr float P_SHIFT = 7.0f, P_LOW = -14.0f, P_REST = 4096.0f;  // log2, log2, factor
+// F16 weights, in log2: a head's are put around P_SHIFT and stay there while none passes P_TOP and none is below P_LOW.  The rest
+// behind the first term's 11 bits goes times 2^12: both terms together keep 22 bits from F16's smallest normal value on, 2^-14,
+// 19 from P_LOW on, and are off by 2^-37 at most below.  Where that may count in a result (what the item has added up so far
+// is not 2^22 times what a tile could lose), such weights are added in Float32.  Scores of a standard deviation of 1, 3 and 5
+// nats, 0.5 GiB of E4M3 of width 128: 112, 124 and 177 us; all low weights in Float32 113, 140 and 388; a second pass of
+// the tensor cores for them 131, 139 and 176 (registers).
+constexpr float P_SHIFT = 8.0f, P_TOP = 15.0f, P_LOW = -18.0f, P_REST = 4096.0f;
 
 template <int DTYPE, int WP>
 struct Shape {
@@ -146,9 +150,10 @@ struct Shape {
   static constexpr int TILE = 2 * TK * ROW;       // keys and values of a tile
   // Warps and stages that fill about 192 KB.  With enough arithmetic per byte more warps are worth more than a second stage
   // for each: what one waits for, the others compute over.  0.5 GiB of cache, 82 us at the copy rate: E4M3 of width 64
-  // eight warps 165 us, twelve 136 (143 with the weights' range, below); F32 of width 128 six warps of two stages 119, twelve of one 102; F32 of width 256 three
-  // of two 268, six of one 178.  BF16 and F16 of width 64 and 128 take 93 to 97 with eight.  E4M3 of width 128 has too few
-  // registers with twelve: 64 requests of 3000 tokens, 8 kv heads of it, 113 us with twelve, 91 with eleven.
+  // eight warps 165 us, twelve 136; F32 of width 128 six warps of two stages 119, twelve of one 102; F32 of width 256 three of
+  // two 268, six of one 178 (each before the weights' range below and the cut TF32 terms: 143, 100 and 174 now).  BF16 and
+  // F16 of width 64 and 128 take 93 to 97 with eight.  E4M3 of width 128 spills registers with twelve (131 us), not with
+  // eleven (112); with eight, of twice the registers, it takes 120.
   static constexpr int WARPS = TILE <= 8192 ? (DTYPE == STB_E4M3 && ROW <= 128 ? (WP == 128 ? 11 : 12) : 8) : (DTYPE == STB_F32 && ROW == 512 ? 12 : 6);
   static constexpr int STAGES = 196608 / (WARPS * TILE) < 6 ? 196608 / (WARPS * TILE) : 6;
   static constexpr int META = 16 + (DTYPE == STB_E4M3 ? TK * 8 : 0);  // per stage: valid mask, scales of keys and values
@@ -573,7 +578,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
   auto dim_of = [&](int i, int k) { return SCALED ? i * 16 + 2 * g + k : i * 16 + g + 8 * k; };
 
   // What takes the weights' scale from a result; E4M3's own can pass Float32's range at either end: its root, applied twice.
-  auto back = [](float shift) { return SCALED ? exp2f(0.5f * (shift - P_SHIFT)) : (HALF ? 0x1p-7f : 1.0f); };
+  auto back = [](float shift) { return SCALED ? exp2f(0.5f * (shift - P_SHIFT)) : (HALF ? exp2f(-P_SHIFT) : 1.0f); };
 
   // The result of an item's tiles that this warp has seen: all of them to y; a part to the block's pieces (a first
   // part, while the ring is in use) or over the warp's own ring (a last part).
@@ -705,7 +710,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
             sc[b][2 * k] = sc[b][2 * k + 1] = sw[SCALED ? b : 0][2 * k] = sw[SCALED ? b : 0][2 * k + 1] = -INFINITY;
     }
     // What is rare, by one vote: a score that passed its maximum by far, or (F16 weights) one out of the weights' range.
-    auto weighed = [&](int b, int i) { return SCALED ? sw[b][i] : sc[b][i]; };  // log2 of the weight
+    auto weighed = [&](int b, int i) -> float & { return SCALED ? sw[SCALED ? b : 0][i] : sc[b][i]; };  // log2 of the weight
     auto is_rare = [&](bool masked_too) {
       bool rare = false;
 #pragma unroll
@@ -714,7 +719,7 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
         for (int i = 0; i < 4; i++) {
           if (SCALED || !HALF) rare |= sc[b][i] > m1[i & 1] + LAZY;
           if (HALF) {
-            rare |= weighed(b, i) > base[i & 1] + (P_SHIFT + LAZY);
+            rare |= weighed(b, i) > base[i & 1] + P_TOP;
             if (masked_too) rare |= weighed(b, i) < base[i & 1] + P_LOW;
             else rare |= (weighed(b, i) < base[i & 1] + P_LOW) & (weighed(b, i) != -INFINITY);
           }
@@ -725,17 +730,24 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       if (!HALF || is_rare(false)) {  // move the heads' maxima, and the weights' base to this tile's
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-          float t1 = -INFINITY, t2 = -INFINITY;  // of this tile
+          float t1 = -INFINITY, t2 = -INFINITY, least = INFINITY;  // of this tile
 #pragma unroll
-          for (int b = 0; b < MB; b++) {
-            t1 = fmaxf(t1, fmaxf(sc[b][j], sc[b][2 + j]));
-            if (SCALED) t2 = fmaxf(t2, fmaxf(sw[b][j], sw[b][2 + j]));
-          }
+          for (int b = 0; b < MB; b++)
+#pragma unroll
+            for (int i = j; i < 4; i += 2) {
+              t1 = fmaxf(t1, sc[b][i]);
+              if (HALF) {
+                if (SCALED) t2 = fmaxf(t2, sw[b][i]);
+                if (weighed(b, i) != -INFINITY) least = fminf(least, weighed(b, i));
+              }
+            }
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) {
             t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, off));
             if (SCALED) t2 = fmaxf(t2, __shfl_xor_sync(0xffffffffu, t2, off));
+            if (HALF) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, off));
           }
+          if (!SCALED) t2 = t1;
           const float n1 = fmaxf(m1[j], t1), n2 = SCALED ? fmaxf(m2[j], t2) : n1;
           const float f1 = n1 == m1[j] ? 1.0f : pow2(m1[j] - n1), f2 = n2 == m2[j] ? 1.0f : pow2(m2[j] - n2);
           sum[j] *= f1;
@@ -746,29 +758,55 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
           }
           m1[j] = n1;
           m2[j] = n2;
-          if (HALF) {
-            if (!SCALED) t2 = t1;
-            if (t2 != -INFINITY) {
-              base[j] = n2 - (P_SHIFT + fminf(100.0f, ceilf(n2 - t2)));
-              down[j] = pow2(base[j] - n2 + P_SHIFT);
-            }
+          if (HALF && t2 != -INFINITY) {
+            if (t2 > base[j] + P_TOP || least < base[j] + P_LOW) base[j] = fmaxf(t2, n2 - 100.0f) - P_SHIFT;
+            down[j] = pow2(base[j] - n2 + P_SHIFT);
           }
         }
-        if constexpr (HALF) {  // weights out of the range even so: in Float32, key by key
-          float apart[MB][4];
+        if constexpr (HALF) {
+          auto is_low = [&](int b, int i) { return (weighed(b, i) < base[i & 1] + P_LOW) & (weighed(b, i) != -INFINITY); };
           bool some = false;
 #pragma unroll
           for (int b = 0; b < MB; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const bool low = (weighed(b, i) < base[i & 1] + P_LOW) & (weighed(b, i) != -INFINITY);
-              apart[b][i] = low ? pow2(weighed(b, i) - base[i & 1]) : 0.0f;
-              if (!SCALED) sum[i & 1] += low ? pow2(sc[b][i] - m1[i & 1]) : 0.0f;
-              if (SCALED) sw[b][i] = low ? -INFINITY : sw[b][i];
-              else sc[b][i] = low ? -INFINITY : sc[b][i];
-              some |= apart[b][i] > 0.0f;
+            for (int i = 0; i < 4; i++) some |= is_low(b, i);
+          if (__any_sync(0xffffffffu, some)) {  // would 2^-37 of all values be 2^-22 of what some result holds already?
+            float widest = 448.0f;
+            if (!SCALED) {
+              __half2 top = __float2half2_rn(0.0f);
+#pragma unroll 1
+              for (int n = 0; n < MB * S::PAIRS; n++) {
+                uint32_t v[4];
+                const int chunk = n / MB * 2 + (lane >> 4);
+                load_matrix4(v, chunk_at<S::ROW>(values, n % MB * 16 + (lane & 15), chunk < row_chunks ? chunk : 0));
+#pragma unroll
+                for (int k = 0; k < 4; k++) top = __hmax2(top, __habs2(*reinterpret_cast<const __half2 *>(&v[k])));
+              }
+              const float mine = __half2float(__hmax(__low2half(top), __high2half(top)));
+              widest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mine)));
             }
-          if (__any_sync(0xffffffffu, some)) {
+            float least[2] = {INFINITY, INFINITY};
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+#pragma unroll
+              for (int k = 0; k < 2; k++)
+                if ((SCALED ? i : 2 * i + k) < row_chunks) {
+#pragma unroll
+                  for (int j = 0; j < 2; j++) least[j] = fminf(least[j], fabsf(o[i][j + 2 * k]));
+                }
+            some = (least[0] < down[0] * widest * (TK * 0x1p-15f)) | (least[1] < down[1] * widest * (TK * 0x1p-15f));
+          }
+          if (__any_sync(0xffffffffu, some)) {  // in Float32, key by key
+            float apart[MB][4];
+#pragma unroll
+            for (int b = 0; b < MB; b++)
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                const bool low = is_low(b, i);
+                apart[b][i] = low ? pow2(weighed(b, i) - base[i & 1]) : 0.0f;
+                if (!SCALED) sum[i & 1] += low ? pow2(sc[b][i] - m1[i & 1]) : 0.0f;
+                weighed(b, i) = low ? -INFINITY : weighed(b, i);
+              }
 #pragma unroll 1
             for (int key = 0; key < TK; key++) {
               float x[2];

@@ -273,6 +273,28 @@ def test_weights_of_every_size_in_one_cache(session, dtype):
         np.testing.assert_array_less(np.abs(got[b] - want), (40 + 16 * score.max()) * HALF * mass + 1e-37)
 
 
+@pytest.mark.parametrize("dtype,width", [("F32", 64), ("BF16", 64), ("F16", 64), ("F16", 128), ("E4M3", 64), ("E4M3", 128), ("E4M3", 256), ("E4M3", 36)])
+@pytest.mark.parametrize("spread", [3, 6, 15])
+def test_scores_of_any_spread(session, dtype, width, spread):
+    """Scores with a standard deviation of `spread` nats: tiles whose weights span much more than F16's exponents; some
+    values zero, so that only low weights make a dimension.  Bounds as above."""
+    rng = np.random.default_rng(spread + width)
+    lengths = [33, 700, 3001, 1]
+    tables, pages = tables_for(rng, lengths, 16)
+    o = PagedCacheOracle(rng, pages, 2, 16, width, dtype)
+    q = (spread * rng.standard_normal((4, 10, width))).astype(np.float32)
+    for b, n in enumerate(lengths):
+        v = rng.standard_normal((n, 2, width)).astype(np.float32)
+        v[rng.random(n) < 0.5, :, :width // 2] = 0.0
+        o.append(1, v, tables, np.full(n, b), np.arange(n))
+    with Held(session) as h:
+        got = attended(h, o, q, tables, lengths)
+    check_rows(got, o, q, tables, lengths)
+    for b, n in enumerate(lengths):
+        want, _, score = attend(q[b], o.rows(0, tables, b, n), o.rows(1, tables, b, n))
+        assert np.linalg.norm(got[b] - want) <= (2e-6 + 16 * HALF * score.max()) * np.linalg.norm(want)
+
+
 # ------------------------------------------------------------------ scores of minus infinity
 
 
