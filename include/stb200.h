@@ -160,7 +160,9 @@ typedef struct stb_adapter_pool {
 /* y[m] = x[m].W^T + scales[t] * (x[m].A_t^T).B_t^T + bias with t = rows[m], int32 [M] on the device: the slot
  * of row m, negative for a row without an adapter.  Rows may name slots in any order and repeat them; a
  * slot's factors are read once for up to 16 of its rows, 64 rows of the call at a time.  The shared product is
- * stb_linear's (or, for one or two rows, the same sum in another order); the thin products accumulate in Float32.  A slot >= pool->slots leaves its row without an adapter and
+ * stb_linear's (or, for one or two rows, the same sum in another order); the thin products take x, their own first
+ * result and Float32 factors with 22 bits at least (all of them for one or two rows) and accumulate in Float32.  A NaN
+ * stays one; an infinity gives infinities or NaNs.  A slot >= pool->slots leaves its row without an adapter and
  * fails the next stb_sync / stb_download.  y may not overlap an input.  The session's scratch holds the thin products
  * of one call at a time and grows with the largest: make a call of the size before capturing one (STB_ERR_STATE
  * otherwise), and replay graphs that captured it on one stream at a time. */
@@ -279,11 +281,18 @@ int stb_op_paged_read(stb_session *s, const stb_paged_cache *cache, uint64_t tab
  * rows q_row apart; head h reads key/value head h / (heads / kv_heads)) against the first lengths[b] tokens of
  * tables[b], scores scaled by 1 / sqrt(width), softmax in Float32 with the running maximum.  lengths: int32
  * [batch] on the device, the new token's own key included (append first).  A length of zero or below gives a
- * row of zeros; one behind the table is cut to it.  The cache is split over its length among all SMs and the
- * parts joined in a fixed order: the same call gives the same bits.  Weights of up to 2^8 times the largest values
- * are summed before the division, and have to stay finite; an infinite value makes its dimension NaN.  The session's one
- * workspace (13.3 MB of its budget) serves all calls, in stream order: replay graphs that captured this call on one
- * stream at a time.  y may not overlap q or the cache. */
+ * row of zeros; one behind the table is cut to it.  The cache is split over its length among all SMs and the parts
+ * joined in a fixed order: the same call gives the same bits.
+ * Where the cache's rows are whole 16-byte pieces of at most 256 elements, the products take these bits: BF16 caches 24 of
+ * queries and weights; F16 and E4M3 22 of a head's largest query element and of weights down to 2^-22 of the largest
+ * around them, 19 down to 2^-26, and what lower ones lose is below 2^-22 of the result; F32 22 of queries, weights and
+ * keys, 21 of values.  Elsewhere Float32.
+ * A key whose score is -infinity weighs nothing, and a request of such keys alone gives zeros.  A NaN of the query makes its
+ * head NaN, one of a key its request's heads on that key/value head, one of a value its dimension; an infinite value makes
+ * its dimension infinite or NaN, an infinite element of query or key its scores.  Weights of up to 2^8 times the largest
+ * values are summed before the division, and have to stay finite.
+ * The session's one workspace (13.3 MB of its budget) serves all calls, in stream order: replay graphs that captured this
+ * call on one stream at a time.  y may not overlap q or the cache. */
 int stb_op_paged_attention(stb_session *s, const stb_paged_cache *cache, uint64_t q, int64_t q_row, int heads,
                            uint64_t tables, int batch, int blocks, uint64_t lengths, uint64_t y, int64_t y_row);
 

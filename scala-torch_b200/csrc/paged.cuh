@@ -7,10 +7,16 @@
 
 namespace stb {
 
-// The kernels of a batch of several requests start while the one before drains: each waits for it before it reads anything,
-// weights too, and lets the next one start only then, so whoever starts early finds all that came before its own
-// predecessor done.  One after another in a stream, norm and rotation of one token 3.0 -> 2.7 us, a cache write 2.2 -> 1.7,
-// attention over 33 tokens 5.9 -> 5.1; from Python 8.2 -> 5.3 us per call of the last.
+// The kernels of a batch of several requests start while the one before drains.  The rule they keep: before its wait a kernel
+// reads only what was complete before its predecessor started, writes nothing that one reads or writes, and every block
+// waits before it exits -- so a kernel that is done means that all before it are.  Norm and rotation, the cache's kernels,
+// attention and pool_small_kernel wait first, read then, and let the next one start only then.  Two differ (adapter_pool.cu):
+// pool_up_kernel lets the next one start at once and reads the rows' slots, ranks, scales and B before its wait: they were
+// complete when pool_down_kernel, having waited, let the next one start.  pool_down_kernel behind a vector product (`behind`)
+// reads and writes at once and waits at its end: that product was launched plainly, after all before it, and touches
+// neither thin nor what the plan reads.
+// One after another in a stream, norm and rotation of one token 3.0 -> 2.7 us, a cache write 2.2 -> 1.7, attention over 33
+// tokens 5.9 -> 5.1; from Python 8.2 -> 5.3 us per call of the last.
 
 // A cache of the caller's (stb_paged_cache), with the page table of the call.
 struct PagedView {

@@ -2,11 +2,11 @@
 //   y[b, h] = sum_j softmax_j(q[b, h] . k_j / sqrt(width)) v_j,   j < lengths[b],  h on kv head h / group,
 // zeros where lengths[b] <= 0.
 //
-// What bounds it: every cached byte is read once, 4 * group flops per element: HBM, as long as the arithmetic keeps
-// out of the way.  With 8 query heads on a kv head, Float32 FMAs would take 8 flops per BF16 byte (52 TFLOP/s at the
-// copy rate of 6.5 TB/s, near the SM's FP32 peak) and twice that for E4M3, so both products run on the tensor
-// cores (mma.sync, fed by each warp's own ring: with 8 columns there is no reuse that larger tiles could find), with
-// Float32 accuracy kept by splitting the Float32 side into terms that the products take exactly:
+// What bounds it: every cached byte is read once per 8 query heads of its kv head (an item takes 8 at a time), with 4 flops
+// per element and head: HBM, as long as the arithmetic keeps out of the way.  With 8 query heads on a kv head, Float32 FMAs
+// would take 8 flops per BF16 byte (52 TFLOP/s at the copy rate of 6.5 TB/s, near the SM's FP32 peak) and twice that for
+// E4M3, so both products run on the tensor cores (mma.sync, fed by each warp's own ring: with 8 columns there is no reuse that
+// larger tiles could find), with Float32 accuracy kept by splitting the Float32 side into terms that the products take exactly:
 //   * BF16 cache: q and p in three BF16 terms (24 bits);
 //   * F16 and E4M3 cache (E4M3 widens to F16 exactly): two F16 terms (22 bits).  q after a power of two that puts the largest
 //     of a head at 2^12 (22 bits of that largest one); weights after one per head that follows the tiles' largest, the
@@ -25,9 +25,9 @@
 // arrive, always in the order of the keys.  Few short items go to one block each, many to one warp each (no join at all),
 // many of medium length to one block each as the line has them (none between blocks).
 //
-// Measured: 24 requests of up to 16384 BF16 tokens (8 kv heads of 128, 64 heads) 157 us = 6.1 TB/s, 0.93 of the copy rate;
-// one request of 60001 E4M3 tokens 36 us = 3.4 TB/s (its stream runs at 6.4; the rest is the start and two joins); 8 requests of up
-// to 544 E4M3 tokens 11.4 us; one of 33 tokens 5.1 us.
+// Measured in a captured graph: 24 requests of up to 16384 BF16 tokens (8 kv heads of 128, 64 heads) 156 us = 6.1 TB/s, 0.94 of
+// the copy rate; one request of 60001 E4M3 tokens 37 us = 3.4 TB/s (its stream runs at 6.2; the rest is the start and two joins);
+// 8 requests of up to 544 E4M3 tokens 11.4 us; one of 33 tokens 5.1 us.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -60,7 +60,7 @@ __device__ __forceinline__ int attend_length(const PagedView &c, const AttendArg
 // ------------------------------------------------------------------ any width, alignment and type
 
 // One block per (request, query head): its warps take keys in turn, a lane every 32nd dimension, Float32 FMAs.
-// For caches whose rows are no multiple of 16 bytes or wider than 256.
+// For caches whose rows are no multiple of 16 bytes or wider than 256: the cache goes through once per query head.
 template <int DTYPE>
 __global__ void __launch_bounds__(256) paged_attention_any_kernel(const PagedView c, const AttendArgs a) {
   constexpr int W = 8, D = 16;  // warps; dimensions of a lane (width <= 512)
@@ -127,7 +127,8 @@ constexpr int WHOLE_TILES = 8;       // most tiles of an item that one warp take
 // Most tiles of an item that one block takes alone where there are more items than blocks, and twice as many where there
 // are half as many again: the blocks' stretches differ by up to an item, and none is joined between blocks.  256 items of
 // up to 300 BF16 tokens 21.7 -> 15.6 us, 400 of up to 500 22.3 -> 17.5; 160 of 500 21.6 -> 19.6, of 1000 (63 tiles) 29.6
-// against 32.8; 400 of 1000 51 -> 47.
+// against 32.8; 400 of 1000 51 -> 47.  F32 tiles of 16 keys reach the limit at half as many tokens; 160 items of 500 of them
+// lose, 33.3 -> 37.5: some blocks take two items and most one.
 constexpr int ROUND_TILES = 32;
 constexpr int BLOCK_PIECES = 20800;  // floats of a block's pieces, at most: (2 + warps) of 8 heads x (width + 4)
 constexpr int MAX_BATCH = 1024;      // requests of one launch (their prefix sums lie in shared memory)
