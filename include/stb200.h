@@ -161,8 +161,8 @@ typedef struct stb_adapter_pool {
  * of row m, negative for a row without an adapter.  Rows may name slots in any order and repeat them; a
  * slot's factors are read once for up to 16 of its rows, 64 rows of the call at a time.  The shared product is
  * stb_linear's (or, for one or two rows, the same sum in another order); the thin products take x, their own first
- * result and Float32 factors with 22 bits at least (all of them for one or two rows) and accumulate in Float32.  A NaN
- * stays one; an infinity gives infinities or NaNs.  A slot >= pool->slots leaves its row without an adapter and
+ * result and Float32 factors with 22 bits at least (all of them for one or two rows with small factors) and accumulate in
+ * Float32.  A NaN stays one; an infinity gives infinities or NaNs.  A slot >= pool->slots leaves its row without an adapter and
  * fails the next stb_sync / stb_download.  y may not overlap an input.  The session's scratch holds the thin products
  * of one call at a time and grows with the largest: make a call of the size before capturing one (STB_ERR_STATE
  * otherwise), and replay graphs that captured it on one stream at a time. */
