@@ -10,8 +10,8 @@
 //   * BF16 cache: q and p in three BF16 terms (24 bits);
 //   * F16 and E4M3 cache (E4M3 widens to F16 exactly): two F16 terms (22 bits).  q after a power of two that puts the largest
 //     of a head at 2^12 (22 bits of that largest one); weights after one per head that follows the tiles' largest, the
-//     second term's times 2^12, in a sum of its own.  Weights 2^26 times lower than their tile's largest are added in
-//     Float32, key by key, where the result is not large enough that their last bits cannot count;
+//     second term's times 2^12, in a sum of its own.  What both miss of weights 2^26 times lower than their tile's largest
+//     is added in Float32, key by key, where the result is not large enough that those bits cannot count;
 //   * F32 cache: both sides in two TF32 terms (q and p 23 bits, keys 22, values 21), without the product of the lower ones.
 // The tensor core truncates its sums, so chains are kept short (at most 8 products) and joined by Float32 additions.
 //
@@ -26,8 +26,8 @@
 // many of medium length to one block each as the line has them (none between blocks).
 //
 // Measured in a captured graph: 24 requests of up to 16384 BF16 tokens (8 kv heads of 128, 64 heads) 156 us = 6.1 TB/s, 0.94 of
-// the copy rate; one request of 60001 E4M3 tokens 37 us = 3.4 TB/s (its stream runs at 6.2; the rest is the start and two joins);
-// 8 requests of up to 544 E4M3 tokens 11.4 us; one of 33 tokens 5.1 us.
+// the copy rate; one request of 60001 E4M3 tokens 38 us = 3.3 TB/s (its stream runs at 6.2; the rest is the start and two joins);
+// 8 requests of up to 544 E4M3 tokens 11.6 us; one of 33 tokens 5.0 us.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -135,11 +135,17 @@ constexpr int MAX_BATCH = 1024;      // requests of one launch (their prefix sum
 constexpr float LAZY = 8.0f;         // a maximum moves only when a score passes it by 2^8
 // F16 weights, in log2: a head's are put around P_SHIFT and stay there while none passes P_TOP and none is below P_LOW.  The rest
 // behind the first term's 11 bits goes times 2^12: both terms together keep 22 bits from F16's smallest normal value on, 2^-14,
-// 19 from P_LOW on, and are off by 2^-37 at most below.  Where that may count in a result (what the item has added up so far
-// is not 2^22 times what a tile could lose), such weights are added in Float32.  Scores of a standard deviation of 1, 3 and 5
-// nats, 0.5 GiB of E4M3 of width 128: 112, 124 and 177 us; all low weights in Float32 113, 140 and 388; a second pass of
-// the tensor cores for them 131, 139 and 176 (registers).
+// 19 from P_LOW on, and are off by 2^-37 at most below.  Where that may count in a result (some sum so far is not 2^22 times
+// what a tile could lose), what is missing is added in Float32.  Scores of a standard deviation of 1, 3 and 5 nats, 0.5 GiB of
+// E4M3 of width 128: 109, 115 and 156 us; all low weights in Float32 113, 140 and 388; a second pass of the tensor cores for
+// them 131, 139 and 176 (registers); looked at before the tile's products 112, 124 and 177.
 constexpr float P_SHIFT = 8.0f, P_TOP = 15.0f, P_LOW = -18.0f, P_REST = 4096.0f;
+
+// What two F16 terms miss of a weight.
+__device__ __forceinline__ float missing(float w) {
+  const float rest = w - __half2float(__float2half_rn(w));
+  return rest - __half2float(__float2half_rn(rest * P_REST)) * (1.0f / P_REST);
+}
 
 template <int DTYPE, int WP>
 struct Shape {
@@ -153,9 +159,8 @@ struct Shape {
   // for each: what one waits for, the others compute over.  0.5 GiB of cache, 82 us at the copy rate: E4M3 of width 64
   // eight warps 165 us, twelve 136; F32 of width 128 six warps of two stages 119, twelve of one 102; F32 of width 256 three of
   // two 268, six of one 178 (each before the weights' range below and the cut TF32 terms: 143, 100 and 174 now).  BF16 and
-  // F16 of width 64 and 128 take 93 to 97 with eight.  E4M3 of width 128 spills registers with twelve (131 us), not with
-  // eleven (112); with eight, of twice the registers, it takes 120.
-  static constexpr int WARPS = TILE <= 8192 ? (DTYPE == STB_E4M3 && ROW <= 128 ? (WP == 128 ? 11 : 12) : 8) : (DTYPE == STB_F32 && ROW == 512 ? 12 : 6);
+  // F16 of width 64 and 128 take 93 to 97 with eight, E4M3 of width 128 120 with eight and 109 with twelve.
+  static constexpr int WARPS = TILE <= 8192 ? (DTYPE == STB_E4M3 && ROW <= 128 ? 12 : 8) : (DTYPE == STB_F32 && ROW == 512 ? 12 : 6);
   static constexpr int STAGES = 196608 / (WARPS * TILE) < 6 ? 196608 / (WARPS * TILE) : 6;
   static constexpr int META = 16 + (DTYPE == STB_E4M3 ? TK * 8 : 0);  // per stage: valid mask, scales of keys and values
   static constexpr bool META_SCALES = DTYPE == STB_E4M3;
@@ -727,6 +732,8 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
         }
       return __any_sync(0xffffffffu, rare);  // the same for the whole warp
     };
+    bool low = false;
+    volatile float later[MB * 4];  // in local memory, which only tiles with low weights touch
     if (is_rare(true)) {  // a masked key looks so at first
       if (!HALF || is_rare(false)) {  // move the heads' maxima, and the weights' base to this tile's
 #pragma unroll
@@ -771,72 +778,12 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
           for (int b = 0; b < MB; b++)
 #pragma unroll
             for (int i = 0; i < 4; i++) some |= is_low(b, i);
-          if (__any_sync(0xffffffffu, some)) {  // would 2^-37 of all values be 2^-22 of what some result holds already?
-            float widest = 448.0f;
-            if (!SCALED) {
-              __half2 top = __float2half2_rn(0.0f);
-#pragma unroll 1
-              for (int n = 0; n < MB * S::PAIRS; n++) {
-                uint32_t v[4];
-                const int chunk = n / MB * 2 + (lane >> 4);
-                load_matrix4(v, chunk_at<S::ROW>(values, n % MB * 16 + (lane & 15), chunk < row_chunks ? chunk : 0));
-#pragma unroll
-                for (int k = 0; k < 4; k++) top = __hmax2(top, __habs2(*reinterpret_cast<const __half2 *>(&v[k])));
-              }
-              const float mine = __half2float(__hmax(__low2half(top), __high2half(top)));
-              widest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mine)));
-            }
-            float least[2] = {INFINITY, INFINITY};
-#pragma unroll
-            for (int i = 0; i < NT; i++)
-#pragma unroll
-              for (int k = 0; k < 2; k++)
-                if ((SCALED ? i : 2 * i + k) < row_chunks) {
-#pragma unroll
-                  for (int j = 0; j < 2; j++) least[j] = fminf(least[j], fabsf(o[i][j + 2 * k]));
-                }
-            some = (least[0] < down[0] * widest * (TK * 0x1p-15f)) | (least[1] < down[1] * widest * (TK * 0x1p-15f));
-          }
-          if (__any_sync(0xffffffffu, some)) {  // in Float32, key by key
-            float apart[MB][4];
+          low = __any_sync(0xffffffffu, some);
+          if (low) {
 #pragma unroll
             for (int b = 0; b < MB; b++)
 #pragma unroll
-              for (int i = 0; i < 4; i++) {
-                const bool low = is_low(b, i);
-                apart[b][i] = low ? pow2(weighed(b, i) - base[i & 1]) : 0.0f;
-                if (!SCALED) sum[i & 1] += low ? pow2(sc[b][i] - m1[i & 1]) : 0.0f;
-                weighed(b, i) = low ? -INFINITY : weighed(b, i);
-              }
-#pragma unroll 1
-            for (int key = 0; key < TK; key++) {
-              float x[2];
-#pragma unroll
-              for (int j = 0; j < 2; j++) {
-                x[j] = apart[0][j];
-#pragma unroll
-                for (int i = 1; i < 2 * MB; i++) x[j] = key >> 3 == i ? apart[i >> 1][2 * (i & 1) + j] : x[j];
-                x[j] = __shfl_sync(0xffffffffu, x[j], (key & 7) * 4 + t) * down[j];
-              }
-              if (!__any_sync(0xffffffffu, (x[0] > 0.0f) | (x[1] > 0.0f))) continue;
-#pragma unroll
-              for (int i = 0; i < NT; i++)
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                  float v;
-                  if constexpr (SCALED) {
-                    uint32_t u;
-                    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(u) : "r"(chunk_at<S::ROW>(values, key, i) + 2 * g + k));
-                    v = widen_e4m3x2((uint16_t)u).x;
-                  } else {
-                    uint16_t u;
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(chunk_at<S::ROW>(values, key, 2 * i + k) + 2 * g));
-                    v = widen1<__half>(u);
-                  }
-                  o[i][2 * k] = fmaf(x[0], v, o[i][2 * k]);
-                  o[i][2 * k + 1] = fmaf(x[1], v, o[i][2 * k + 1]);
-                }
-            }
+              for (int i = 0; i < 4; i++) later[b * 4 + i] = is_low(b, i) ? missing(pow2(weighed(b, i) - base[i & 1])) : 0.0f;
           }
         }
       }
@@ -932,6 +879,63 @@ __global__ void __launch_bounds__(Shape<DTYPE, WP>::THREADS, 1) paged_attention_
       }
     }
 
+    if constexpr (HALF) {
+      if (low) {  // would 2^-37 of all values be 2^-22 of some result?
+        float widest = 448.0f;
+        if (!SCALED) {
+          __half2 top = __float2half2_rn(0.0f);
+#pragma unroll 1
+          for (int n = 0; n < MB * S::PAIRS; n++) {
+            uint32_t v[4];
+            const int chunk = n / MB * 2 + (lane >> 4);
+            load_matrix4(v, chunk_at<S::ROW>(values, n % MB * 16 + (lane & 15), chunk < row_chunks ? chunk : 0));
+#pragma unroll
+            for (int k = 0; k < 4; k++) top = __hmax2(top, __habs2(*reinterpret_cast<const __half2 *>(&v[k])));
+          }
+          const float mine = __half2float(__hmax(__low2half(top), __high2half(top)));
+          widest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mine)));
+        }
+        float least[2] = {INFINITY, INFINITY};
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+          for (int k = 0; k < 2; k++)
+            if ((SCALED ? i : 2 * i + k) < row_chunks) {
+#pragma unroll
+              for (int j = 0; j < 2; j++) least[j] = fminf(least[j], fabsf(o[i][j + 2 * k]));
+            }
+        const bool some = (least[0] < down[0] * widest * (TK * 0x1p-15f)) | (least[1] < down[1] * widest * (TK * 0x1p-15f));
+        if (__any_sync(0xffffffffu, some)) {  // what the low weights miss, in Float32, key by key
+#pragma unroll 1
+          for (int key = 0; key < TK; key++) {
+            float x[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+              const float mine = later[2 * (key >> 3) + j];
+              x[j] = __shfl_sync(0xffffffffu, mine, (key & 7) * 4 + t) * down[j];
+            }
+            if (!__any_sync(0xffffffffu, (x[0] != 0.0f) | (x[1] != 0.0f))) continue;
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+#pragma unroll
+              for (int k = 0; k < 2; k++) {
+                float v;
+                if constexpr (SCALED) {
+                  uint32_t u;
+                  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(u) : "r"(chunk_at<S::ROW>(values, key, i) + 2 * g + k));
+                  v = widen_e4m3x2((uint16_t)u).x;
+                } else {
+                  uint16_t u;
+                  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(chunk_at<S::ROW>(values, key, 2 * i + k) + 2 * g));
+                  v = widen1<__half>(u);
+                }
+                o[i][2 * k] = fmaf(x[0], v, o[i][2 * k]);
+                o[i][2 * k + 1] = fmaf(x[1], v, o[i][2 * k + 1]);
+              }
+          }
+        }
+      }
+    }
     const bool ends = use.tile + 1 == use.tiles;
     if (ends || i + 1 == todo) {
       if (!ends) {  // the part goes over the ring
